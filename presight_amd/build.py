@@ -10,8 +10,10 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "_obj")
 LIB = os.path.join(HERE, "libpresight_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc",
-         "-Wno-unused-result", "-I" + CSRC]
+# packed fp32 arithmetic (v_pk_{add,mul,fma}_f32) is off: some of its forms have given wrong results on this part now and then, and
+# the optimizer makes them from ordinary scalar code (the host pass does not know the feature and says so: harmless)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Xclang", "-target-feature", "-Xclang",
+         "-packed-fp32-ops", "-Wno-unused-result", "-I" + CSRC]
 
 
 def _sources():
@@ -19,7 +21,9 @@ def _sources():
 
 
 def _headers_mtime():
-    return max(os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC) if f.endswith(".hpp"))
+    """newest of the headers and of this file (the flags): an object older than it is compiled again"""
+    return max([os.path.getmtime(os.path.abspath(__file__))]
+               + [os.path.getmtime(os.path.join(CSRC, f)) for f in os.listdir(CSRC) if f.endswith(".hpp")])
 
 
 def _compile(src):

@@ -57,13 +57,15 @@ __device__ __forceinline__ void sh4(float x, float y, float z, float (&o)[16]) {
   o[15] = 0.5900435899266435f * x * (xx - 3.0f * yy);
 }
 
-// argmin_k ||p - c_k||_2 (first minimum wins, like torch.argmin)
+// argmin_k ||p - c_k||_2 (first minimum wins, like torch.argmin).  Which operations are fused is written out: a point between two
+// centroids must not change sides with the compiler's choice.
 __device__ __forceinline__ int nearest_centroid(float px, float py, float pz, const float* __restrict__ c, int K) {
+#pragma clang fp contract(off)
   int best = 0;
   float bd = 3.4e38f;
   for (int k = 0; k < K; ++k) {
     const float dx = px - c[k * 3], dy = py - c[k * 3 + 1], dz = pz - c[k * 3 + 2];
-    const float d = dx * dx + dy * dy + dz * dz;
+    const float d = fmaf(dy, dy, dx * dx) + dz * dz;
     if (d < bd) {
       bd = d;
       best = k;

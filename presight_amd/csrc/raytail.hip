@@ -76,8 +76,9 @@ __global__ __launch_bounds__(256) void ray_dsigma_bwd_kernel(const float* __rest
   const float* e = ebins + ray * (S + 1);
   float gr = 0.0f;
   if (ok && rgb_s != nullptr && d_rgb != nullptr) {
+#pragma clang fp contract(off)  // (as composite_bwd_w_kernel has it)
     const float* pr = rgb_s + (ray * S + s) * 3;
-    gr += pr[0] * d_rgb[ray * 3] + pr[1] * d_rgb[ray * 3 + 1] + pr[2] * d_rgb[ray * 3 + 2];
+    gr += fmaf(pr[0], d_rgb[ray * 3], pr[1] * d_rgb[ray * 3 + 1]) + pr[2] * d_rgb[ray * 3 + 2];
   }
   float ga = d_acc ? d_acc[ray] : 0.0f;
   if (d_acc2 != nullptr) ga = d_acc ? ga + d_acc2[ray] : d_acc2[ray];

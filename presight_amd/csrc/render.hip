@@ -21,6 +21,7 @@ constexpr int kMaxCh = 4;  // up to 256 samples per ray
 __device__ __forceinline__ float spacing_fn(float x, float thr) { return x < thr ? x / (2.0f * thr) : 1.0f - 1.0f / (2.0f * x / thr); }
 __device__ __forceinline__ float spacing_inv(float x, float thr) { return x < 0.5f ? x * (2.0f * thr) : thr / (2.0f - 2.0f * x); }
 __device__ __forceinline__ float s_to_euclid(float s, float s_near, float s_far, float thr) {
+#pragma clang fp contract(off)  // both products are rounded, as torch does: the compiler would be free to fuse either
   return spacing_inv(s * s_far + (1.0f - s) * s_near, thr);
 }
 using ps::nan_to_num;
@@ -30,6 +31,9 @@ __global__ void generate_rays_kernel(const int64_t* __restrict__ ray_indices, co
                                      const float* __restrict__ fx, const float* __restrict__ fy, const float* __restrict__ cx,
                                      const float* __restrict__ cy, int64_t R, float* __restrict__ origins,
                                      float* __restrict__ dirs, float* __restrict__ pixel_area, float* __restrict__ dir_norm) {
+// Which products are fused with which sums is written out, pixel by pixel: everything behind this kernel hangs on the last bit of a
+// direction, which must not change with the compiler's choice.
+#pragma clang fp contract(off)
   const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
   if (i >= R) return;
   const int64_t cam = ray_indices[i * 3 + 0];
@@ -43,23 +47,33 @@ __global__ void generate_rays_kernel(const int64_t* __restrict__ ray_indices, co
   float n0 = 0.f;
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    float v[3];
+    float v[3], sq;
+    if (k == 0) {
+      v[0] = fmaf(py[k], M[1], px[k] * M[0]) - M[2];
+      v[1] = fmaf(px[k], M[4], py[k] * M[5]) - M[6];
+      v[2] = (px[k] * M[8] + py[k] * M[9]) - M[10];
+      sq = fmaf(v[2], v[2], v[0] * v[0] + v[1] * v[1]);
+    } else {
 #pragma unroll
-    for (int r = 0; r < 3; ++r) v[r] = px[k] * M[r * 4 + 0] + py[k] * M[r * 4 + 1] + (-1.0f) * M[r * 4 + 2];
-    float nrm = sqrtf(v[0] * v[0] + v[1] * v[1] + v[2] * v[2]);
+      for (int r = 0; r < 3; ++r)
+        v[r] = (k == 1 ? fmaf(px[k], M[r * 4], py[k] * M[r * 4 + 1]) : fmaf(py[k], M[r * 4 + 1], px[k] * M[r * 4])) - M[r * 4 + 2];
+      sq = fmaf(v[1], v[1], v[0] * v[0]) + v[2] * v[2];
+    }
+    float nrm = sqrtf(sq);
     nrm = fmaxf(nrm, 1e-8f);
     if (k == 0) n0 = nrm;
 #pragma unroll
     for (int r = 0; r < 3; ++r) d[k][r] = v[r] / nrm;
   }
-  float dx = 0.f, dy = 0.f;
+  float ex[3], ey[3];
 #pragma unroll
   for (int r = 0; r < 3; ++r) {
-    dx += (d[0][r] - d[1][r]) * (d[0][r] - d[1][r]);
-    dy += (d[0][r] - d[2][r]) * (d[0][r] - d[2][r]);
+    ex[r] = d[0][r] - d[1][r];
+    ey[r] = d[0][r] - d[2][r];
     origins[i * 3 + r] = M[r * 4 + 3];
     dirs[i * 3 + r] = d[0][r];
   }
+  const float dx = fmaf(ex[1], ex[1], ex[0] * ex[0]) + ex[2] * ex[2], dy = fmaf(ey[1], ey[1], ey[0] * ey[0]) + ey[2] * ey[2];
   pixel_area[i] = sqrtf(dx) * sqrtf(dy);
   if (dir_norm) dir_norm[i] = n0;
 }
@@ -666,14 +680,20 @@ __global__ __launch_bounds__(256) void composite_bwd_w_kernel(const float* __res
     const bool ok = sr < S;
     float gr = v[0];
     if (ok && rgb_s != nullptr && d_rgb != nullptr) {
+#pragma clang fp contract(off)  // (which of the three products is fused is written out: d(density) of a saturated ray cancels to these bits)
       const float* pr = rgb_s + (ray * S + sr) * 3;
-      gr += pr[0] * d_rgb[ray * 3] + pr[1] * d_rgb[ray * 3 + 1] + pr[2] * d_rgb[ray * 3 + 2];
+      gr += fmaf(pr[0], d_rgb[ray * 3], pr[1] * d_rgb[ray * 3 + 1]) + pr[2] * d_rgb[ray * 3 + 2];
     }
     const float ws = ok ? w[sr] : 0.0f;
     const float mid = ok ? (e[sr] + e[sr + 1]) / 2.0f : 0.0f;
     gr += d_acc ? d_acc[ray] : 0.0f;
     if (d_exp != nullptr) {
-      const float A = ps_wave_sum(ws * mid), B = ps_wave_sum(ws) + 1e-10f;
+      float wm;
+      {  // rounded by itself, not inside the first addition of the sum: mid / B - A / (B * B) cancels down to these bits
+#pragma clang fp contract(off)
+        wm = ws * mid;
+      }
+      const float A = ps_wave_sum(wm), B = ps_wave_sum(ws) + 1e-10f;
       gr += d_exp[ray] * (mid / B - A / (B * B));
     }
     if (ok) {  // (+ the addends, in this order: what `dw += add0; dw += add1` launches used to do)
@@ -711,7 +731,12 @@ __global__ __launch_bounds__(256) void composite_bwd_w_kernel(const float* __res
   const float mid = lane < S ? (e[lane] + e[lane + 1]) / 2.0f : 0.0f;
   float g = v[0] + (d_acc ? d_acc[ray] : 0.0f);
   if (d_exp != nullptr) {  // expected depth D = A/(B+eps): dD/dw_s = t_s/(B+eps) - A/(B+eps)^2
-    const float A = ps_wave_sum(ws * mid), B = ps_wave_sum(ws) + 1e-10f;
+    float wm;
+    {
+#pragma clang fp contract(off)  // (as above)
+      wm = ws * mid;
+    }
+    const float A = ps_wave_sum(wm), B = ps_wave_sum(ws) + 1e-10f;
     g += d_exp[ray] * (mid / B - A / (B * B));
   }
   if (lane < S) {
