@@ -621,6 +621,41 @@ int ps_interlevel_loss_scaled(const float* c, const float* w, const float* cp, c
 int ps_finish_losses(const float* const* terms, const int64_t* n, const float* denom, const float* scale, const int* out_of,
                      int n_desc, float* const* out, int n_out, float* total, uint32_t* ticket, void* stream);
 
+/* ---- experts: rows sorted by expert and back, and the experts' linear layers on the sorted rows --------------------------------
+ * dtype of rows, weights and their gradients: 0 fp32, 1 fp16, 2 bf16; sums in fp32, one rounding.  k experts per row, E experts,
+ * M = N*k assignments f = n*k + j.  Strides are in elements between rows; the elements of a row are consecutive.
+ *   ps_expert_plan          ids [N,k] int32, or int64 (ids_are_64); an id outside [0, E) assigns to nobody.  offsets [E+1]: expert e's
+ *                           rows are the sorted places offsets[e] .. offsets[e+1]; src [M]: place -> assignment, by (expert, f), -1
+ *                           behind offsets[E]; dst [M]: assignment -> place or -1.  workspace: ps_expert_plan_workspace ints.  E <= 1024
+ *   ps_expert_dispatch      rows [M,D]: rows[dst[n,j]] = x[n]; zeros behind *held (= offsets + E)
+ *   ps_expert_combine       y [N,D] = sum_j weights[n,j] * rows[dst[n,j]] over the dst >= 0; weights NULL: ones (then it is the gradient
+ *                           of dispatch)
+ *   ps_expert_combine_bwd   drows [M,D] = weights * dy at their places, zeros behind *held (may be NULL); dw [N,k] = <dy, rows> (may be
+ *                           NULL), 0 for assignments to nobody
+ *   ps_expert_linear_fwd    y [M,out] = W_e x + b_e for expert e's rows, zeros for the rows of nobody; weight [E,out,in], bias [E,out] or
+ *                           NULL.  Offsets are bounded to [0, M]: no row outside is touched
+ *   ps_expert_linear_dx     dx [M,in] = W_e^T dy
+ *   ps_expert_linear_dw     dweight [E,out,in] = sum over expert e's rows of dy x^T, dbias [E,out] = sum dy (may be NULL); workspace:
+ *                           ps_expert_linear_dw_workspace bytes (NULL if 0) */
+int64_t ps_expert_plan_workspace(int64_t M, int E);
+int ps_expert_plan(const void* ids, int ids_are_64, int64_t M, int E, int32_t* offsets, int32_t* src, int32_t* dst,
+                   int32_t* workspace /*nullable*/, void* stream);
+int ps_expert_dispatch(const void* x, int64_t x_stride, const int32_t* dst, const int32_t* held, int64_t N, int k, int64_t D, int dtype,
+                       void* rows, void* stream);
+int ps_expert_combine(const void* rows, int64_t rows_stride, const float* weights /*nullable*/, const int32_t* dst, int64_t N, int k,
+                      int64_t D, int dtype, void* y, void* stream);
+int ps_expert_combine_bwd(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, const float* weights,
+                          const int32_t* dst, const int32_t* held, int64_t N, int k, int64_t D, int dtype, void* drows /*nullable*/,
+                          float* dw /*nullable*/, void* stream);
+int ps_expert_linear_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias /*nullable*/, const int32_t* offsets,
+                         int64_t M, int E, int64_t n_in, int64_t n_out, int dtype, void* y, void* stream);
+int ps_expert_linear_dx(const void* dy, int64_t dy_stride, const void* weight, const int32_t* offsets, int64_t M, int E, int64_t n_in,
+                        int64_t n_out, int dtype, void* dx, void* stream);
+int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype);
+int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const int32_t* offsets, int64_t M, int E,
+                        int64_t n_in, int64_t n_out, int dtype, void* dweight, void* dbias /*nullable*/, void* workspace /*nullable*/,
+                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,301 @@
+// The experts' linear layers on rows sorted by expert: rows [M, in], offsets [E+1] (expert e's rows are offsets[e] .. offsets[e+1]),
+// weight [E, out, in], bias [E, out].
+//     y[p]  = W_e x[p] + b_e                     tiles of (rows of one expert) x (out),  k = in     x k-contiguous, W k-contiguous
+//     dx[p] = W_e^T dy[p]                        tiles of (rows of one expert) x (in),   k = out    dy k-contiguous, W row-contiguous
+//     dW_e  = sum_p dy[p] x[p]^T, db_e = sum_p dy[p]   tiles of (out) x (in) of one expert, k = its rows, both row-contiguous
+// The experts' lengths are known on the device only.  A launch holds ceil(M / BM) + E row tiles, which is enough for any split of the
+// rows; every workgroup finds its expert and tile from the offsets, and the workgroups left over clear the rows of nobody.
+#include "gemm_core.hpp"
+
+namespace {
+
+using namespace ps;
+
+struct RowTile {
+  int expert;    // -1: left over
+  int64_t row0;  // first row of the tile | left over: index among the left-over tiles
+  int rows;      // rows of the tile      | left over: how many there are
+};
+
+__device__ __forceinline__ int64_t bounded(int v, int64_t M) { return v < 0 ? 0 : (v > M ? M : v); }
+
+// Which expert's rows tile t holds (uniform over the wave): a prefix sum of tiles over the experts, 64 at a time.
+template <int BM>
+__device__ __forceinline__ RowTile find_row_tile(const int* __restrict__ offsets, int E, int64_t M, int t, int tiles) {
+  const int lane = threadIdx.x & 63;
+  int base = 0;
+  for (int e0 = 0; e0 < E; e0 += 64) {
+    const int e = e0 + lane;
+    int64_t lo = 0, hi = 0;
+    if (e < E) {
+      lo = bounded(offsets[e], M);
+      hi = bounded(offsets[e + 1], M);
+    }
+    const int len = hi > lo ? (int)(hi - lo) : 0;
+    int incl = (len + BM - 1) / BM;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += o;
+    }
+    const int all = __shfl(incl, 63, 64);
+    if (t < base + all) {
+      const int who = uniform(__ffsll((long long)__ballot(t < base + incl)) - 1);
+      const int n = (len + BM - 1) / BM;
+      const int k = t - base - (__shfl(incl, who, 64) - __shfl(n, who, 64));
+      const int row0 = __shfl((int)lo, who, 64) + k * BM, left = __shfl(len, who, 64) - k * BM;
+      return {uniform(e0 + who), (int64_t)uniform(row0), uniform(left < BM ? left : BM)};
+    }
+    base += all;
+  }
+  return {-1, (int64_t)uniform(t - base), uniform(tiles - base)};
+}
+
+// zeros to columns [n0, n0 + cols) of the rows before offsets[0] and from offsets[E] on, shared out over the left-over tiles
+template <typename T, int BM>
+__device__ __forceinline__ void clear_outside(const int* __restrict__ offsets, int E, int64_t M, const RowTile& t, T* __restrict__ y, int N, int n0, int cols) {
+  const int64_t head = bounded(offsets[0], M), end = bounded(offsets[E], M), tail0 = end > head ? end : head;
+  const int64_t outside = head + (M - tail0);
+  for (int64_t q0 = t.row0 * BM; q0 < outside; q0 += (int64_t)t.rows * BM) {
+    for (int i = threadIdx.x; i < BM * cols; i += blockDim.x) {
+      const int64_t q = q0 + i / cols;
+      if (q < outside) y[(q < head ? q : tail0 + (q - head)) * N + n0 + i % cols] = from_f32<T>(0.0f);
+    }
+  }
+}
+
+// A workgroup's tile into memory: four consecutive n per lane and block
+template <typename T, int MI, int NJ>
+__device__ __forceinline__ void store_tile(f32x4 (&acc)[MI][NJ], T* __restrict__ y, int64_t ldy, int rows, int cols, int m0, int n0, const T* __restrict__ bias) {
+  const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  const bool packed = ((ldy * sizeof(T)) % (4 * sizeof(T))) == 0 && ((uintptr_t)y % (4 * sizeof(T))) == 0;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int n = n0 + j * 16 + g * 4;
+    float b[4] = {0.f, 0.f, 0.f, 0.f};
+    if (bias != nullptr) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (n + q < cols) b[q] = to_f32(bias[n + q]);
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + i * 16 + r;
+      if (m >= rows) continue;
+      T* o = y + m * ldy + n;
+      if (packed && n + 3 < cols) {
+        Pack<T, 4> p;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) p.v[q] = from_f32<T>(acc[i][j][q] + b[q]);
+        store_pack(o, p);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < cols) o[q] = from_f32<T>(acc[i][j][q] + b[q]);
+      }
+    }
+  }
+}
+
+// y[p] = sum_k x[p][k] W(n,k) (+ bias): W_RC = false: weight rows are k-contiguous (forward), true: n-contiguous (input gradient)
+template <typename T, int BM, int BN, int WM, int WN, int VB, bool W_RC>
+__global__ __launch_bounds__(64 * WM * WN) void linear_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias,
+                                                              const int* __restrict__ offsets, int64_t M, int E, int N, int K, int row_tiles,
+                                                              T* __restrict__ y) {
+  constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16, BK = kTileK<T>;
+  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * kTileRowBytes];
+  const int n_tiles = (N + BN - 1) / BN;
+  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles;
+  const RowTile t = find_row_tile<BM>(offsets, E, M, tm, row_tiles);
+  const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
+  if (t.expert < 0) {
+    clear_outside<T, BM>(offsets, E, M, t, y, N, n0, cols);
+    return;
+  }
+  const T* xa = x + t.row0 * ldx;
+  const T* wb = weight + (int64_t)t.expert * N * K + (W_RC ? (int64_t)n0 : (int64_t)n0 * K);
+  const unsigned lda = (unsigned)(ldx * sizeof(T)), ldb = (unsigned)((W_RC ? N : K) * sizeof(T));
+  TileLoader<T, BM, NT, VB, false> la;
+  TileLoader<T, BN, NT, VB, W_RC> lb;
+  auto load = [&](int k0) {
+    la.load(window(xa + k0, ((int64_t)(t.rows - 1) * ldx + (K - k0)) * sizeof(T)), lda, K - k0);
+    if constexpr (W_RC) {
+      const int kr = K - k0 < BK ? K - k0 : BK;
+      lb.load(window(wb + (int64_t)k0 * N, ((int64_t)(kr - 1) * N + (N - n0)) * sizeof(T)), ldb, N - n0);
+    } else {
+      lb.load(window(wb + k0, ((int64_t)(cols - 1) * K + (K - k0)) * sizeof(T)), ldb, K - k0);
+    }
+  };
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  load(0);
+  la.store(lds[0]);
+  lb.store(lds[0] + BM * kTileRowBytes);
+  __syncthreads();
+  for (int k0 = 0, cur = 0; k0 < K; k0 += BK, cur ^= 1) {
+    const bool more = k0 + BK < K;
+    if (more) load(k0 + BK);
+    tile_mma<T, MI, NJ>(lds[cur], lds[cur] + BM * kTileRowBytes, wm, wn, acc);
+    if (more) {
+      la.store(lds[cur ^ 1]);
+      lb.store(lds[cur ^ 1] + BM * kTileRowBytes);
+    }
+    __syncthreads();
+  }
+  store_tile<T, MI, NJ>(acc, y + t.row0 * N + n0, N, t.rows, cols, wm, wn, bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
+}
+
+// One piece of an expert's rows against a (out) x (in) tile.  split == false: the piece is all of the expert's rows and the tile is
+// written in T; true: tile `unit` of at most `piece` rows, written as fp32 partial sums [unit][out][in] that dw_join_kernel adds up.
+template <typename T, int BM, int BN, int WM, int WN, int VB>
+__global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
+                                                                 const int* __restrict__ offsets, int64_t M, int E, int N, int K, T* __restrict__ dw,
+                                                                 T* __restrict__ db) {
+  constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16, BK = kTileK<T>;
+  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * kTileRowBytes];
+  const int n_tiles = (K + BN - 1) / BN, m_tiles = (N + BM - 1) / BM;
+  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles % m_tiles, e = blockIdx.x / (n_tiles * m_tiles);
+  const int64_t lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
+  const int64_t row0 = lo;
+  const int len = uniform(hi > lo ? (int)(hi - lo) : 0);
+  const int m0 = tm * BM, n0 = tn * BN;
+  TileLoader<T, BM, NT, VB, true> la;
+  TileLoader<T, BN, NT, VB, true> lb;
+  auto load = [&](int k0) {
+    const int kr = len - k0 < BK ? len - k0 : BK;
+    la.load(window(dy + (row0 + k0) * ldy + m0, ((int64_t)(kr - 1) * ldy + (N - m0)) * sizeof(T)), (unsigned)(ldy * sizeof(T)), N - m0);
+    lb.load(window(x + (row0 + k0) * ldx + n0, ((int64_t)(kr - 1) * ldx + (K - n0)) * sizeof(T)), (unsigned)(ldx * sizeof(T)), K - n0);
+  };
+  const bool sums = db != nullptr && tn == 0;
+  float s[decltype(la)::N][kChunk<T>] = {};
+  f32x4 acc[MI][NJ];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  if (len > 0) {
+    load(0);
+    if (sums) la.add_rows(s);
+    la.store(lds[0]);
+    lb.store(lds[0] + BM * kTileRowBytes);
+  }
+  __syncthreads();
+  for (int k0 = 0, cur = 0; k0 < len; k0 += BK, cur ^= 1) {
+    const bool more = k0 + BK < len;
+    if (more) load(k0 + BK);
+    tile_mma<T, MI, NJ>(lds[cur], lds[cur] + BM * kTileRowBytes, wm, wn, acc);
+    if (more) {
+      if (sums) la.add_rows(s);
+      la.store(lds[cur ^ 1]);
+      lb.store(lds[cur ^ 1] + BM * kTileRowBytes);
+    }
+    __syncthreads();
+  }
+  store_tile<T, MI, NJ>(acc, dw + (int64_t)e * N * K + (int64_t)m0 * K + n0, K, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn, nullptr);
+  if (sums) {  // the threads of one column of blocks add up in order of k
+    float* part = reinterpret_cast<float*>(&lds[0][0]);
+    constexpr int kAcross = BM / kChunk<T>, kDeep = kTileK<T> / 4;
+#pragma unroll
+    for (int b = 0; b < decltype(la)::N; ++b) {
+      const int id = b * NT + threadIdx.x;
+      if (id < 2 * BM)
+#pragma unroll
+        for (int i = 0; i < kChunk<T>; ++i) part[(id / kAcross) * BM + (id % kAcross) * kChunk<T> + i] = s[b][i];
+    }
+    __syncthreads();
+    for (int m = threadIdx.x; m < BM && m0 + m < N; m += NT) {
+      float v = 0.0f;
+      for (int k = 0; k < kDeep; ++k) v += part[k * BM + m];
+      db[(int64_t)e * N + m0 + m] = from_f32<T>(v);
+    }
+  }
+}
+
+template <typename F>
+int by_type(int dtype, F&& f) {
+  if (dtype == kF32) return f(float{});
+  if (dtype == kF16) return f(_Float16{});
+  if (dtype == kBF16) return f(__bf16{});
+  ps_set_error("unknown element type (0 fp32, 1 fp16, 2 bf16)");
+  return -1;
+}
+
+template <typename T, typename F>
+int by_piece(int vb, F&& f) {
+  if (vb == 16) return f(std::integral_constant<int, 16>{});
+  if constexpr (sizeof(T) == 2) {
+    if (vb == 2) return f(std::integral_constant<int, 2>{});
+  }
+  return f(std::integral_constant<int, 4>{});
+}
+
+constexpr int64_t kMaxWidth = 1 << 20;
+
+bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
+  return M >= 0 && M < ((int64_t)1 << 31) - (1 << 20) && E >= 1 && E <= 65536 && n_in >= 1 && n_in <= kMaxWidth && n_out >= 1 && n_out <= kMaxWidth;
+}
+
+template <bool W_RC>
+int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, int dtype,
+                  void* y, hipStream_t s) {
+  return by_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const int vb = piece_bytes(sizeof(T), {ldx, N, K}, {x, weight});
+    return by_piece<T>(vb, [&](auto piece) {
+      constexpr int VB = decltype(piece)::value, BM = 128, BN = 128;
+      const int64_t row_tiles = (M + BM - 1) / BM + E, blocks = row_tiles * ((N + BN - 1) / BN);
+      PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
+      linear_kernel<T, BM, BN, 2, 2, VB, W_RC><<<(unsigned)blocks, 256, 0, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N, K,
+                                                                              (int)row_tiles, (T*)y);
+      PS_CHECK_LAUNCH();
+    });
+  });
+}
+
+}  // namespace
+
+extern "C" int ps_expert_linear_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E,
+                                    int64_t n_in, int64_t n_out, int dtype, void* y, void* stream) {
+  PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && x_stride >= n_in && x_stride <= kMaxWidth, "ps_expert_linear_fwd: sizes out of range");
+  if (M == 0) return 0;
+  PS_REQUIRE(x != nullptr && weight != nullptr && offsets != nullptr && y != nullptr, "ps_expert_linear_fwd: null argument");
+  return launch_linear<false>(x, x_stride, weight, bias, offsets, M, E, (int)n_out, (int)n_in, dtype, y, (hipStream_t)stream);
+}
+
+extern "C" int ps_expert_linear_dx(const void* dy, int64_t dy_stride, const void* weight, const int32_t* offsets, int64_t M, int E, int64_t n_in,
+                                   int64_t n_out, int dtype, void* dx, void* stream) {
+  PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && dy_stride >= n_out && dy_stride <= kMaxWidth, "ps_expert_linear_dx: sizes out of range");
+  if (M == 0) return 0;
+  PS_REQUIRE(dy != nullptr && weight != nullptr && offsets != nullptr && dx != nullptr, "ps_expert_linear_dx: null argument");
+  return launch_linear<true>(dy, dy_stride, weight, nullptr, offsets, M, E, (int)n_in, (int)n_out, dtype, dx, (hipStream_t)stream);
+}
+
+extern "C" int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
+  (void)M, (void)E, (void)n_in, (void)n_out, (void)dtype;
+  return 0;
+}
+
+extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const int32_t* offsets, int64_t M, int E,
+                                   int64_t n_in, int64_t n_out, int dtype, void* dweight, void* dbias, void* workspace, void* stream) {
+  PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && x_stride >= n_in && x_stride <= kMaxWidth && dy_stride >= n_out && dy_stride <= kMaxWidth,
+             "ps_expert_linear_dw: sizes out of range");
+  PS_REQUIRE((M == 0 || (dy != nullptr && x != nullptr)) && offsets != nullptr && dweight != nullptr, "ps_expert_linear_dw: null argument");
+  (void)workspace;
+  return by_type(dtype, [&](auto zero) {
+    using T = decltype(zero);
+    const int vb = piece_bytes(sizeof(T), {dy_stride, x_stride, n_in, n_out}, {dy, x});
+    return by_piece<T>(vb, [&](auto piece) {
+      constexpr int VB = decltype(piece)::value, BM = 128, BN = 128;
+      const int64_t blocks = (int64_t)E * ((n_out + BM - 1) / BM) * ((n_in + BN - 1) / BN);
+      PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
+      linear_dw_kernel<T, BM, BN, 2, 2, VB><<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const T*)dy, dy_stride, (const T*)x, x_stride, offsets, M, E,
+                                                                                            (int)n_out, (int)n_in, (T*)dweight, (T*)dbias);
+      PS_CHECK_LAUNCH();
+    });
+  });
+}

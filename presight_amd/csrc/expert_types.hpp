@@ -1,0 +1,31 @@
+// Element types of the expert and matrix-update operators (fp32, fp16, bf16) and rows read and written in packs of them.
+#pragma once
+#include <initializer_list>
+#include "common.hpp"
+
+namespace ps {
+
+enum : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
+__device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {  // round to nearest even
+  return (T)v;
+}
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, VEC>*>(p);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) {
+  *reinterpret_cast<Pack<T, VEC>*>(p) = v;
+}
+
+}  // namespace ps
