@@ -656,6 +656,21 @@ int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_
                         int64_t n_in, int64_t n_out, int dtype, void* dweight, void* dbias /*nullable*/, void* workspace /*nullable*/,
                         void* stream);
 
+/* ---- the orthogonalised update: G [B,m,n] (dtype as above) -> X of the same type after `steps` of X <- a X + (b S + c S S) X, S = X X^T,
+ * from X = G / (||G||_F + eps), every matrix by itself.  The caller checks that, from singular values in [0, 1], the iterates' squared
+ * singular values t and |a + b t + c t^2| stay under 15, and gives a power of two >= 1 that the latter stays under (grow).
+ * min(m, n) <= 16384, steps 1..64.  workspace: ps_newton_schulz_workspace bytes (NULL if 0).
+ *   ps_muon_step            for each of n_stacks stacks (HOST arrays of device pointers and sizes): buf <- momentum buf + (1 - momentum) g;
+ *                           u = nesterov ? momentum buf + (1 - momentum) g : buf; p <- keep p - rate X(u); p, g, buf fp32 [B,m,n].  One
+ *                           workspace, the largest that any stack needs, serves them one after the other */
+int64_t ps_newton_schulz_workspace(int64_t B, int64_t m, int64_t n);
+int ps_newton_schulz(const void* g, int64_t B, int64_t m, int64_t n, int dtype, int steps, double a, double b, double c, float grow, float eps,
+                     void* out, void* workspace, void* stream);
+int ps_muon_step(int n_stacks, float* const* p /*host*/, const float* const* g /*host*/, float* const* buf /*host*/,
+                 const int64_t* B /*host*/, const int64_t* m /*host*/, const int64_t* n /*host*/, const float* rate /*host*/,
+                 double momentum, int nesterov, float keep, int steps, double a, double b, double c, float grow, float eps,
+                 void* workspace, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,8 +1,11 @@
 """Adam on the HIP kernel (ps_adam_step), torch.optim.Adam-compatible numerics for the reference's settings
-(ns/engine/optimizers.py:73-170: one Adam per parameter group, lr 1e-2, eps 1e-15, weight_decay 1e-5)."""
+(ns/engine/optimizers.py:73-170: one Adam per parameter group, lr 1e-2, eps 1e-15, weight_decay 1e-5); and for weight matrices, single or
+stacked by expert, the orthogonalised update (newton_schulz) and the momentum step that applies it (HipMuon)."""
 from __future__ import annotations
 
-from typing import Iterable, List, Optional, Sequence
+import functools
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple
 
 import ctypes
 
@@ -10,6 +13,7 @@ import torch
 
 from ._lib import check, lib
 from .dist import intersect_ranges
+from .experts import DTYPE_CODES, _gpu, _on, _typed
 from .ops import _p, _stream
 
 
@@ -254,3 +258,151 @@ class WarmupMultiStepSchedule:
         self.t = int(sd["t"])
         self.lr_init = float(sd.get("lr_init", self.lr_init))
         self.opt.lr = self.lr_at(self.t)
+
+
+# ------------------------------------------------------------------------------------------------ the orthogonalised update
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # pushes (0, 1] into about [0.7, 1.2] in five steps: steep at zero, flat around one
+NS_MAX_SIDE = 16384  # of the short side
+_NS_BOUND = 15.0  # on squared singular values and on the polynomial: what the kernels' fp16 planes can hold (csrc/orthogonal.hip)
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_check(steps: int, a: float, b: float, c: float) -> float:
+    """the singular values of every iterate's S and of a + b S + c S^2, bounded from those of the first iterate (at most 1) -> the power
+    of two that the latter stay under"""
+    if not all(math.isfinite(v) for v in (a, b, c)):
+        raise ValueError(f"presight_amd: the coefficients must be finite (got {(a, b, c)})")
+    u, grow = 1.0, 1.0
+    for _ in range(steps):
+        t = u * u
+        inner = [0.0, t] + ([-b / (2 * c)] if c != 0 and 0 < -b / (2 * c) < t else [])
+        p = max(abs(a + b * v + c * v * v) for v in inner)
+        # extremes of v (a + b v^2 + c v^4) on [0, u]: the ends and the roots of a + 3 b w + 5 c w^2, w = v^2
+        roots: List[float] = []
+        if c != 0:
+            d = 9 * b * b - 20 * a * c
+            if d >= 0:
+                roots = [(-3 * b + s * math.sqrt(d)) / (10 * c) for s in (1, -1)]
+        elif b != 0:
+            roots = [-a / (3 * b)]
+        ends = [u] + [math.sqrt(w) for w in roots if 0 < w < t]
+        u = max(abs(v * (a + b * v * v + c * v ** 4)) for v in ends)
+        if max(p, u * u) > _NS_BOUND:
+            raise ValueError(f"presight_amd: with coefficients {(a, b, c)} the iterates grow too large within {steps} steps")
+        while grow < p:
+            grow *= 2.0
+    return grow
+
+
+def _ns_args(steps: int, coefficients: Tuple[float, float, float], eps: float) -> Tuple[int, float, float, float, float, float]:
+    if int(steps) != steps or not 1 <= steps <= 64:
+        raise ValueError(f"presight_amd: 1 to 64 steps (got {steps})")
+    if len(coefficients) != 3:
+        raise ValueError(f"presight_amd: three coefficients (got {coefficients})")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"presight_amd: eps must be finite and not negative (got {eps})")
+    a, b, c = (float(v) for v in coefficients)
+    return int(steps), a, b, c, _ns_check(int(steps), a, b, c), float(eps)
+
+
+def _matrices(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
+    if t.dim() < 2:
+        raise ValueError(f"presight_amd: {name} must be a matrix or a stack of matrices (got shape {tuple(t.shape)})")
+    m, n = t.shape[-2:]
+    B = math.prod(t.shape[:-2])
+    if min(m, n) > NS_MAX_SIDE or max(m, n) > 1 << 20 or B > 65535:
+        raise ValueError(f"presight_amd: {name}: up to 65535 matrices of {NS_MAX_SIDE} x {1 << 20} (got shape {tuple(t.shape)})")
+    return B, m, n
+
+
+@torch.no_grad()
+def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
+    """g [..., m, n] in fp32, fp16 or bf16 -> a tensor of its shape and type: every matrix scaled to X = G / (||G||_F + eps) and taken
+    `steps` times through X <- a X + (b S + c S S) X with S = X X^T: its singular vectors kept, its singular values moved towards one.
+    Products of fp16 pairs (22 bits) summed in fp32, one rounding at the end.  A zero matrix stays zero; a matrix with an infinite or
+    undefined entry becomes undefined, without touching the others of the stack.  Not differentiable."""
+    args = _ns_args(steps, tuple(coefficients), eps)
+    code = _typed(_gpu(g, "g"), "g")
+    B, m, n = _matrices(g, "g")
+    g = g.contiguous()
+    with _on(g.device):
+        out = torch.empty_like(g)
+        if out.numel():
+            nbytes = lib().ps_newton_schulz_workspace(B, m, n)
+            ws = torch.empty(nbytes, device=g.device, dtype=torch.uint8) if nbytes else None
+            check(lib().ps_newton_schulz(_p(g), B, m, n, code, *args, _p(out), _p(ws), _stream()), "ps_newton_schulz")
+    return out
+
+
+class HipMuon:
+    """Momentum with an orthogonalised update, for weight matrices [out, in] and stacks of them [experts, out, in] (embeddings, hash
+    tables, biases and output scalars belong to HipAdam):
+        buf <- momentum * buf + (1 - momentum) * grad
+        u    = momentum * buf + (1 - momentum) * grad   (nesterov)   |   buf
+        p   <- (1 - lr * weight_decay) * p - lr * scale * newton_schulz(u)
+    scale: "spectral": sqrt(max(1, out / in)), an update whose effect on activations does not depend on the width;
+           "rms": 0.2 * sqrt(max(out, in)), an update of the size Adam's has (its learning rates carry over).
+    Parameters are contiguous fp32; one without a gradient is skipped, its momentum included.  lr may be changed between steps.
+    Gradients held by a FlatGrads are read where it keeps them (a parameter counts as without a gradient until the backward pass has
+    reached it); parameters of its device-decided groups are refused."""
+
+    def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, ns_steps: int = 5, ns_coefficients: Tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7,
+                 scale: str = "spectral"):
+        self.params: List[torch.nn.Parameter] = [p for p in params if p.requires_grad and p.numel() > 0]
+        for p in self.params:
+            if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
+                raise RuntimeError("HipMuon: parameters must be contiguous fp32 CUDA tensors")
+            _matrices(p, "a parameter")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"HipMuon: 0 <= momentum < 1 (got {momentum})")
+        if scale not in ("spectral", "rms"):
+            raise ValueError(f"HipMuon: scale is 'spectral' or 'rms' (got {scale!r})")
+        self.lr, self.momentum, self.nesterov, self.weight_decay, self.scale = lr, momentum, nesterov, weight_decay, scale
+        self.ns = _ns_args(ns_steps, tuple(ns_coefficients), eps)
+        self.step_count = 0
+        self.momentum_buffers = [torch.zeros_like(p, requires_grad=False) for p in self.params]
+
+    def _rate(self, p: torch.Tensor) -> float:
+        out, n_in = p.shape[-2:]
+        return self.lr * (math.sqrt(max(1.0, out / n_in)) if self.scale == "spectral" else 0.2 * math.sqrt(max(out, n_in)))
+
+    @torch.no_grad()
+    def step(self) -> None:
+        self.step_count += 1
+        by_device: dict = {}
+        for p, buf in zip(self.params, self.momentum_buffers):
+            g = p.grad
+            if g is None or (getattr(p, "_ps_direct_grad", False) and not p._ps_touched):
+                continue
+            if getattr(p, "_ps_group", None) is not None:
+                raise RuntimeError("HipMuon: whether this parameter has a gradient is decided on the device; it belongs to HipAdam")
+            if g.dtype != torch.float32 or g.device != p.device or g.shape != p.shape:
+                raise RuntimeError("HipMuon: gradients must be dense fp32 tensors on their parameter's device")
+            by_device.setdefault(p.device, []).append((p, g.contiguous(), buf))
+        for device, stacks in by_device.items():
+            k = len(stacks)
+            sizes = [_matrices(p, "a parameter") for p, _, _ in stacks]
+            i64, ptr = ctypes.c_int64 * k, ctypes.c_void_p * k
+            with _on(device):
+                nbytes = max(lib().ps_newton_schulz_workspace(*s) for s in sizes)
+                ws = torch.empty(nbytes, device=device, dtype=torch.uint8) if nbytes else None
+                check(lib().ps_muon_step(k, ptr(*[_p(s[0]) for s in stacks]), ptr(*[_p(s[1]) for s in stacks]), ptr(*[_p(s[2]) for s in stacks]),
+                                         i64(*[s[0] for s in sizes]), i64(*[s[1] for s in sizes]), i64(*[s[2] for s in sizes]),
+                                         (ctypes.c_float * k)(*[self._rate(s[0]) for s in stacks]), self.momentum, int(self.nesterov),
+                                         1.0 - self.lr * self.weight_decay, *self.ns, _p(ws), _stream()), "ps_muon_step")
+
+    def zero_grad(self):
+        for p in self.params:
+            if p.grad is not None:
+                p.grad.zero_()
+
+    def state_dict(self):
+        return {"step": self.step_count, "lr": self.lr, "momentum_buffers": self.momentum_buffers}
+
+    def load_state_dict(self, sd):
+        if len(sd["momentum_buffers"]) != len(self.momentum_buffers):
+            raise ValueError("HipMuon: the state holds another number of parameters")
+        self.step_count, self.lr = sd["step"], sd["lr"]
+        for a, b in zip(self.momentum_buffers, sd["momentum_buffers"]):
+            a.copy_(b)

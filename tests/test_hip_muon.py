@@ -1,0 +1,317 @@
+"""The orthogonalised update and its optimizer (presight_amd.optim.newton_schulz, HipMuon) against plain 64-bit restatements.
+
+Tolerance.  Rounding errors of the iterates grow by up to the polynomial's steepest slope (about 4) per step in the small singular
+directions and are damped in the others, so a bound from the formula alone is a thousand times too wide.  It is taken from the same
+formula in plain fp32 instead: its distance from 64 bits in the Frobenius norm, per matrix.  The kernels hold 22 bits where fp32 holds 24
+but sum the same fp32 way: each of a step's three stored results (S, a + b S + c S S, X) carries a rounding of 2^-23 in place of 2^-24, and
+each of the three products a dropped term of 2^-24, so at most four times the unit that the plain form rounds with: 4 x its distance.  A
+matrix for which that distance happens to be tiny gets 16 * 2^-24 of its norm instead.  The result's own rounding comes on top."""
+import math
+
+import pytest
+import torch
+
+from presight_amd import optim
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+ABC = optim.NS_COEFFICIENTS
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "gpu tests need a GPU"
+    return torch.device("cuda:0")
+
+
+def iterate(g, steps=5, abc=ABC, eps=1e-7):
+    """the definition, in g's own precision, short side first"""
+    a, b, c = abc
+    x = g.transpose(-2, -1) if g.shape[-2] > g.shape[-1] else g
+    x = x / (x.double().square().sum((-2, -1), keepdim=True).sqrt() + eps).to(x.dtype)
+    for _ in range(steps):
+        s = x @ x.transpose(-2, -1)
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.transpose(-2, -1) if g.shape[-2] > g.shape[-1] else x
+
+
+def norms(t):
+    return t.double().flatten(-2).norm(dim=-1)
+
+
+def check(got, g, steps=5, abc=ABC, eps=1e-7):
+    g = g.detach().cpu()
+    ref = iterate(g.double(), steps, abc, eps)
+    plain = norms(iterate(g.float(), steps, abc, eps).double() - ref)
+    f = torch.finfo(got.dtype)
+    rounding = norms(ref) * f.eps / 2 + f.smallest_normal * f.eps * math.sqrt(g.shape[-1] * g.shape[-2])
+    bound = torch.maximum(4 * plain, 16 * 2.0 ** -24 * norms(ref)) + (rounding if got.dtype != torch.float32 else 0)
+    err = norms(got.detach().cpu().double() - ref)
+    assert got.shape == g.shape and torch.isfinite(got).all()
+    assert (err <= bound).all(), f"worst {float((err / bound.clamp_min(1e-300)).max()):.2f} x the bound, relative {float((err / norms(ref)).max()):.1e}"
+    return ref
+
+
+# ------------------------------------------------------------------------------------------------ refusals (no GPU needed)
+def test_refuses_what_it_cannot_do():
+    g = torch.zeros(4, 5)
+    with pytest.raises(RuntimeError, match="must live on the GPU"):
+        optim.newton_schulz(g)
+    for kw in (dict(steps=0), dict(steps=65), dict(steps=2.5), dict(coefficients=(1.0, 2.0)), dict(coefficients=(3.0, 3.0, 3.0)),
+               dict(coefficients=(float("nan"), 0.0, 0.0)), dict(eps=-1.0), dict(eps=float("inf"))):
+        with pytest.raises(ValueError):
+            optim.newton_schulz(g, **kw)
+    with pytest.raises(RuntimeError, match="contiguous fp32 CUDA"):
+        optim.HipMuon([torch.nn.Parameter(g)])
+
+
+def test_bound_of_the_polynomial_holds_by_sampling():
+    """what _ns_check lets through stays inside its bound on a fine grid; what leaves it is refused"""
+    for abc in (ABC, (2.0, -1.5, 0.5), (1.5, -0.5, 0.0), (3.0, -16 / 5, 6 / 5), (1.0, 0.0, 0.0), (5.0, 0.0, 0.0), (1.0, 2.0, 0.0), (-2.0, 1.0, 3.0)):
+        v = torch.linspace(0, 1, 20001, dtype=torch.float64)
+        worst = 1.0
+        for _ in range(3):
+            worst = max(worst, float((abc[0] + abc[1] * v ** 2 + abc[2] * v ** 4).abs().max()), float((v * v).max()))
+            v = (v * (abc[0] + abc[1] * v ** 2 + abc[2] * v ** 4)).abs()
+            v = torch.linspace(0, float(v.max()), 20001, dtype=torch.float64)
+            worst = max(worst, float(v.max()), float((v * v).max()))
+        if worst > 15.001:
+            with pytest.raises(ValueError):
+                optim._ns_check(3, *abc)
+        elif worst < 14.9:
+            assert optim._ns_check(3, *abc) <= 16.0
+
+
+def test_library_refuses_bad_sizes():
+    from presight_amd._lib import lib
+
+    h = lib()
+    assert h.ps_newton_schulz_workspace(0, 80, 90) == 0 and h.ps_newton_schulz_workspace(1, 80, 90) > 0
+    for rc in (h.ps_newton_schulz(None, 1, 8, 8, 0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, None, None, None),
+               h.ps_newton_schulz(None, 1, 8, 8, 0, 0, 1.0, 0.0, 0.0, 1.0, 0.0, None, None, None),
+               h.ps_newton_schulz(None, 1, 20000, 20000, 0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, None, None, None),
+               h.ps_newton_schulz(None, 1 << 17, 8, 8, 0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, None, None, None),
+               h.ps_muon_step(1, None, None, None, None, None, None, None, 0.9, 1, 1.0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, None, None)):
+        assert rc != 0
+    assert h.ps_newton_schulz(None, 0, 8, 8, 0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, None, None, None) == 0
+
+
+# ------------------------------------------------------------------------------------------------ values
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 1), (1, 70), (64, 64), (2, 2, 5, 7), (16, 64, 40), (5, 80, 64), (3, 385, 129), (7, 3, 64), (2, 65, 63),
+                                   (1, 128, 128), (2, 129, 200), (4, 33, 900), (1, 640, 512), (1, 257, 1030), (130, 9, 4)])
+def test_newton_schulz(dev, shape, dtype):
+    g = torch.Generator().manual_seed(sum(shape))
+    x = (torch.randn(shape, generator=g) * 3e-3).to(TYPES[dtype])
+    check(optim.newton_schulz(x.to(dev)), x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps,abc,eps", [(1, ABC, 1e-7), (2, (2.0, -1.5, 0.5), 0.0), (10, (1.5, -0.5, 0.0), 1e-3), (5, (1.0, 0.0, 0.0), 1e-7)])
+def test_other_polynomials(dev, steps, abc, eps):
+    x = torch.randn(3, 70, 50, generator=torch.Generator().manual_seed(1))
+    check(optim.newton_schulz(x.to(dev), steps=steps, coefficients=abc, eps=eps), x, steps, abc, eps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(64, 48), (300, 200)])
+@pytest.mark.parametrize("scale", [1e-30, 1e-12, 1.0, 1e18, 3e37])
+def test_any_scale(dev, shape, scale):
+    """sums of squares that leave fp32's range; below eps the result shrinks with the input, as the definition has it"""
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(3)) * scale
+    check(optim.newton_schulz(x.to(dev)), x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [40, 200])
+def test_of_low_rank_and_of_zero(dev, side):
+    g = torch.Generator().manual_seed(5)
+    x = torch.stack([torch.randn(side, 1, generator=g) @ torch.randn(1, 2 * side, generator=g), torch.zeros(side, 2 * side),
+                     torch.randn(side, 3, generator=g) @ torch.randn(3, 2 * side, generator=g)])
+    y = optim.newton_schulz(x.to(dev))
+    check(y, x)
+    assert not y[1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [40, 200])
+def test_undefined_entries_stay_in_their_matrix(dev, side):
+    x = torch.randn(4, side, side + 5, generator=torch.Generator().manual_seed(6))
+    clean = optim.newton_schulz(x.to(dev))
+    x[1, 3, 4], x[2, 0, 0] = float("nan"), float("inf")
+    y = optim.newton_schulz(x.to(dev))
+    assert torch.equal(y[0], clean[0]) and torch.equal(y[3], clean[3])
+    assert torch.isnan(y[1]).all() and torch.isnan(y[2]).all()
+
+
+@pytest.mark.gpu
+def test_singular_values_move_to_one_and_vectors_stay(dev):
+    g = torch.Generator().manual_seed(7)
+    u, _, v = torch.linalg.svd(torch.randn(96, 160, generator=g, dtype=torch.float64), full_matrices=False)
+    x = (u * torch.linspace(0.05, 1, 96, dtype=torch.float64)) @ v
+    y = optim.newton_schulz(x.float().to(dev)).cpu().double()
+    d = u.T @ y @ v.T
+    s = d.diagonal()
+    assert float(s.min()) > 0.6 and float(s.max()) < 1.3 and float((d - torch.diag(s)).abs().max()) < 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 64, 40), (2, 200, 136)])
+def test_other_layouts_and_empty(dev, shape):
+    x = torch.randn(shape, generator=torch.Generator().manual_seed(8)).to(dev)
+    want = optim.newton_schulz(x)
+    assert torch.equal(optim.newton_schulz(x.transpose(1, 2).contiguous().transpose(1, 2)), want)
+    wide = torch.zeros(shape[0], shape[1], shape[2] + 3, device=dev)
+    wide[..., 1:-2] = x
+    assert torch.equal(optim.newton_schulz(wide[..., 1:-2]), want)
+    assert torch.equal(optim.newton_schulz(x[1]), want[1])  # (a matrix does not see the rest of its stack)
+    assert optim.newton_schulz(x[:0]).shape == (0,) + shape[1:] and optim.newton_schulz(x[:, :0]).shape == (shape[0], 0, shape[2])
+
+
+@pytest.mark.gpu
+def test_a_large_matrix(dev):
+    """1500 x 2300: against 64 bits on the GPU"""
+    x = torch.randn(1500, 2300, generator=torch.Generator().manual_seed(9)).to(dev)
+    ref, plain = iterate(x.double()), iterate(x)
+    bound = max(4 * float((plain.double() - ref).norm()), 16 * 2.0 ** -24 * float(ref.norm()))
+    assert float((optim.newton_schulz(x).double() - ref).norm()) <= bound
+
+
+# ------------------------------------------------------------------------------------------------ the optimizer
+def muon_ref(p, g, buf, lr, mu, nesterov, wd, scale):
+    buf = mu * buf + (1 - mu) * g
+    u = mu * buf + (1 - mu) * g if nesterov else buf
+    out, n_in = p.shape[-2:]
+    rate = lr * (math.sqrt(max(1.0, out / n_in)) if scale == "spectral" else 0.2 * math.sqrt(max(out, n_in)))
+    return (1 - lr * wd) * p - rate * iterate(u), buf, rate
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nesterov,scale", [(True, "spectral"), (False, "rms")])
+@pytest.mark.parametrize("shapes", [[(16, 64, 40), (80, 64), (3, 64), (1, 64)], [(2, 300, 200), (64, 64), (260, 1000)]])
+def test_muon_steps(dev, shapes, nesterov, scale):
+    """three steps with fresh gradients, weight decay and a changed learning rate; a parameter whose gradient is missing in the second"""
+    g = torch.Generator().manual_seed(10)
+    start = [torch.randn(s, generator=g) for s in shapes]
+    params = [torch.nn.Parameter(t.to(dev)) for t in start]
+    opt = optim.HipMuon(params, lr=0.03, momentum=0.9, nesterov=nesterov, weight_decay=0.1, scale=scale)
+    ref = [(t.double(), torch.zeros(t.shape, dtype=torch.float64)) for t in start]
+    size = [0.0] * len(shapes)
+    for step in range(3):
+        opt.lr = 0.03 / (1 + step)
+        for i, p in enumerate(params):
+            grad = torch.randn(p.shape, generator=g) * 10.0 ** (step - 2)
+            p.grad = grad.to(dev)
+            if step == 1 and i == 1:
+                p.grad = None
+                continue
+            new, buf, rate = muon_ref(*[t for t in (ref[i][0], grad.double(), ref[i][1])], opt.lr, 0.9, nesterov, 0.1, scale)
+            ref[i] = (new, buf)
+            size[i] += rate
+        opt.step()
+    for i, (p, buf) in enumerate(zip(params, opt.momentum_buffers)):
+        # updates: relative error below 1e-4 each (test_newton_schulz's bound at these sizes is smaller); parameters: three fp32 roundings of
+        # values that the last one bounds within a factor of two
+        many = math.prod(p.shape[:-2]) or 1
+        bound = 1e-4 * size[i] * 1.3 * math.sqrt(many * min(p.shape[-2:])) + 6 * 2.0 ** -24 * 2 * float(ref[i][0].norm())
+        assert float((p.detach().cpu().double() - ref[i][0]).norm()) <= bound
+        torch.testing.assert_close(buf.cpu().double(), ref[i][1], rtol=0, atol=8 * 2.0 ** -24 * float(ref[i][1].abs().max()))
+
+
+@pytest.mark.gpu
+def test_muon_state_and_refusals(dev):
+    g = torch.Generator().manual_seed(11)
+    p = torch.nn.Parameter(torch.randn(6, 48, 32, generator=g).to(dev))
+    q = torch.nn.Parameter(p.detach().clone())
+    a, b = optim.HipMuon([p]), optim.HipMuon([q])
+    for i in range(3):
+        grad = torch.randn(p.shape, generator=g).to(dev)
+        p.grad = grad
+        a.step()
+        if i == 1:
+            b.load_state_dict(a.state_dict())
+            q.data.copy_(p.data)
+        if i == 2:
+            q.grad = grad.clone()
+            b.step()
+    assert torch.equal(p, q) and torch.equal(a.momentum_buffers[0], b.momentum_buffers[0]) and b.step_count == 3
+    for bad in (torch.zeros(4, device=dev), torch.zeros(4, 4, device=dev).half()):
+        with pytest.raises((ValueError, RuntimeError)):
+            optim.HipMuon([torch.nn.Parameter(bad)])
+    with pytest.raises(ValueError):
+        optim.HipMuon([p], momentum=1.0)
+    with pytest.raises(ValueError):
+        optim.HipMuon([p], scale="other")
+    p.grad = None
+    p._ps_group = 0
+    p.grad = grad
+    with pytest.raises(RuntimeError, match="decided on the device"):
+        a.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [[(16, 64, 40), (3, 64)], [(2, 200, 300)]])
+def test_muon_captured(dev, shapes):
+    """a captured step, replayed on new gradients with eager work in between, walks the eager path bit for bit"""
+    g = torch.Generator().manual_seed(12)
+    start = [torch.randn(s, generator=g).to(dev) for s in shapes]
+    eager, graphed = ([torch.nn.Parameter(t.clone()) for t in start] for _ in range(2))
+    a, b = optim.HipMuon(eager), optim.HipMuon(graphed)
+    static = [torch.zeros_like(t) for t in start]
+    for p, s in zip(graphed, static):
+        p.grad = s
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # (a step without gradients leaves nothing behind but the decay)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            b.step()
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(4):
+        for p, s in zip(eager, static):
+            p.grad = torch.randn(p.shape, generator=g).to(dev)
+            s.copy_(p.grad)
+        graph.replay()
+        a.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(eager, graphed))
+        assert all(torch.equal(p, q) for p, q in zip(a.momentum_buffers, b.momentum_buffers))
+
+
+@pytest.mark.gpu
+def test_experts_trained_by_muon(dev):
+    """the operators as they are used together: rows to their experts, two layers, back with gates, gradients, the step on the stacked
+    weights; against 64 bits"""
+    from presight_amd import experts
+
+    g = torch.Generator().manual_seed(13)
+    N, k, E, D, H = 500, 2, 6, 40, 64
+    ids = torch.randint(-1, E, (N, k), generator=g)
+    x, gates, dy = torch.randn(N, D, generator=g), torch.rand(N, k, generator=g), torch.randn(N, D, generator=g)
+    w1, w2 = torch.randn(E, H, D, generator=g) / D ** 0.5, torch.randn(E, D, H, generator=g) / H ** 0.5
+
+    def forward64(w1, w2):
+        y = torch.zeros(N, D, dtype=torch.float64)
+        for j in range(k):
+            for e in range(E):
+                m = ids[:, j] == e
+                h = torch.relu(x[m].double() @ w1[e].T)
+                y = y.index_add(0, m.nonzero()[:, 0], gates[m, j].double()[:, None] * (h @ w2[e].T))
+        return y
+
+    refs = [w1.double().requires_grad_(True), w2.double().requires_grad_(True)]
+    y64 = forward64(*refs)
+    grads = torch.autograd.grad(y64, refs, dy.double())
+    params = [torch.nn.Parameter(t.to(dev)) for t in (w1, w2)]
+    opt = optim.HipMuon(params, lr=0.02, weight_decay=0.01)
+    plan = experts.expert_plan(ids.to(dev), E)
+    h = torch.relu(experts.expert_linear(experts.expert_dispatch(x.to(dev), plan), params[0], None, plan))
+    y = experts.expert_combine(experts.expert_linear(h, params[1], None, plan), gates.to(dev), plan)
+    torch.testing.assert_close(y.detach().cpu().double(), y64.detach(), rtol=0, atol=(D + H + 4) * 2.0 ** -23 * float(y64.abs().max()) * 4)
+    y.backward(dy.to(dev))
+    opt.step()
+    for p, ref, grad in zip(params, refs, grads):
+        new, _, rate = muon_ref(ref.detach(), grad, torch.zeros_like(grad), 0.02, 0.95, True, 0.01, "spectral")
+        # the gradient's relative error (sums of about 170 rows of about 100 terms) grows by at most the polynomial's slope per step
+        slack = rate * 4 ** 5 * (N + D + H) * 2.0 ** -23 * math.sqrt(E * 40) + 4 * 2.0 ** -24 * float(new.norm())
+        assert float((p.detach().cpu().double() - new).norm()) <= slack
