@@ -651,7 +651,7 @@ int ps_expert_linear_fwd(const void* x, int64_t x_stride, const void* weight, co
                          int64_t M, int E, int64_t n_in, int64_t n_out, int dtype, void* y, void* stream);
 int ps_expert_linear_dx(const void* dy, int64_t dy_stride, const void* weight, const int32_t* offsets, int64_t M, int E, int64_t n_in,
                         int64_t n_out, int dtype, void* dx, void* stream);
-int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype);
+int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out);
 int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const int32_t* offsets, int64_t M, int E,
                         int64_t n_in, int64_t n_out, int dtype, void* dweight, void* dbias /*nullable*/, void* workspace /*nullable*/,
                         void* stream);

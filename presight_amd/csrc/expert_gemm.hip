@@ -5,6 +5,7 @@
 //     dW_e  = sum_p dy[p] x[p]^T, db_e = sum_p dy[p]   tiles of (out) x (in) of one expert, k = its rows, both row-contiguous
 // The experts' lengths are known on the device only.  A launch holds ceil(M / BM) + E row tiles, which is enough for any split of the
 // rows; every workgroup finds its expert and tile from the offsets, and the workgroups left over clear the rows of nobody.
+#include <type_traits>
 #include "gemm_core.hpp"
 
 namespace {
@@ -19,9 +20,8 @@ struct RowTile {
 
 __device__ __forceinline__ int64_t bounded(int v, int64_t M) { return v < 0 ? 0 : (v > M ? M : v); }
 
-// Which expert's rows tile t holds (uniform over the wave): a prefix sum of tiles over the experts, 64 at a time.
-template <int BM>
-__device__ __forceinline__ RowTile find_row_tile(const int* __restrict__ offsets, int E, int64_t M, int t, int tiles) {
+// Which expert's rows tile t (of `piece` rows) holds, uniform over the wave: a prefix sum of tiles over the experts, 64 at a time.
+__device__ __forceinline__ RowTile find_row_tile(const int* __restrict__ offsets, int E, int64_t M, int piece, int t, int tiles) {
   const int lane = threadIdx.x & 63;
   int base = 0;
   for (int e0 = 0; e0 < E; e0 += 64) {
@@ -32,7 +32,7 @@ __device__ __forceinline__ RowTile find_row_tile(const int* __restrict__ offsets
       hi = bounded(offsets[e + 1], M);
     }
     const int len = hi > lo ? (int)(hi - lo) : 0;
-    int incl = (len + BM - 1) / BM;
+    int incl = (len + piece - 1) / piece;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(incl, d, 64);
@@ -41,10 +41,10 @@ __device__ __forceinline__ RowTile find_row_tile(const int* __restrict__ offsets
     const int all = __shfl(incl, 63, 64);
     if (t < base + all) {
       const int who = uniform(__ffsll((long long)__ballot(t < base + incl)) - 1);
-      const int n = (len + BM - 1) / BM;
+      const int n = (len + piece - 1) / piece;
       const int k = t - base - (__shfl(incl, who, 64) - __shfl(n, who, 64));
-      const int row0 = __shfl((int)lo, who, 64) + k * BM, left = __shfl(len, who, 64) - k * BM;
-      return {uniform(e0 + who), (int64_t)uniform(row0), uniform(left < BM ? left : BM)};
+      const int row0 = __shfl((int)lo, who, 64) + k * piece, left = __shfl(len, who, 64) - k * piece;
+      return {uniform(e0 + who), (int64_t)uniform(row0), uniform(left < piece ? left : piece)};
     }
     base += all;
   }
@@ -106,7 +106,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_kernel(const T* __restric
   __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * kTileRowBytes];
   const int n_tiles = (N + BN - 1) / BN;
   const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles;
-  const RowTile t = find_row_tile<BM>(offsets, E, M, tm, row_tiles);
+  const RowTile t = find_row_tile(offsets, E, M, BM, tm, row_tiles);
   const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
   if (t.expert < 0) {
     clear_outside<T, BM>(offsets, E, M, t, y, N, n0, cols);
@@ -216,6 +216,161 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __rest
   }
 }
 
+// ------------------------------------------------------------------------------------------------ aligned operands
+// The same two kernels for operands whose pieces are whole 16-byte chunks: tiles go straight into LDS, two stages, the loads of the next
+// tile in flight while the matrix instructions run over this one.
+// SUMS: also the sums of A's rows over k, as a product with ones (`sums`: whether this wave wants them).
+template <typename T, int BM, int BN, int WM, int WN, bool A_RC, bool B_RC, bool SUMS>
+__device__ __forceinline__ void direct_loop(char* lds, int K, const DirectSource<T, BM, 64 * WM * WN, A_RC>& sa,
+                                            const DirectSource<T, BN, 64 * WM * WN, B_RC>& sb, f32x4 (&acc)[BM / WM / 16][BN / WN / 16],
+                                            f32x4 (&row_sums)[SUMS ? BM / WM / 16 : 1], bool sums) {
+  constexpr int MI = BM / WM / 16, NJ = BN / WN / 16, BK = kTileK<T>, kStage = (BM + BN) * kTileRowBytes;
+  using TA = DirectTile<T, BM, 64 * WM * WN, A_RC>;
+  using TB = DirectTile<T, BN, 64 * WM * WN, B_RC>;
+  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  u32x4 ones;
+  if constexpr (SUMS) {
+    const unsigned one = sizeof(T) == 4 ? 0x3f800000u : (__is_same(T, _Float16) ? 0x3c003c00u : 0x3f803f80u);
+    ones = u32x4{one, one, one, one};
+#pragma unroll
+    for (int i = 0; i < MI; ++i) row_sums[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (K <= 0) return;
+  sa.load(0, lds);
+  sb.load(0, lds + BM * kTileRowBytes);
+  __syncthreads();
+  for (int k0 = 0, cur = 0; k0 < K; k0 += BK, cur ^= 1) {
+    char* a = lds + cur * kStage;
+    if (k0 + BK < K) {
+      char* next = lds + (cur ^ 1) * kStage;
+      sa.load(k0 + BK, next);
+      sb.load(k0 + BK, next + BM * kTileRowBytes);
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      u32x4 fa[MI], fb[NJ];
+#pragma unroll
+      for (int i = 0; i < MI; ++i) fa[i] = TA::fragment(a, wm + i * 16, s);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) fb[j] = TB::fragment(a + BM * kTileRowBytes, wn + j * 16, s);
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = mma_block<T>(fa[i], fb[j], acc[i][j]);
+      if constexpr (SUMS) {
+        if (sums)
+#pragma unroll
+          for (int i = 0; i < MI; ++i) row_sums[i] = mma_block<T>(fa[i], ones, row_sums[i]);
+      }
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool W_RC>
+__global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight,
+                                                                     const T* __restrict__ bias, const int* __restrict__ offsets, int64_t M, int E,
+                                                                     int N, int K, int row_tiles, T* __restrict__ y) {
+  constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int n_tiles = (N + BN - 1) / BN;
+  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles;
+  const RowTile t = find_row_tile(offsets, E, M, BM, tm, row_tiles);
+  const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
+  if (t.expert < 0) {
+    clear_outside<T, BM>(offsets, E, M, t, y, N, n0, cols);
+    return;
+  }
+  const T* wb = weight + (int64_t)t.expert * N * K + (W_RC ? (int64_t)n0 : (int64_t)n0 * K);
+  const DirectSource<T, BM, NT, false> sa(x + t.row0 * ldx, ldx, t.rows, K);
+  const DirectSource<T, BN, NT, W_RC> sb(wb, W_RC ? N : K, W_RC ? N - n0 : cols, K);
+  f32x4 acc[MI][NJ], none[1];
+  direct_loop<T, BM, BN, WM, WN, false, W_RC, false>(lds, K, sa, sb, acc, none, false);
+  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  store_tile<T, MI, NJ>(acc, y + t.row0 * N + n0, N, t.rows, cols, wm, wn, bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
+}
+
+// Weight gradients.  Few and small weights with many rows would leave most of the chip idle: then (SPLIT) the experts' rows are cut into
+// pieces of `piece` rows, whoever they belong to, every piece writes its own fp32 sums [unit][out][in] (and [unit][out]), and
+// dw_join_kernel adds up the pieces of each expert in order.  Also shorter sums: a piece rounds `piece` / 4 times where the whole
+// column would round a hundred times as often.
+template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
+__global__ __launch_bounds__(64 * WM * WN) void linear_dw_direct_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
+                                                                        const int* __restrict__ offsets, int64_t M, int E, int N, int K, int piece,
+                                                                        int units, void* __restrict__ dw, void* __restrict__ db) {
+  constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
+  using Out = std::conditional_t<SPLIT, float, T>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int n_tiles = (K + BN - 1) / BN, m_tiles = (N + BM - 1) / BM;
+  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles % m_tiles, unit = blockIdx.x / (n_tiles * m_tiles);
+  int64_t row0;
+  int len;
+  if constexpr (SPLIT) {
+    const RowTile t = find_row_tile(offsets, E, M, piece, unit, units);
+    if (t.expert < 0) return;  // (nobody reads the units left over)
+    row0 = t.row0;
+    len = t.rows;
+  } else {
+    const int64_t lo = bounded(offsets[unit], M), hi = bounded(offsets[unit + 1], M);
+    row0 = lo;
+    len = uniform(hi > lo ? (int)(hi - lo) : 0);
+  }
+  const int m0 = tm * BM, n0 = tn * BN;
+  const DirectSource<T, BM, NT, true> sa(dy + row0 * ldy + m0, ldy, N - m0, len);
+  const DirectSource<T, BN, NT, true> sb(x + row0 * ldx + n0, ldx, K - n0, len);
+  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  const bool sums = db != nullptr && tn == 0 && wn == 0;
+  f32x4 acc[MI][NJ], row_sums[MI];
+  direct_loop<T, BM, BN, WM, WN, true, true, true>(lds, len, sa, sb, acc, row_sums, sums);
+  Out* o = reinterpret_cast<Out*>(dw) + (int64_t)unit * N * K + (int64_t)m0 * K + n0;
+  store_tile<Out, MI, NJ>(acc, o, K, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn, nullptr);
+  if (sums && (threadIdx.x & 63) < 16) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+      const int m = m0 + wm + i * 16 + (threadIdx.x & 15);
+      if (m < N) reinterpret_cast<Out*>(db)[(int64_t)unit * N + m] = from_f32<Out>(row_sums[i][0]);
+    }
+  }
+}
+
+// dW_e, db_e = the sums of expert e's pieces, in order
+template <typename T>
+__global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ parts, const float* __restrict__ db_parts, const int* __restrict__ offsets,
+                                                      int64_t M, int64_t size, int N, int piece, T* __restrict__ dw, T* __restrict__ db) {
+  __shared__ int wave_sum[4];
+  const int e = blockIdx.y;
+  int before = 0;
+  for (int i = threadIdx.x; i < e; i += 256) {
+    const int64_t lo = bounded(offsets[i], M), hi = bounded(offsets[i + 1], M);
+    if (hi > lo) before += (int)((hi - lo + piece - 1) / piece);
+  }
+  for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d, 64);
+  if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = before;
+  __syncthreads();
+  const int64_t first = (int64_t)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+  const int64_t lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
+  const int n = hi > lo ? (int)((hi - lo + piece - 1) / piece) : 0;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i < size) {  // (size is a multiple of four: the direct kernels' rule)
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < n; ++u) v += *reinterpret_cast<const f32x4*>(parts + (first + u) * size + i);
+    Pack<T, 4> o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) o.v[q] = from_f32<T>(v[q]);
+    store_pack(dw + (int64_t)e * size + i, o);
+  }
+  if (db != nullptr)
+    for (int m = blockIdx.x * 256 + threadIdx.x; m < N; m += gridDim.x * 256) {
+      float v = 0.0f;
+      for (int u = 0; u < n; ++u) v += db_parts[(first + u) * N + m];
+      db[(int64_t)e * N + m] = from_f32<T>(v);
+    }
+}
+
 template <typename F>
 int by_type(int dtype, F&& f) {
   if (dtype == kF32) return f(float{});
@@ -240,12 +395,45 @@ bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
   return M >= 0 && M < ((int64_t)1 << 31) - (1 << 20) && E >= 1 && E <= 65536 && n_in >= 1 && n_in <= kMaxWidth && n_out >= 1 && n_out <= kMaxWidth;
 }
 
+constexpr int kCompute = 256;  // compute units
+
+// Tile sizes of the direct kernels, by work per tile.  256 x 256 reads each operand byte half as often as 128 x 128 and is twice as far
+// from the LDS's read rate, but one tile fills a compute unit: it is taken where it wastes little of itself and there is a tile for
+// every compute unit.  Narrow outputs and few rows per expert take the smaller ones.
+int linear_tile(int64_t rows, int64_t groups, int64_t cols) {
+  const int64_t each = rows / groups;
+  if (cols > 128 && each >= 192 && (rows / 256 + groups) * ((cols + 255) / 256) >= kCompute) return 256;
+  return cols > 64 && each >= 64 ? 128 : 64;
+}
+
+template <typename K>
+void allow_lds(K* kernel, int bytes) {
+  if (bytes > 64 * 1024) hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <typename T, int B, int WM, int WN, bool W_RC>
+int launch_linear_direct(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
+                         hipStream_t s) {
+  constexpr int lds = 4 * B * kTileRowBytes;
+  const int64_t row_tiles = (M + B - 1) / B + E, blocks = row_tiles * ((N + B - 1) / B);
+  PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
+  allow_lds(linear_direct_kernel<T, B, B, WM, WN, W_RC>, lds);
+  linear_direct_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N,
+                                                                                         K, (int)row_tiles, (T*)y);
+  PS_CHECK_LAUNCH();
+}
+
 template <bool W_RC>
 int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, int dtype,
                   void* y, hipStream_t s) {
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const int vb = piece_bytes(sizeof(T), {ldx, N, K}, {x, weight});
+    if (vb == 16) switch (linear_tile(M, E, N)) {
+        case 256: return launch_linear_direct<T, 256, 2, 4, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
+        case 128: return launch_linear_direct<T, 128, 2, 2, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
+        default: return launch_linear_direct<T, 64, 2, 2, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
+      }
     return by_piece<T>(vb, [&](auto piece) {
       constexpr int VB = decltype(piece)::value, BM = 128, BN = 128;
       const int64_t row_tiles = (M + BM - 1) / BM + E, blocks = row_tiles * ((N + BN - 1) / BN);
@@ -255,6 +443,54 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
       PS_CHECK_LAUNCH();
     });
   });
+}
+
+// How the weight gradients are cut: the tile, and the rows of a piece (0: one piece per expert)
+struct DwPlan {
+  int tile, piece;
+  int64_t units;
+};
+DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out) {
+  DwPlan p;
+  const int64_t least = n_in < n_out ? n_in : n_out;
+  auto tiles = [&](int64_t b) { return ((n_in + b - 1) / b) * ((n_out + b - 1) / b) * E; };
+  p.tile = least > 128 && tiles(256) >= kCompute ? 256 : (least > 64 && tiles(128) >= kCompute ? 128 : 64);
+  if (p.tile == 64 && least > 64) p.tile = 128;
+  p.piece = 0;
+  p.units = E;
+  const int64_t each = M / E, t = tiles(p.tile);
+  if (t < 2 * kCompute && each >= 512) {  // pieces for about four workgroups per compute unit, of at least 256 rows
+    const int64_t want = (4 * kCompute + t - 1) / t;
+    int64_t piece = ((each + want - 1) / want + 63) & ~(int64_t)63;
+    p.piece = (int)(piece < 256 ? 256 : piece);
+    p.units = (M + p.piece - 1) / p.piece + E;
+  }
+  return p;
+}
+
+int64_t dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out) {
+  const DwPlan p = dw_plan(M, E, n_in, n_out);
+  return p.piece == 0 ? 0 : p.units * (n_in * n_out + n_out) * (int64_t)sizeof(float);
+}
+
+template <typename T, int B, int WM, int WN, bool SPLIT>
+int launch_dw_tile(const DwPlan& p, const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* offsets, int64_t M, int E, int N, int K,
+                   void* dw, void* db, hipStream_t s) {
+  constexpr int lds = 4 * B * kTileRowBytes;
+  const int64_t blocks = p.units * ((N + B - 1) / B) * ((K + B - 1) / B);
+  PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
+  allow_lds(linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT>, lds);
+  linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy, ldy, (const T*)x, ldx, offsets, M, E, N, K, p.piece,
+                                                                                             (int)p.units, dw, db);
+  PS_CHECK_LAUNCH();
+}
+
+template <typename T, bool SPLIT>
+int launch_dw_direct(const DwPlan& p, const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* offsets, int64_t M, int E, int N, int K,
+                     void* dw, void* db, hipStream_t s) {
+  if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, SPLIT>(p, dy, ldy, x, ldx, offsets, M, E, N, K, dw, db, s);
+  if (p.tile == 128) return launch_dw_tile<T, 128, 2, 2, SPLIT>(p, dy, ldy, x, ldx, offsets, M, E, N, K, dw, db, s);
+  return launch_dw_tile<T, 64, 2, 2, SPLIT>(p, dy, ldy, x, ldx, offsets, M, E, N, K, dw, db, s);
 }
 
 }  // namespace
@@ -275,9 +511,8 @@ extern "C" int ps_expert_linear_dx(const void* dy, int64_t dy_stride, const void
   return launch_linear<true>(dy, dy_stride, weight, nullptr, offsets, M, E, (int)n_in, (int)n_out, dtype, dx, (hipStream_t)stream);
 }
 
-extern "C" int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
-  (void)M, (void)E, (void)n_in, (void)n_out, (void)dtype;
-  return 0;
+extern "C" int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out) {
+  return sizes_ok(M, E, n_in, n_out) ? dw_workspace(M, E, n_in, n_out) : 0;
 }
 
 extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const int32_t* offsets, int64_t M, int E,
@@ -285,16 +520,29 @@ extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void
   PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && x_stride >= n_in && x_stride <= kMaxWidth && dy_stride >= n_out && dy_stride <= kMaxWidth,
              "ps_expert_linear_dw: sizes out of range");
   PS_REQUIRE((M == 0 || (dy != nullptr && x != nullptr)) && offsets != nullptr && dweight != nullptr, "ps_expert_linear_dw: null argument");
-  (void)workspace;
+  const DwPlan p = dw_plan(M, E, n_in, n_out);
+  PS_REQUIRE(p.piece == 0 || workspace != nullptr, "ps_expert_linear_dw: needs its workspace (ps_expert_linear_dw_workspace)");
+  const int N = (int)n_out, K = (int)n_in;
+  hipStream_t s = (hipStream_t)stream;
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const int vb = piece_bytes(sizeof(T), {dy_stride, x_stride, n_in, n_out}, {dy, x});
+    if (vb == 16) {
+      if (p.piece == 0) return launch_dw_direct<T, false>(p, dy, dy_stride, x, x_stride, offsets, M, E, N, K, dweight, dbias, s);
+      float* parts = (float*)workspace;
+      float* db_parts = parts + p.units * n_in * n_out;
+      const int rc = launch_dw_direct<T, true>(p, dy, dy_stride, x, x_stride, offsets, M, E, N, K, parts, dbias != nullptr ? db_parts : nullptr, s);
+      if (rc != 0) return rc;
+      dw_join_kernel<T><<<dim3((unsigned)((n_in * n_out / 4 + 255) / 256), (unsigned)E), 256, 0, s>>>(parts, db_parts, offsets, M, n_in * n_out, N, p.piece,
+                                                                                                     (T*)dweight, (T*)dbias);
+      PS_CHECK_LAUNCH();
+    }
     return by_piece<T>(vb, [&](auto piece) {
       constexpr int VB = decltype(piece)::value, BM = 128, BN = 128;
       const int64_t blocks = (int64_t)E * ((n_out + BM - 1) / BM) * ((n_in + BN - 1) / BN);
       PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
-      linear_dw_kernel<T, BM, BN, 2, 2, VB><<<(unsigned)blocks, 256, 0, (hipStream_t)stream>>>((const T*)dy, dy_stride, (const T*)x, x_stride, offsets, M, E,
-                                                                                            (int)n_out, (int)n_in, (T*)dweight, (T*)dbias);
+      linear_dw_kernel<T, BM, BN, 2, 2, VB><<<(unsigned)blocks, 256, 0, s>>>((const T*)dy, dy_stride, (const T*)x, x_stride, offsets, M, E, N, K,
+                                                                            (T*)dweight, (T*)dbias);
       PS_CHECK_LAUNCH();
     });
   });

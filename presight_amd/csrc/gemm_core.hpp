@@ -171,6 +171,119 @@ __device__ __forceinline__ void tile_mma(const char* a_lds, const char* b_lds, i
   }
 }
 
+// ------------------------------------------------------------------------------------------------ tiles loaded straight into LDS
+// Operands whose pieces are whole 16-byte chunks need no registers on the way: buffer loads write LDS directly, 1 KiB per wave and
+// instruction in lane order, and zeros where the descriptor ends.  The tile keeps the operand's own direction: KC as above, RC as rows of
+// k (BR elements each), from which 16-bit fragments are read with the transposing LDS loads (16 lanes fetch 4 k x 16 rows, each lane ends
+// up with the 4 k of its row) and fp32 ones element by element.  What would collide in the banks is spread by permuting chunks within a
+// tile row, on the global side of the load.
+template <typename T, int BR, int NT, bool RC>
+struct DirectTile {
+  static constexpr int kBytes = BR * kTileRowBytes;
+  static constexpr int N = kBytes / 16 / NT;                    // chunks per thread
+  static constexpr int kRow = RC ? BR * (int)sizeof(T) : kTileRowBytes;  // bytes of a tile row
+  static constexpr int kAcross = kRow / 16;
+  static_assert(kBytes % (16 * NT) == 0 && (!RC || kAcross >= 8), "whole chunks per thread; eight chunks to permute among");
+
+  // 16-bit RC: half a wave reads 32 bytes of the eight rows 8 g + (0..3), g = two neighbours; fp32: 64 bytes of four rows 4 g + q
+  __device__ static int spread(int row) {
+    if constexpr (!RC) {
+      return (row >> 1) & 7;
+    } else if constexpr (sizeof(T) == 4) {
+      return ((row >> 2) & 3) << 2 & (kAcross - 1);
+    } else if constexpr (kAcross >= 16) {
+      return ((row & 3) | ((row >> 3) & 1) << 2) << 1;
+    } else {
+      return (((row >> 1) & 1) | ((row >> 3) & 1) << 1) << 1;  // (rows of 128 bytes: their parity is a bank bit already)
+    }
+  }
+
+  unsigned off[N];  // byte offsets of this thread's chunks from the tile's corner
+  int first[N];     // KC: first k, RC: first row of each chunk
+  __device__ __forceinline__ void setup(unsigned ld_bytes) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int id = i * NT + threadIdx.x, row = id / kAcross, c = (id % kAcross) ^ spread(row);
+      off[i] = row * ld_bytes + c * 16;
+      first[i] = c * kChunk<T>;
+    }
+  }
+  // left: elements of the contiguous direction from the tile's corner on
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t w, int left, char* lds) const {
+    char* base = lds + uniform(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(w, (__attribute__((address_space(3))) void*)(base + i * NT * 16), 16, first[i] < left ? off[i] : kOutside, 0,
+                                               0, 0);
+  }
+  // this lane's fragment of the 16 rows from r0 on (a multiple of 16), half s of the tile's k
+  __device__ static __forceinline__ u32x4 fragment(const char* lds, int r0, int s) {
+    const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    if constexpr (!RC) {
+      const int row = r0 + r;
+      return *reinterpret_cast<const u32x4*>(lds + row * kTileRowBytes + (((s * 4 + g) ^ spread(r)) << 4));
+    } else if constexpr (sizeof(T) == 4) {
+      u32x4 v;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int k = s * 16 + g * 4 + q;
+        v[q] = *reinterpret_cast<const unsigned*>(lds + k * kRow + ((((r0 + r) >> 2) ^ spread(k)) << 4) + (r & 3) * 4);
+      }
+      return v;
+    } else {
+      typedef short s16x4 __attribute__((ext_vector_type(4)));
+      u32x4 v;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = s * 32 + g * 8 + h * 4 + (r >> 2);
+        const char* p = lds + k * kRow + ((((r0 >> 3) + ((r & 3) >> 1)) ^ spread(k)) << 4) + (r & 1) * 8;
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass drops a kernel's stub over a builtin it does not know)
+        const u32x2 o = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+#else
+        const u32x2 o = *reinterpret_cast<const u32x2*>(p);
+#endif
+        v[2 * h] = o[0];
+        v[2 * h + 1] = o[1];
+      }
+      return v;
+    }
+  }
+};
+
+// An operand's tiles along k: `rows` rows (KC) or elements of a row (RC) from the tile's corner `base` on, K of k
+template <typename T, int BR, int NT, bool RC>
+struct DirectSource {
+  DirectTile<T, BR, NT, RC> tile;
+  const T* base;
+  int64_t ld;
+  int rows, K;
+  __device__ __forceinline__ DirectSource(const T* base_, int64_t ld_, int rows_, int K_) : base(base_), ld(ld_), rows(rows_), K(K_) {
+    tile.setup((unsigned)(ld * sizeof(T)));
+  }
+  __device__ __forceinline__ void load(int k0, char* to) const {
+    if constexpr (RC) {
+      const int kr = K - k0 < kTileK<T> ? K - k0 : kTileK<T>;
+      tile.load(window(base + k0 * ld, ((int64_t)(kr - 1) * ld + rows) * sizeof(T)), rows, to);
+    } else {
+      tile.load(window(base + k0, ((int64_t)(rows - 1) * ld + (K - k0)) * sizeof(T)), K - k0, to);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ f32x4 mma_block(u32x4 a, u32x4 b, f32x4 acc) {  // (b's rows are the instruction's rows, as in tile_mma)
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 bf = __builtin_bit_cast(f32x4, b), af = __builtin_bit_cast(f32x4, a);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[q], af[q], acc, 0, 0, 0);
+    return acc;
+  } else if constexpr (__is_same(T, _Float16)) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b), __builtin_bit_cast(f16x8, a), acc, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b), __builtin_bit_cast(bf16x8, a), acc, 0, 0, 0);
+  }
+}
+
 // widest piece (16, 4 or 2 bytes) that divides every byte count and address
 inline int piece_bytes(int size, std::initializer_list<int64_t> elems, std::initializer_list<const void*> ptrs) {
   uint64_t bits = 0;

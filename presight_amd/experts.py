@@ -231,7 +231,7 @@ class _ExpertLinear(torch.autograd.Function):
                 xs = _spaced(x)
                 dw = torch.empty(E, n_out, n_in, device=x.device, dtype=x.dtype)
                 db = torch.empty(E, n_out, device=x.device, dtype=x.dtype) if ctx.has_bias and need_b else None
-                nbytes = lib().ps_expert_linear_dw_workspace(M, E, n_in, n_out, code)
+                nbytes = lib().ps_expert_linear_dw_workspace(M, E, n_in, n_out)
                 ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
                 check(lib().ps_expert_linear_dw(_p(dy), _ld(dy), _p(xs), _ld(xs), _p(offsets), M, E, n_in, n_out, code, _p(dw), _p(db), _p(ws),
                                                 _stream()), "ps_expert_linear_dw")
