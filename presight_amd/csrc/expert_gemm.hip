@@ -271,16 +271,62 @@ __device__ __forceinline__ void direct_loop(char* lds, int K, const DirectSource
   }
 }
 
+// A wave's part of a tile into memory, turned in LDS on the way: four values per lane and row make requests of 8 to 16 bytes (65536 x
+// 1024 bf16: 12.6 million of them, a third of the kernel's time); from a row of the wave's own LDS slice (MI * 16 rows in as many passes
+// as it takes) every lane writes 16 bytes of whole 64- to 256-byte rows.  No other wave reads the slice, and the tiles are done with.
+template <typename T, int MI, int NJ, int SLICE>
+__device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slice, T* __restrict__ y, int64_t ldy, int rows, int cols, int m0, int n0,
+                                                const T* __restrict__ bias) {
+  constexpr int kRow = NJ * 16 * (int)sizeof(T), kAcross = kRow / 16;  // bytes and chunks of a row
+  constexpr int kFit = SLICE / (16 * kRow), kPass = kFit < MI ? kFit : MI;  // blocks of 16 rows per pass
+  constexpr int kSpread = kAcross < 8 ? kAcross - 1 : 7;
+  static_assert(kPass >= 1 && MI % kPass == 0, "whole blocks of rows per pass");
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  float b[NJ][4] = {};
+  if (bias != nullptr) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = n0 + j * 16 + g * 4 + q;
+        if (n < cols) b[j][q] = to_f32(bias[n]);
+      }
+  }
+#pragma unroll
+  for (int p = 0; p < MI / kPass; ++p) {
+#pragma unroll
+    for (int i = 0; i < kPass; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        Pack<T, 4> o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o.v[q] = from_f32<T>(acc[p * kPass + i][j][q] + b[j][q]);
+        const int row = i * 16 + r, byte = (j * 16 + g * 4) * (int)sizeof(T);
+        store_pack(reinterpret_cast<T*>(slice + row * kRow + (((byte >> 4) ^ (row & kSpread)) << 4) + (byte & 15)), o);
+      }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int t = 0; t < kPass * 16 * kAcross / 64; ++t) {
+      const int id = t * 64 + lane, row = id / kAcross, c = id % kAcross, m = m0 + p * kPass * 16 + row, n = n0 + c * kChunk<T>;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(slice + row * kRow + ((c ^ (row & kSpread)) << 4));
+      if (m < rows && n < cols) *reinterpret_cast<u32x4*>(y + m * ldy + n) = v;
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool W_RC>
 __global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight,
                                                                      const T* __restrict__ bias, const int* __restrict__ offsets, int64_t M, int E,
                                                                      int N, int K, int row_tiles, T* __restrict__ y) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int n_tiles = (N + BN - 1) / BN;
-  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles;
-  const RowTile t = find_row_tile(offsets, E, M, BM, tm, row_tiles);
-  const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
+  const TileAt at = patched_tile(blockIdx.x, row_tiles, (N + BN - 1) / BN);
+  if (!at.valid) return;
+  const RowTile t = find_row_tile(offsets, E, M, BM, at.m, row_tiles);
+  const int n0 = at.n * BN, cols = N - n0 < BN ? N - n0 : BN;
   if (t.expert < 0) {
     clear_outside<T, BM>(offsets, E, M, t, y, N, n0, cols);
     return;
@@ -290,8 +336,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __
   const DirectSource<T, BN, NT, W_RC> sb(wb, W_RC ? N : K, W_RC ? N - n0 : cols, K);
   f32x4 acc[MI][NJ], none[1];
   direct_loop<T, BM, BN, WM, WN, false, W_RC, false>(lds, K, sa, sb, acc, none, false);
-  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-  store_tile<T, MI, NJ>(acc, y + t.row0 * N + n0, N, t.rows, cols, wm, wn, bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
+  const int wave = uniform(threadIdx.x >> 6), wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  constexpr int kSlice = 2 * (BM + BN) * kTileRowBytes / (WM * WN);
+  store_tile_rows<T, MI, NJ, kSlice>(acc, lds + wave * kSlice, y + t.row0 * N + n0, N, t.rows, cols, wm, wn,
+                                     bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
 }
 
 // Weight gradients.  Few and small weights with many rows would leave most of the chip idle: then (SPLIT) the experts' rows are cut into
@@ -306,7 +354,10 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_dw_direct_kernel(const T*
   using Out = std::conditional_t<SPLIT, float, T>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int n_tiles = (K + BN - 1) / BN, m_tiles = (N + BM - 1) / BM;
-  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles % m_tiles, unit = blockIdx.x / (n_tiles * m_tiles);
+  // (a unit's tiles share all of their operands: they stay on one XCD)
+  const int tiles = n_tiles * m_tiles, slot = blockIdx.x / kXcds, unit = slot / tiles * kXcds + blockIdx.x % kXcds;
+  if (unit >= units) return;
+  const int tn = slot % n_tiles, tm = slot % tiles / n_tiles;
   int64_t row0;
   int len;
   if constexpr (SPLIT) {
@@ -322,12 +373,14 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_dw_direct_kernel(const T*
   const int m0 = tm * BM, n0 = tn * BN;
   const DirectSource<T, BM, NT, true> sa(dy + row0 * ldy + m0, ldy, N - m0, len);
   const DirectSource<T, BN, NT, true> sb(x + row0 * ldx + n0, ldx, K - n0, len);
-  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
+  const int wave = uniform(threadIdx.x >> 6), wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const bool sums = db != nullptr && tn == 0 && wn == 0;
   f32x4 acc[MI][NJ], row_sums[MI];
   direct_loop<T, BM, BN, WM, WN, true, true, true>(lds, len, sa, sb, acc, row_sums, sums);
   Out* o = reinterpret_cast<Out*>(dw) + (int64_t)unit * N * K + (int64_t)m0 * K + n0;
-  store_tile<Out, MI, NJ>(acc, o, K, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn, nullptr);
+  constexpr int kSlice = 2 * (BM + BN) * kTileRowBytes / (WM * WN);
+  store_tile_rows<Out, MI, NJ, kSlice>(acc, lds + wave * kSlice, o, K, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn,
+                                       static_cast<const Out*>(nullptr));
   if (sums && (threadIdx.x & 63) < 16) {
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
@@ -415,7 +468,7 @@ template <typename T, int B, int WM, int WN, bool W_RC>
 int launch_linear_direct(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
                          hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t row_tiles = (M + B - 1) / B + E, blocks = row_tiles * ((N + B - 1) / B);
+  const int64_t row_tiles = (M + B - 1) / B + E, blocks = patched_blocks(row_tiles, (N + B - 1) / B);
   PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
   allow_lds(linear_direct_kernel<T, B, B, WM, WN, W_RC>, lds);
   linear_direct_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N,
@@ -428,7 +481,7 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
                   void* y, hipStream_t s) {
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vb = piece_bytes(sizeof(T), {ldx, N, K}, {x, weight});
+    const int vb = piece_bytes(sizeof(T), {ldx, N, K}, {x, weight, y});
     if (vb == 16) switch (linear_tile(M, E, N)) {
         case 256: return launch_linear_direct<T, 256, 2, 4, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
         case 128: return launch_linear_direct<T, 128, 2, 2, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
@@ -477,7 +530,7 @@ template <typename T, int B, int WM, int WN, bool SPLIT>
 int launch_dw_tile(const DwPlan& p, const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* offsets, int64_t M, int E, int N, int K,
                    void* dw, void* db, hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t blocks = p.units * ((N + B - 1) / B) * ((K + B - 1) / B);
+  const int64_t blocks = (p.units + kXcds - 1) / kXcds * kXcds * ((N + B - 1) / B) * ((K + B - 1) / B);
   PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
   allow_lds(linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT>, lds);
   linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy, ldy, (const T*)x, ldx, offsets, M, E, N, K, p.piece,
@@ -526,7 +579,7 @@ extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void
   hipStream_t s = (hipStream_t)stream;
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vb = piece_bytes(sizeof(T), {dy_stride, x_stride, n_in, n_out}, {dy, x});
+    const int vb = piece_bytes(sizeof(T), {dy_stride, x_stride, n_in, n_out}, {dy, x, dweight, workspace});
     if (vb == 16) {
       if (p.piece == 0) return launch_dw_direct<T, false>(p, dy, dy_stride, x, x_stride, offsets, M, E, N, K, dweight, dbias, s);
       float* parts = (float*)workspace;
