@@ -286,22 +286,21 @@ __device__ __forceinline__ f32x4 mma_block(u32x4 a, u32x4 b, f32x4 acc) {  // (b
 
 // ------------------------------------------------------------------------------------------------ which tile where
 // Workgroups go round the eight XCDs, each with an L2 of its own.  A grid of m x n tiles is cut into patches of 4 x 8 tiles that share
-// their operands' rows, and a patch stays on one XCD: about what runs there at a time.  (65536 x 2048 x 1024 bf16 over 32 experts, tiles
-// of 256 dealt out one by one: every XCD reads nearly everything.)
-constexpr int kXcds = 8, kPatchM = 4, kPatchN = 8;
+// their operands' rows (fewer than 8 across: 32 in all), and a patch stays on one XCD: what runs there at a time.
+constexpr int kXcds = 8, kPatch = 32, kPatchN = 8;
 struct TileAt {
   int m, n;
   bool valid;
 };
 __host__ __device__ inline int64_t patched_blocks(int64_t m_tiles, int64_t n_tiles) {
-  const int64_t pn = n_tiles < kPatchN ? n_tiles : kPatchN;
-  const int64_t patches = ((m_tiles + kPatchM - 1) / kPatchM) * ((n_tiles + pn - 1) / pn);
-  return (patches + kXcds - 1) / kXcds * kXcds * kPatchM * pn;
+  const int64_t pn = n_tiles < kPatchN ? n_tiles : kPatchN, pm = kPatch / pn;
+  const int64_t patches = ((m_tiles + pm - 1) / pm) * ((n_tiles + pn - 1) / pn);
+  return (patches + kXcds - 1) / kXcds * kXcds * pm * pn;
 }
 __device__ __forceinline__ TileAt patched_tile(int block, int m_tiles, int n_tiles) {
-  const int pn = n_tiles < kPatchN ? n_tiles : kPatchN, size = kPatchM * pn, across = (n_tiles + pn - 1) / pn;
+  const int pn = n_tiles < kPatchN ? n_tiles : kPatchN, pm = kPatch / pn, size = pm * pn, across = (n_tiles + pn - 1) / pn;
   const int slot = block / kXcds, patch = slot / size * kXcds + block % kXcds, in = slot % size;
-  const int m = patch / across * kPatchM + in / pn, n = patch % across * pn + in % pn;
+  const int m = patch / across * pm + in / pn, n = patch % across * pn + in % pn;
   return {m, n, m < m_tiles && n < n_tiles};
 }
 

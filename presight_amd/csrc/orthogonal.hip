@@ -193,116 +193,173 @@ struct Operands {
   int ra, rb, k;              // k: padded, and the rows' distance
 };
 
-constexpr int kPairTile = 128;
+// A workgroup's tile: 128 x 128, eight waves of 64 x 32.  Two tiles of 64 k of all four planes (hi and lo of either operand, 64 KiB) in
+// LDS: the loads of the next tile run beside this one's 384 matrix instructions, three on every pair of fragments.  The two small
+// products add up apart from the large one: each of their additions to it would cost it another rounding.
+//
+// The result leaves through LDS both as it is and turned, as rows of 256 bytes: X needs both ways round, and of a symmetric result only
+// the tiles on and below the diagonal are computed and their turned copies are the others.
+constexpr int kPairTile = 128, kPairThreads = 512, kPairPlane = kPairTile * kTileRowBytes;  // bytes of one plane's tile
+constexpr int kPairLds = 2 * 4 * kPairPlane;
+
+// byte of element `col` (fp16 or fp32) in row `row` of a turned-out tile: 16-byte chunks spread so that the 16 rows that a wave writes at a
+// time and the 4 columns of a lane meet different banks
+template <typename V>
+__device__ __forceinline__ int out_addr(int row, int col) {
+  const int byte = col * (int)sizeof(V);
+  return row * kPairTile * (int)sizeof(V) + (((byte >> 4) ^ (row & 15)) << 4) + (byte & 15);
+}
 
 template <typename T, Product WHAT>
-__global__ __launch_bounds__(256) void ns_product_kernel(Operands o, Shape h, Work w, int step, Poly c, Result res) {
-  constexpr int BM = kPairTile, BN = kPairTile, NT = 256, MI = 4, NJ = 4;
-  constexpr int kPart = BM * kTileRowBytes;  // bytes of one plane's tile
-  __shared__ __attribute__((aligned(16))) char lds[4 * kPart];
-  const int tm_n = (o.ra + BM - 1) / BM, tn_n = (o.rb + BN - 1) / BN;
-  const int tn = blockIdx.x % tn_n, tm = blockIdx.x / tn_n % tm_n;
-  const int64_t batch = blockIdx.x / (tn_n * tm_n);
-  const int m0 = tm * BM, n0 = tn * BN;
-  const int rows = o.ra - m0 < BM ? o.ra - m0 : BM, cols = o.rb - n0 < BN ? o.rb - n0 : BN;
-  const _Float16* a = o.a + (batch * o.ra + m0) * o.k;
-  const _Float16* b = o.b + (batch * o.rb + n0) * o.k;
-  const unsigned ld = (unsigned)o.k * 2;
-  TileLoader<_Float16, BM, NT, 16, false> ah, al, bh, bl;
-  auto load = [&](int k0) {
-    const int64_t abytes = ((int64_t)(rows - 1) * o.k + (o.k - k0)) * 2, bbytes = ((int64_t)(cols - 1) * o.k + (o.k - k0)) * 2;
-    ah.load(window(a + k0, abytes), ld, o.k - k0);
-    al.load(window(a + o.a_plane + k0, abytes), ld, o.k - k0);
-    bh.load(window(b + k0, bbytes), ld, o.k - k0);
-    bl.load(window(b + o.b_plane + k0, bbytes), ld, o.k - k0);
+__global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Shape h, Work w, int step, Poly c, Result res) {
+  constexpr int B = kPairTile, NT = kPairThreads, MI = 4, NJ = 2;
+  constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
+  using Tile = DirectTile<_Float16, B, NT, false>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  const int m_tiles = (o.ra + B - 1) / B, n_tiles = (o.rb + B - 1) / B;
+  const int64_t batch = blockIdx.y;
+  int tm, tn;
+  if constexpr (kSymmetric) {  // blockIdx.x counts the tiles tm >= tn row by row
+    tm = (int)((sqrtf(8.0f * blockIdx.x + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > (int)blockIdx.x) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= (int)blockIdx.x) ++tm;
+    tm = uniform(tm);
+    tn = blockIdx.x - tm * (tm + 1) / 2;
+  } else {
+    const TileAt at = patched_tile(blockIdx.x, m_tiles, n_tiles);
+    if (!at.valid) return;
+    tm = at.m, tn = at.n;
+  }
+  const int m0 = tm * B, n0 = tn * B;
+  const int rows = o.ra - m0 < B ? o.ra - m0 : B, cols = o.rb - n0 < B ? o.rb - n0 : B;
+  const _Float16* pa = o.a + (batch * o.ra + m0) * o.k;
+  const _Float16* pb = o.b + (batch * o.rb + n0) * o.k;
+  const DirectSource<_Float16, B, NT, false> ah(pa, o.k, rows, o.k), al(pa + o.a_plane, o.k, rows, o.k), bh(pb, o.k, cols, o.k),
+      bl(pb + o.b_plane, o.k, cols, o.k);
+  auto load = [&](int k0, char* to) {
+    ah.load(k0, to);
+    al.load(k0, to + kPairPlane);
+    bh.load(k0, to + 2 * kPairPlane);
+    bl.load(k0, to + 3 * kPairPlane);
   };
-  // the two small products add up apart from the large one: each of their additions to it would cost it another rounding
+  const int wave = threadIdx.x >> 6, wm = (wave >> 2) * 64, wn = (wave & 3) * 32;
   f32x4 acc[MI][NJ], fine[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = fine[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int wave = threadIdx.x >> 6, wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-  load(0);
-  for (int k0 = 0; k0 < o.k; k0 += 64) {
+  load(0, lds);
+  __syncthreads();
+  for (int k0 = 0, cur = 0; k0 < o.k; k0 += kTileK<_Float16>, cur ^= 1) {
+    const char* t = lds + cur * 4 * kPairPlane;
+    if (k0 + kTileK<_Float16> < o.k) load(k0 + kTileK<_Float16>, lds + (cur ^ 1) * 4 * kPairPlane);
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      u32x4 fa[2][MI], fb[2][NJ];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) fb[p][j] = Tile::fragment(t + (2 + p) * kPairPlane, wn + j * 16, s);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) fa[p][i] = Tile::fragment(t + p * kPairPlane, wm + i * 16, s);
+      }
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          acc[i][j] = mma_block<_Float16>(fa[0][i], fb[0][j], acc[i][j]);
+          fine[i][j] = mma_block<_Float16>(fa[0][i], fb[1][j], fine[i][j]);
+          fine[i][j] = mma_block<_Float16>(fa[1][i], fb[0][j], fine[i][j]);
+        }
+    }
     __syncthreads();
-    ah.store(lds);
-    al.store(lds + kPart);
-    bh.store(lds + 2 * kPart);
-    bl.store(lds + 3 * kPart);
-    __syncthreads();
-    if (k0 + 64 < o.k) load(k0 + 64);
-    tile_mma<_Float16, MI, NJ>(lds, lds + 2 * kPart, wm, wn, acc);
-    tile_mma<_Float16, MI, NJ>(lds, lds + 3 * kPart, wm, wn, fine);
-    tile_mma<_Float16, MI, NJ>(lds + kPart, lds + 2 * kPart, wm, wn, fine);
   }
   const float ratio = ratio_at(w.ratio[batch], step, c.grow);
   // kPoly: a + b r^2 S^ + c r^4 S^ S^, formed in 64 bits: an error of a coefficient would be common to all entries and grow like a
   // singular value's, and it is the small product of a step | kApply: over the step's growth of r | kLast: X = r X^
-  const double r2 = (double)ratio * ratio, pb = c.b * r2 / kPlaneScale, pc = c.c * r2 * r2 * kProductScale;
+  const double r2 = (double)ratio * ratio, cb = c.b * r2 / kPlaneScale, cc = c.c * r2 * r2 * kProductScale;
   const float out_scale = WHAT == kApply ? kProductScale * (ratio > 0.0f ? ratio / ratio_at(ratio, 1, c.grow) : 1.0f)
                                          : (WHAT == kLast ? kProductScale * ratio : kProductScale);
-  _Float16* const xt_next = w.xt[(step + 1) & 1];
   const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  constexpr int kOut = B * B * 2;  // bytes of a plane's tile: hi, lo, then hi and lo turned
 #pragma unroll
   for (int i = 0; i < MI; ++i) {
-    const int m = m0 + wm + i * 16 + r;
-    if (m >= (WHAT == kApply ? h.sp : o.ra)) continue;
+    const int m = wm + i * 16 + r;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+    for (int j = 0; j < NJ; ++j) {
+      const int n = wn + j * 16 + g * 4;
+      if constexpr (WHAT == kLast) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn + j * 16 + g * 4 + q;
-        const float sum = acc[i][j][q] + fine[i][j][q];
-        float v = sum * out_scale;
-        _Float16 hi, lo;
-        if constexpr (WHAT == kGram || WHAT == kPoly) {
-          if (n >= h.sp) continue;
-          const int64_t at = (batch * h.s + m) * h.sp + n;
-          if (n >= h.s) {
-            hi = lo = (_Float16)0.0f;  // the padding of k in the products to come
-          } else if constexpr (WHAT == kPoly) {
-            split(pc * sum + (pb * ((double)(float)w.gram[at] + (double)(float)w.gram[w.s_plane + at]) + (m == n ? c.a : 0.0)), hi, lo);
-          } else {
-            split(v, hi, lo);
-          }
-          _Float16* out = WHAT == kGram ? w.gram : w.poly;
-          out[at] = hi;
-          out[w.s_plane + at] = lo;
-        } else if constexpr (WHAT == kApply) {
-          if (n >= h.lp) continue;
-          if (n >= h.l || m >= h.s) v = 0.0f;  // the padding of k, both ways round
-          split(v, hi, lo);
-          if (m < h.s) {
-            const int64_t at = (batch * h.s + m) * h.lp + n;
-            w.x[at] = hi;
-            w.x[w.x_plane + at] = lo;
-          }
-          if (n < h.l) {
-            const int64_t t = (batch * h.l + n) * h.sp + m;
-            xt_next[t] = hi;
-            xt_next[w.xt_plane + t] = lo;
-          }
-        } else {
-          if (n >= h.l) continue;
-          const int64_t at = batch * h.m * h.n + (h.tall ? (int64_t)n * h.n + m : (int64_t)m * h.n + n);
-          if (res.update) {
-            float* p = reinterpret_cast<float*>(res.out) + at;
-            *p = res.keep * *p - res.rate * v;
-          } else {
-            reinterpret_cast<T*>(res.out)[at] = from_f32<T>(v);
+        for (int q = 0; q < 4; ++q) {
+          const float v = (acc[i][j][q] + fine[i][j][q]) * out_scale;
+          *reinterpret_cast<float*>(lds + (h.tall ? out_addr<float>(n + q, m) : out_addr<float>(m, n + q))) = v;
+        }
+      } else {
+        Pack<_Float16, 4> hi, lo, gh, gl;
+        if constexpr (WHAT == kPoly) {
+          gh = gl = Pack<_Float16, 4>{};
+          if (m < rows && n < cols) {  // (rows are padded to 64: whole packs)
+            const int64_t at = (batch * h.s + m0 + m) * h.sp + n0 + n;
+            gh = load_pack<_Float16, 4>(w.gram + at);
+            gl = load_pack<_Float16, 4>(w.gram + w.s_plane + at);
           }
         }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float sum = acc[i][j][q] + fine[i][j][q];
+          if constexpr (WHAT == kPoly) {
+            const double one = m0 + m == n0 + n + q && m < rows ? c.a : 0.0;  // (rows and columns of the padding stay zero)
+            split(cc * sum + (cb * ((double)(float)gh.v[q] + (double)(float)gl.v[q]) + one), hi.v[q], lo.v[q]);
+          } else {
+            split(sum * out_scale, hi.v[q], lo.v[q]);
+          }
+          *reinterpret_cast<_Float16*>(lds + 2 * kOut + out_addr<_Float16>(n + q, m)) = hi.v[q];
+          *reinterpret_cast<_Float16*>(lds + 3 * kOut + out_addr<_Float16>(n + q, m)) = lo.v[q];
+        }
+        store_pack(reinterpret_cast<_Float16*>(lds + out_addr<_Float16>(m, n)), hi);
+        store_pack(reinterpret_cast<_Float16*>(lds + kOut + out_addr<_Float16>(m, n)), lo);
       }
+    }
+  }
+  __syncthreads();
+  if constexpr (WHAT == kLast) {
+    const int r0 = h.tall ? n0 : m0, c0 = h.tall ? m0 : n0, rn = h.tall ? cols : rows, cn = h.tall ? rows : cols;
+    const int64_t base = batch * h.m * h.n + (int64_t)r0 * h.n + c0;
+    for (int id = threadIdx.x; id < B * B; id += NT) {
+      const int row = id / B, col = id % B;
+      if (row >= rn || col >= cn) continue;
+      const float v = *reinterpret_cast<const float*>(lds + out_addr<float>(row, col));
+      const int64_t at = base + (int64_t)row * h.n + col;
+      if (res.update) {
+        float* p = reinterpret_cast<float*>(res.out) + at;
+        *p = res.keep * *p - res.rate * v;
+      } else {
+        reinterpret_cast<T*>(res.out)[at] = from_f32<T>(v);
+      }
+    }
+  } else {
+    _Float16* same = (WHAT == kGram ? w.gram : (WHAT == kPoly ? w.poly : w.x)) + batch * h.s * (kSymmetric ? h.sp : h.lp);
+    _Float16* turned = kSymmetric ? same : w.xt[(step + 1) & 1] + batch * h.l * h.sp;
+    const int64_t same_plane = kSymmetric ? w.s_plane : w.x_plane, turned_plane = kSymmetric ? w.s_plane : w.xt_plane;
+    const int same_ld = kSymmetric ? h.sp : h.lp, turned_ld = h.sp;
+    for (int id = threadIdx.x; id < 4 * B * (B / 8); id += NT) {
+      const int part = id / (B * (B / 8)), row = id / (B / 8) % B, col = id % (B / 8) * 8;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + part * kOut + out_addr<_Float16>(row, col));
+      if (part < 2) {
+        if (row < rows && n0 + col < same_ld) *reinterpret_cast<u32x4*>(same + (part & 1) * same_plane + (int64_t)(m0 + row) * same_ld + n0 + col) = v;
+      } else if (!kSymmetric || tm != tn) {
+        if (row < cols && m0 + col < turned_ld) *reinterpret_cast<u32x4*>(turned + (part & 1) * turned_plane + (int64_t)(n0 + row) * turned_ld + m0 + col) = v;
+      }
+    }
   }
 }
 
-int64_t pair_tiles(int64_t ra, int64_t rb, int64_t B) { return ((ra + kPairTile - 1) / kPairTile) * ((rb + kPairTile - 1) / kPairTile) * B; }
-
 template <typename T, Product WHAT>
 void launch_product(const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res, hipStream_t s) {
-  const int64_t tiles = pair_tiles(o.ra, o.rb, B);
-  ns_product_kernel<T, WHAT><<<(unsigned)tiles, 256, 0, s>>>(o, h, w, step, c, res);
+  const int64_t m = (o.ra + kPairTile - 1) / kPairTile, n = (o.rb + kPairTile - 1) / kPairTile;
+  const int64_t blocks = WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : patched_blocks(m, n);
+  hipFuncSetAttribute((const void*)ns_product_kernel<T, WHAT>, hipFuncAttributeMaxDynamicSharedMemorySize, kPairLds);
+  ns_product_kernel<T, WHAT><<<dim3((unsigned)blocks, (unsigned)B), kPairThreads, kPairLds, s>>>(o, h, w, step, c, res);
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -492,8 +549,7 @@ int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Pol
 constexpr int64_t kMaxSide = 1 << 20;
 
 bool sizes_ok(int64_t B, int64_t m, int64_t n, int steps) {
-  return B >= 0 && B <= 65535 && m >= 0 && n >= 0 && m <= kMaxSide && n <= kMaxSide && steps >= 1 && steps <= 64 && (m < n ? m : n) <= 16384 &&
-         pair_tiles(m, n, B) < ((int64_t)1 << 31);
+  return B >= 0 && B <= 65535 && m >= 0 && n >= 0 && m <= kMaxSide && n <= kMaxSide && steps >= 1 && steps <= 64 && (m < n ? m : n) <= 16384;
 }
 
 }  // namespace
