@@ -3,8 +3,8 @@
 //     y[p]  = W_e x[p] + b_e                     tiles of (rows of one expert) x (out),  k = in     x k-contiguous, W k-contiguous
 //     dx[p] = W_e^T dy[p]                        tiles of (rows of one expert) x (in),   k = out    dy k-contiguous, W row-contiguous
 //     dW_e  = sum_p dy[p] x[p]^T, db_e = sum_p dy[p]   tiles of (out) x (in) of one expert, k = its rows, both row-contiguous
-// The experts' lengths are known on the device only.  A launch holds ceil(M / BM) + E row tiles, which is enough for any split of the
-// rows; every workgroup finds its expert and tile from the offsets, and the workgroups left over clear the rows of nobody.
+// The experts' lengths are known on the device only.  A launch holds ceil(M / BM) + E row tiles and one workgroup more, which is enough for
+// any split of the rows; every workgroup finds its expert and tile from the offsets, and those left over clear the rows of nobody.
 #include <type_traits>
 #include "gemm_core.hpp"
 
@@ -13,55 +13,65 @@ namespace {
 using namespace ps;
 
 struct RowTile {
-  int expert;    // -1: left over
-  int64_t row0;  // first row of the tile | left over: index among the left-over tiles
-  int rows;      // rows of the tile      | left over: how many there are
+  int expert;
+  int64_t row0;  // first row of the tile
+  int rows;      // rows of the tile
 };
 
 __device__ __forceinline__ int64_t bounded(int v, int64_t M) { return v < 0 ? 0 : (v > M ? M : v); }
 
-// Which expert's rows tile t (of `piece` rows) holds, uniform over the wave: a prefix sum of tiles over the experts, 64 at a time.
-__device__ __forceinline__ RowTile find_row_tile(const int* __restrict__ offsets, int E, int64_t M, int piece, int t, int tiles) {
-  const int lane = threadIdx.x & 63;
-  int base = 0;
-  for (int e0 = 0; e0 < E; e0 += 64) {
-    const int e = e0 + lane;
-    int64_t lo = 0, hi = 0;
+// The tiles of `piece` rows that the experts' rows make: a prefix sum over the experts, one per lane, 64 at a time.  Up to 64 experts the
+// lanes keep what they have read.
+struct RowTiles {
+  const int* offsets;
+  int64_t M;
+  int E, piece;
+  int lo, len, incl;  // of this lane's expert in the last 64 scanned; incl: tiles up to and with it
+  int total;          // tiles in all
+
+  __device__ __forceinline__ int scan(int e0) {  // -> tiles of these 64 experts
+    const int lane = threadIdx.x & 63, e = e0 + lane;
+    int64_t first = 0, end = 0;
     if (e < E) {
-      lo = bounded(offsets[e], M);
-      hi = bounded(offsets[e + 1], M);
+      first = bounded(offsets[e], M);
+      end = bounded(offsets[e + 1], M);
     }
-    const int len = hi > lo ? (int)(hi - lo) : 0;
-    int incl = (len + piece - 1) / piece;
+    lo = (int)first;
+    len = end > first ? (int)(end - first) : 0;
+    incl = (len + piece - 1) / piece;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int o = __shfl_up(incl, d, 64);
       if (lane >= d) incl += o;
     }
-    const int all = __shfl(incl, 63, 64);
-    if (t < base + all) {
-      const int who = uniform(__ffsll((long long)__ballot(t < base + incl)) - 1);
-      const int n = (len + piece - 1) / piece;
-      const int k = t - base - (__shfl(incl, who, 64) - __shfl(n, who, 64));
-      const int row0 = __shfl((int)lo, who, 64) + k * piece, left = __shfl(len, who, 64) - k * piece;
-      return {uniform(e0 + who), (int64_t)uniform(row0), uniform(left < piece ? left : piece)};
-    }
-    base += all;
+    return __builtin_amdgcn_readlane(incl, 63);
   }
-  return {-1, (int64_t)uniform(t - base), uniform(tiles - base)};
-}
+  __device__ __forceinline__ RowTiles(const int* offsets_, int E_, int64_t M_, int piece_) : offsets(offsets_), M(M_), E(E_), piece(piece_), total(0) {
+    for (int e0 = 0; e0 < E; e0 += 64) total += scan(e0);
+  }
+  // tile t < total, uniform over the wave
+  __device__ __forceinline__ RowTile find(int t) {
+    int e0 = 0, base = 0;
+    if (E > 64)
+      for (;; e0 += 64) {
+        const int n = scan(e0);
+        if (t < base + n) break;
+        base += n;
+      }
+    const int who = uniform(__ffsll((long long)__ballot(t < base + incl)) - 1);
+    const int n = __builtin_amdgcn_readlane(len, who);
+    const int k = t - base - (__builtin_amdgcn_readlane(incl, who) - (n + piece - 1) / piece);
+    return {e0 + who, (int64_t)__builtin_amdgcn_readlane(lo, who) + k * piece, n - k * piece < piece ? n - k * piece : piece};
+  }
+};
 
-// zeros to columns [n0, n0 + cols) of the rows before offsets[0] and from offsets[E] on, shared out over the left-over tiles
-template <typename T, int BM>
-__device__ __forceinline__ void clear_outside(const int* __restrict__ offsets, int E, int64_t M, const RowTile& t, T* __restrict__ y, int N, int n0, int cols) {
+// zeros to the rows before offsets[0] and from offsets[E] on, shared out over `many` workgroups
+template <typename T>
+__device__ __forceinline__ void clear_outside(const int* __restrict__ offsets, int E, int64_t M, int me, int many, T* __restrict__ y, int N) {
   const int64_t head = bounded(offsets[0], M), end = bounded(offsets[E], M), tail0 = end > head ? end : head;
-  const int64_t outside = head + (M - tail0);
-  for (int64_t q0 = t.row0 * BM; q0 < outside; q0 += (int64_t)t.rows * BM) {
-    for (int i = threadIdx.x; i < BM * cols; i += blockDim.x) {
-      const int64_t q = q0 + i / cols;
-      if (q < outside) y[(q < head ? q : tail0 + (q - head)) * N + n0 + i % cols] = from_f32<T>(0.0f);
-    }
-  }
+  const int64_t count = (head + (M - tail0)) * N, step = (int64_t)many * blockDim.x;
+  const int64_t first = head * N;
+  for (int64_t i = (int64_t)me * blockDim.x + threadIdx.x; i < count; i += step) y[i < first ? i : tail0 * N + (i - first)] = from_f32<T>(0.0f);
 }
 
 // A workgroup's tile into memory: four consecutive n per lane and block
@@ -100,18 +110,18 @@ __device__ __forceinline__ void store_tile(f32x4 (&acc)[MI][NJ], T* __restrict__
 // y[p] = sum_k x[p][k] W(n,k) (+ bias): W_RC = false: weight rows are k-contiguous (forward), true: n-contiguous (input gradient)
 template <typename T, int BM, int BN, int WM, int WN, int VB, bool W_RC>
 __global__ __launch_bounds__(64 * WM * WN) void linear_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias,
-                                                              const int* __restrict__ offsets, int64_t M, int E, int N, int K, int row_tiles,
-                                                              T* __restrict__ y) {
+                                                              const int* __restrict__ offsets, int64_t M, int E, int N, int K, T* __restrict__ y) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16, BK = kTileK<T>;
   __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * kTileRowBytes];
   const int n_tiles = (N + BN - 1) / BN;
   const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles;
-  const RowTile t = find_row_tile(offsets, E, M, BM, tm, row_tiles);
-  const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
-  if (t.expert < 0) {
-    clear_outside<T, BM>(offsets, E, M, t, y, N, n0, cols);
+  RowTiles tiles(offsets, E, M, BM);
+  if (tm >= tiles.total) {
+    clear_outside<T>(offsets, E, M, blockIdx.x - tiles.total * n_tiles, gridDim.x - tiles.total * n_tiles, y, N);
     return;
   }
+  const RowTile t = tiles.find(tm);
+  const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
   const T* xa = x + t.row0 * ldx;
   const T* wb = weight + (int64_t)t.expert * N * K + (W_RC ? (int64_t)n0 : (int64_t)n0 * K);
   const unsigned lda = (unsigned)(ldx * sizeof(T)), ldb = (unsigned)((W_RC ? N : K) * sizeof(T));
@@ -320,17 +330,18 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
 template <typename T, int BM, int BN, int WM, int WN, bool W_RC>
 __global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight,
                                                                      const T* __restrict__ bias, const int* __restrict__ offsets, int64_t M, int E,
-                                                                     int N, int K, int row_tiles, T* __restrict__ y) {
+                                                                     int N, int K, T* __restrict__ y) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const TileAt at = patched_tile(blockIdx.x, row_tiles, (N + BN - 1) / BN);
-  if (!at.valid) return;
-  const RowTile t = find_row_tile(offsets, E, M, BM, at.m, row_tiles);
-  const int n0 = at.n * BN, cols = N - n0 < BN ? N - n0 : BN;
-  if (t.expert < 0) {
-    clear_outside<T, BM>(offsets, E, M, t, y, N, n0, cols);
+  RowTiles tiles(offsets, E, M, BM);
+  const int n_tiles = (N + BN - 1) / BN, all = tiles.total * n_tiles, place = xcd_place(blockIdx.x, all);
+  if (place < 0) {
+    clear_outside<T>(offsets, E, M, xcd_spare(blockIdx.x, gridDim.x, all), gridDim.x - all, y, N);
     return;
   }
+  const TileAt at = patched_tile(place, tiles.total, n_tiles);
+  const RowTile t = tiles.find(at.m);
+  const int n0 = at.n * BN, cols = N - n0 < BN ? N - n0 : BN;
   const T* wb = weight + (int64_t)t.expert * N * K + (W_RC ? (int64_t)n0 : (int64_t)n0 * K);
   const DirectSource<T, BM, NT, false> sa(x + t.row0 * ldx, ldx, t.rows, K);
   const DirectSource<T, BN, NT, W_RC> sb(wb, W_RC ? N : K, W_RC ? N - n0 : cols, K);
@@ -349,20 +360,23 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __
 template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void linear_dw_direct_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
                                                                         const int* __restrict__ offsets, int64_t M, int E, int N, int K, int piece,
-                                                                        int units, void* __restrict__ dw, void* __restrict__ db) {
+                                                                        void* __restrict__ dw, void* __restrict__ db) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
   using Out = std::conditional_t<SPLIT, float, T>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int n_tiles = (K + BN - 1) / BN, m_tiles = (N + BM - 1) / BM;
   // (a unit's tiles share all of their operands: they stay on one XCD)
-  const int tiles = n_tiles * m_tiles, slot = blockIdx.x / kXcds, unit = slot / tiles * kXcds + blockIdx.x % kXcds;
-  if (unit >= units) return;
-  const int tn = slot % n_tiles, tm = slot % tiles / n_tiles;
+  const int tiles = n_tiles * m_tiles;
+  int units = E, unit, len;
   int64_t row0;
-  int len;
+  RowTiles pieces(offsets, SPLIT ? E : 0, M, SPLIT ? piece : 1);
+  if constexpr (SPLIT) units = pieces.total;
+  const int place = xcd_place(blockIdx.x, units * tiles);
+  if (place < 0) return;
+  unit = place / tiles;
+  const int tn = place % n_tiles, tm = place % tiles / n_tiles;
   if constexpr (SPLIT) {
-    const RowTile t = find_row_tile(offsets, E, M, piece, unit, units);
-    if (t.expert < 0) return;  // (nobody reads the units left over)
+    const RowTile t = pieces.find(unit);
     row0 = t.row0;
     len = t.rows;
   } else {
@@ -468,11 +482,11 @@ template <typename T, int B, int WM, int WN, bool W_RC>
 int launch_linear_direct(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
                          hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t row_tiles = (M + B - 1) / B + E, blocks = patched_blocks(row_tiles, (N + B - 1) / B);
+  const int64_t row_tiles = (M + B - 1) / B + E, blocks = xcd_blocks(row_tiles * ((N + B - 1) / B) + 1);
   PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
   allow_lds(linear_direct_kernel<T, B, B, WM, WN, W_RC>, lds);
   linear_direct_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N,
-                                                                                         K, (int)row_tiles, (T*)y);
+                                                                                         K, (T*)y);
   PS_CHECK_LAUNCH();
 }
 
@@ -492,7 +506,7 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
       const int64_t row_tiles = (M + BM - 1) / BM + E, blocks = row_tiles * ((N + BN - 1) / BN);
       PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
       linear_kernel<T, BM, BN, 2, 2, VB, W_RC><<<(unsigned)blocks, 256, 0, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N, K,
-                                                                              (int)row_tiles, (T*)y);
+                                                                              (T*)y);
       PS_CHECK_LAUNCH();
     });
   });
@@ -530,11 +544,11 @@ template <typename T, int B, int WM, int WN, bool SPLIT>
 int launch_dw_tile(const DwPlan& p, const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* offsets, int64_t M, int E, int N, int K,
                    void* dw, void* db, hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t blocks = (p.units + kXcds - 1) / kXcds * kXcds * ((N + B - 1) / B) * ((K + B - 1) / B);
+  const int64_t blocks = xcd_blocks(p.units * ((N + B - 1) / B) * ((K + B - 1) / B));
   PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
   allow_lds(linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT>, lds);
   linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy, ldy, (const T*)x, ldx, offsets, M, E, N, K, p.piece,
-                                                                                             (int)p.units, dw, db);
+                                                                                             dw, db);
   PS_CHECK_LAUNCH();
 }
 

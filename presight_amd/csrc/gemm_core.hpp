@@ -285,23 +285,39 @@ __device__ __forceinline__ f32x4 mma_block(u32x4 a, u32x4 b, f32x4 acc) {  // (b
 }
 
 // ------------------------------------------------------------------------------------------------ which tile where
-// Workgroups go round the eight XCDs, each with an L2 of its own.  A grid of m x n tiles is cut into patches of 4 x 8 tiles that share
-// their operands' rows (fewer than 8 across: 32 in all), and a patch stays on one XCD: what runs there at a time.
-constexpr int kXcds = 8, kPatch = 32, kPatchN = 8;
+// Workgroups go round the eight XCDs, each with an L2 of its own.  The tiles of a grid are put in an order in which neighbours share their
+// operands' rows -- patches of 32 tiles, what runs on an XCD at a time, up to 8 across -- and the XCDs take patch after patch in turn, the
+// last incomplete round in eighths.  (Eighths of the whole order: 343 us where turns take 312, forward, 65536 x 2048 x 1024 bf16, 32 experts.)
+constexpr int kXcds = 8, kPatch = 32, kPatchN = 8, kRound = kXcds * kPatch;
+inline int64_t xcd_blocks(int64_t tiles) { return (tiles + kXcds - 1) / kXcds * kXcds; }
+// the workgroup's place in the order, -1: none
+__device__ __forceinline__ int xcd_place(int block, int tiles) {
+  const int xcd = block % kXcds, slot = block / kXcds, rounds = tiles / kRound;
+  if (slot < rounds * kPatch) return slot / kPatch * kRound + xcd * kPatch + slot % kPatch;
+  const int rest = tiles - rounds * kRound, each = (rest + kXcds - 1) / kXcds, in = slot - rounds * kPatch, at = xcd * each + in;
+  return in < each && at < rest ? rounds * kRound + at : -1;
+}
+// the how manieth of the workgroups without a place it is
+__device__ __forceinline__ int xcd_spare(int block, int blocks, int tiles) {
+  const int rounds = tiles / kRound, rest = tiles - rounds * kRound, each = (rest + kXcds - 1) / kXcds, xcd = block % kXcds;
+  auto taken = [&](int x) {
+    const int left = rest - x * each;
+    return rounds * kPatch + (left < 0 ? 0 : (left < each ? left : each));
+  };
+  int before = 0;
+  for (int x = 0; x < xcd; ++x) before += blocks / kXcds - taken(x);
+  return before + block / kXcds - taken(xcd);
+}
 struct TileAt {
   int m, n;
-  bool valid;
 };
-__host__ __device__ inline int64_t patched_blocks(int64_t m_tiles, int64_t n_tiles) {
-  const int64_t pn = n_tiles < kPatchN ? n_tiles : kPatchN, pm = kPatch / pn;
-  const int64_t patches = ((m_tiles + pm - 1) / pm) * ((n_tiles + pn - 1) / pn);
-  return (patches + kXcds - 1) / kXcds * kXcds * pm * pn;
-}
-__device__ __forceinline__ TileAt patched_tile(int block, int m_tiles, int n_tiles) {
-  const int pn = n_tiles < kPatchN ? n_tiles : kPatchN, pm = kPatch / pn, size = pm * pn, across = (n_tiles + pn - 1) / pn;
-  const int slot = block / kXcds, patch = slot / size * kXcds + block % kXcds, in = slot % size;
-  const int m = patch / across * pm + in / pn, n = patch % across * pn + in % pn;
-  return {m, n, m < m_tiles && n < n_tiles};
+__device__ __forceinline__ TileAt patched_tile(int place, int m_tiles, int n_tiles) {
+  const int pn = n_tiles < kPatchN ? n_tiles : kPatchN, pm = kPatch / pn;
+  const int band = place / (pm * n_tiles), high = m_tiles - band * pm < pm ? m_tiles - band * pm : pm;
+  int in = place - band * pm * n_tiles;
+  const int patch = in / (high * pn), wide = n_tiles - patch * pn < pn ? n_tiles - patch * pn : pn;
+  in -= patch * high * pn;
+  return {band * pm + in / wide, patch * pn + in % wide};
 }
 
 // widest piece (16, 4 or 2 bytes) that divides every byte count and address

@@ -19,7 +19,7 @@ using namespace ps;
 
 constexpr float kPlaneScale = 1024.0f;                       // fp16 planes hold 1024 * value
 constexpr float kProductScale = 1.0f / (1024.0f * 1024.0f);  // of a product of two
-constexpr int kNormParts = 64;                               // partial sums of squares per matrix
+constexpr int kNormParts = 256;                              // partial sums of squares per matrix, at most
 
 template <typename V>  // float or double
 __device__ __forceinline__ void split(V v, _Float16& hi, _Float16& lo) {
@@ -47,15 +47,15 @@ Shape shape_of(int64_t m, int64_t n) {
 
 // Workspace of a batch: pairs of planes (hi, then lo, for all matrices)
 struct Work {
-  _Float16 *x, *xt[2], *gram, *poly;  // [B][s][lp], [B][l][sp] twice, [B][s][sp], [B][s][sp]
-  double* norms;                      // [B][kNormParts]
-  float* ratio;                       // [B] r at the start
-  int64_t x_plane, xt_plane, s_plane, bytes;
+  _Float16 *x[2], *gram, *poly;  // [B][s][lp] twice, [B][s][sp], [B][s][sp]
+  double* norms;                 // [B][parts]
+  float* ratio;                  // [B] r at the start
+  int parts;
+  int64_t x_plane, s_plane, bytes;
 };
 Work work_of(const Shape& h, int64_t B, void* base) {
   Work w;
   w.x_plane = B * h.s * (int64_t)h.lp;
-  w.xt_plane = B * h.l * (int64_t)h.sp;
   w.s_plane = B * h.s * (int64_t)h.sp;
   char* p = (char*)base;
   auto take = [&](int64_t bytes) {
@@ -63,11 +63,12 @@ Work work_of(const Shape& h, int64_t B, void* base) {
     p += (bytes + 255) & ~(int64_t)255;
     return q;
   };
+  const int64_t parts = h.m * h.n / 8192;  // (at least a few thousand elements each)
+  w.parts = (int)(parts < 1 ? 1 : (parts > kNormParts ? kNormParts : parts));
   w.norms = (double*)take(B * kNormParts * 8);
   w.ratio = (float*)take(B * 4);
-  w.x = (_Float16*)take(w.x_plane * 4);
-  w.xt[0] = (_Float16*)take(w.xt_plane * 4);
-  w.xt[1] = (_Float16*)take(w.xt_plane * 4);
+  w.x[0] = (_Float16*)take(w.x_plane * 4);
+  w.x[1] = (_Float16*)take(w.x_plane * 4);
   w.gram = (_Float16*)take(w.s_plane * 4);
   w.poly = (_Float16*)take(w.s_plane * 4);
   w.bytes = p - (char*)base;
@@ -83,33 +84,52 @@ struct Source {
   int nesterov;
 };
 
-template <typename T, bool MOMENTUM, bool UPDATE>
-__device__ __forceinline__ float source_value(const Source& src, int64_t i) {
+template <bool MOMENTUM, bool UPDATE>
+__device__ __forceinline__ float source_step(const Source& src, float g, float& b) {
 #pragma clang fp contract(off)  // the same bits in both passes over the source
-  const float g = to_f32(reinterpret_cast<const T*>(src.g)[i]);
   if constexpr (!MOMENTUM) return g;
-  float b = src.buf[i];
-  if constexpr (UPDATE) {
-    b = src.mu * b + src.nu * g;
-    src.buf[i] = b;
-  }
+  if constexpr (UPDATE) b = src.mu * b + src.nu * g;
   return src.nesterov ? src.mu * b + src.nu * g : b;
 }
+template <typename T, bool MOMENTUM, bool UPDATE>
+__device__ __forceinline__ float source_value(const Source& src, int64_t i) {
+  float b = 0.0f;
+  if constexpr (MOMENTUM) b = src.buf[i];
+  const float v = source_step<MOMENTUM, UPDATE>(src, to_f32(reinterpret_cast<const T*>(src.g)[i]), b);
+  if constexpr (MOMENTUM && UPDATE) src.buf[i] = b;
+  return v;
+}
+// V consecutive values (V > 1: aligned to their size)
+template <typename T, bool MOMENTUM, bool UPDATE, int V>
+__device__ __forceinline__ void source_pack(const Source& src, int64_t i, float (&v)[V]) {
+  const Pack<T, V> g = load_pack<T, V>(reinterpret_cast<const T*>(src.g) + i);
+  Pack<float, V> b{};
+  if constexpr (MOMENTUM) b = load_pack<float, V>(src.buf + i);
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = source_step<MOMENTUM, UPDATE>(src, to_f32(g.v[k]), b.v[k]);
+  if constexpr (MOMENTUM && UPDATE) store_pack(src.buf + i, b);
+}
 
-// partial sums of squares, in 64 bits: entries of any fp32 size neither overflow nor vanish
-template <typename T, bool MOMENTUM>
-__global__ __launch_bounds__(256) void ns_norm_kernel(Source src, int64_t size, double* __restrict__ norms) {
+// partial sums of squares, in 64 bits: entries of any fp32 size neither overflow nor vanish.  V elements at a time (V = 4: every matrix
+// starts and ends on a pack).
+template <typename T, bool MOMENTUM, int V>
+__global__ __launch_bounds__(256) void ns_norm_kernel(Source src, int64_t size, Work w) {
   __shared__ double part[4];
   const int64_t base = (int64_t)blockIdx.y * size;
-  double sum = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += kNormParts * 256) {
-    const double v = source_value<T, MOMENTUM, true>(src, base + i);
-    sum += v * v;
+  double sum[V] = {};
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < size; i += (int64_t)gridDim.x * 256 * V) {
+    float v[V];
+    source_pack<T, MOMENTUM, true, V>(src, base + i, v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) sum[k] += (double)v[k] * v[k];
   }
-  for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+  double all = 0.0;
+#pragma unroll
+  for (int k = 0; k < V; ++k) all += sum[k];
+  for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = all;
   __syncthreads();
-  if (threadIdx.x == 0) norms[(int64_t)blockIdx.y * kNormParts + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+  if (threadIdx.x == 0) w.norms[(int64_t)blockIdx.y * w.parts + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
 // r before step i
@@ -124,47 +144,43 @@ __device__ __forceinline__ float ratio_at(float r, int i, float grow) {
   return r;
 }
 
-// X^ = G / norm as planes, both ways round, 32 x 32 elements at a time; zeros in the padding of either
-template <typename T, bool MOMENTUM>
+// X^ = G / norm as planes [s][lp], 64 x 64 elements at a time (turned in LDS where G is tall); zeros in the padding.  V as above, of the
+// rows as given.
+template <typename T, bool MOMENTUM, int V>
 __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work w, float eps) {
-  __shared__ double tile[32][33];
-  __shared__ double inv;
+  __shared__ _Float16 tile[2][64][72];  // (rows of 144 bytes: 16-byte chunks, 36 banks apart)
+  __shared__ double inv_of;
   const int64_t b = blockIdx.z;
-  if (threadIdx.x == 0) {
+  if (threadIdx.x < 64) {
     double sum = 0.0;
-    for (int i = 0; i < kNormParts; ++i) sum += w.norms[b * kNormParts + i];
-    const double norm = sqrt(sum);
-    inv = norm == 0.0 ? 0.0 : 1.0 / norm;
-    if (blockIdx.x == 0 && blockIdx.y == 0) w.ratio[b] = norm == 0.0 ? 0.0f : (float)(norm / (norm + (double)eps));
+    for (int i = threadIdx.x; i < w.parts; i += 64) sum += w.norms[b * w.parts + i];
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
+    if (threadIdx.x == 0) {
+      const double norm = sqrt(sum);
+      inv_of = norm == 0.0 ? 0.0 : 1.0 / norm;
+      if (blockIdx.x == 0 && blockIdx.y == 0) w.ratio[b] = norm == 0.0 ? 0.0f : (float)(norm / (norm + (double)eps));
+    }
   }
   __syncthreads();
-  const int rows = h.tall ? h.l : h.s, cols = h.tall ? h.s : h.l;  // as given: [m, n]
-  const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32, tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+  const double inv = inv_of;
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of G
   const int64_t base = b * h.m * h.n;
-  for (int k = ty; k < 32; k += 8) {
-    const int r = r0 + k, c = c0 + tx;
-    tile[k][tx] = r < rows && c < cols ? source_value<T, MOMENTUM, false>(src, base + (int64_t)r * h.n + c) * inv : 0.0;
+  for (int id = threadIdx.x; id < 64 * 64 / V; id += 256) {
+    const int r = id / (64 / V), c = id % (64 / V) * V;
+    float v[V] = {};
+    if (r0 + r < h.m && c0 + c < h.n) source_pack<T, MOMENTUM, false, V>(src, base + (int64_t)(r0 + r) * h.n + c0 + c, v);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int row = h.tall ? c + k : r, col = h.tall ? r : c + k;
+      split(v[k] * inv, tile[0][row][col], tile[1][row][col]);
+    }
   }
   __syncthreads();
-  // plane rows along the given rows, and along the given columns
-  _Float16* same = h.tall ? w.xt[0] : w.x;
-  _Float16* turned = h.tall ? w.x : w.xt[0];
-  const int64_t same_plane = h.tall ? w.xt_plane : w.x_plane, turned_plane = h.tall ? w.x_plane : w.xt_plane;
-  const int same_ld = h.tall ? h.sp : h.lp, turned_ld = h.tall ? h.lp : h.sp;
-  for (int k = ty; k < 32; k += 8) {
-    _Float16 hi, lo;
-    if (r0 + k < rows && c0 + tx < same_ld) {
-      split(tile[k][tx], hi, lo);
-      const int64_t at = (b * rows + r0 + k) * same_ld + c0 + tx;
-      same[at] = hi;
-      same[same_plane + at] = lo;
-    }
-    if (c0 + k < cols && r0 + tx < turned_ld) {
-      split(tile[tx][k], hi, lo);
-      const int64_t at = (b * cols + c0 + k) * turned_ld + r0 + tx;
-      turned[at] = hi;
-      turned[turned_plane + at] = lo;
-    }
+  const int m0 = h.tall ? c0 : r0, n0 = h.tall ? r0 : c0;  // of X
+  for (int id = threadIdx.x; id < 2 * 64 * 8; id += 256) {
+    const int p = id >> 9, row = (id >> 3) & 63, col = (id & 7) * 8;
+    if (m0 + row < h.s && n0 + col < h.lp)
+      *reinterpret_cast<u32x4*>(w.x[0] + p * w.x_plane + (b * h.s + m0 + row) * h.lp + n0 + col) = *reinterpret_cast<const u32x4*>(&tile[p][row][col]);
   }
 }
 
@@ -172,7 +188,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work
 enum Product {
   kGram,   // S = X X^T                            rows of X     x rows of X,    k = l
   kPoly,   // P = a I + b S + c S S                rows of S     x rows of S,    k = s    (S is symmetric)
-  kApply,  // X' = P X, both ways round            rows of P     x rows of X^T,  k = s
+  kApply,  // X' = P X                             rows of P     x columns of X, k = s
   kLast    // ... of the last step: into the result
 };
 
@@ -188,17 +204,18 @@ struct Poly {
 };
 
 struct Operands {
-  const _Float16 *a, *b;      // [B][ra][k], [B][rb][k]; the lo plane is a_plane / b_plane behind
+  const _Float16 *a, *b;  // [B][ra][k]; [B][rb][k], or for kApply and kLast [B][k_rows][ldb]; the lo planes are a_plane / b_plane behind
   int64_t a_plane, b_plane;
-  int ra, rb, k;              // k: padded, and the rows' distance
+  int ra, rb, k;  // k: padded, and the rows' distance
+  int k_rows, ldb;
 };
 
 // A workgroup's tile: 128 x 128, eight waves of 64 x 32.  Two tiles of 64 k of all four planes (hi and lo of either operand, 64 KiB) in
 // LDS: the loads of the next tile run beside this one's 384 matrix instructions, three on every pair of fragments.  The two small
 // products add up apart from the large one: each of their additions to it would cost it another rounding.
 //
-// The result leaves through LDS both as it is and turned, as rows of 256 bytes: X needs both ways round, and of a symmetric result only
-// the tiles on and below the diagonal are computed and their turned copies are the others.
+// The result leaves through LDS as rows of 256 bytes; of a symmetric one only the tiles on and below the diagonal are computed, and leave
+// turned as well.
 constexpr int kPairTile = 128, kPairThreads = 512, kPairPlane = kPairTile * kTileRowBytes;  // bytes of one plane's tile
 constexpr int kPairLds = 2 * 4 * kPairPlane;
 
@@ -211,31 +228,38 @@ __device__ __forceinline__ int out_addr(int row, int col) {
 }
 
 template <typename T, Product WHAT>
-__global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Shape h, Work w, int step, Poly c, Result res) {
+__global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Shape h, Work w, int batches, int step, Poly c, Result res) {
   constexpr int B = kPairTile, NT = kPairThreads, MI = 4, NJ = 2;
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
-  using Tile = DirectTile<_Float16, B, NT, false>;
+  using TileA = DirectTile<_Float16, B, NT, false>;
+  using TileB = DirectTile<_Float16, B, NT, !kSymmetric>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int m_tiles = (o.ra + B - 1) / B, n_tiles = (o.rb + B - 1) / B;
-  const int64_t batch = blockIdx.y;
+  // (the batch's matrices one under the other; of a symmetric result the tiles tm >= tn, row by row)
+  const int tiles = kSymmetric ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles, place = xcd_place(blockIdx.x, tiles * batches);
+  if (place < 0) return;
   int tm, tn;
-  if constexpr (kSymmetric) {  // blockIdx.x counts the tiles tm >= tn row by row
-    tm = (int)((sqrtf(8.0f * blockIdx.x + 1.0f) - 1.0f) * 0.5f);
-    while (tm * (tm + 1) / 2 > (int)blockIdx.x) --tm;
-    while ((tm + 1) * (tm + 2) / 2 <= (int)blockIdx.x) ++tm;
+  int64_t batch;
+  if constexpr (kSymmetric) {
+    batch = place / tiles;
+    const int in = place % tiles;
+    tm = (int)((sqrtf(8.0f * in + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > in) --tm;
+    while ((tm + 1) * (tm + 2) / 2 <= in) ++tm;
     tm = uniform(tm);
-    tn = blockIdx.x - tm * (tm + 1) / 2;
+    tn = in - tm * (tm + 1) / 2;
   } else {
-    const TileAt at = patched_tile(blockIdx.x, m_tiles, n_tiles);
-    if (!at.valid) return;
-    tm = at.m, tn = at.n;
+    const TileAt at = patched_tile(place, batches * m_tiles, n_tiles);
+    batch = at.m / m_tiles;
+    tm = at.m % m_tiles, tn = at.n;
   }
   const int m0 = tm * B, n0 = tn * B;
   const int rows = o.ra - m0 < B ? o.ra - m0 : B, cols = o.rb - n0 < B ? o.rb - n0 : B;
   const _Float16* pa = o.a + (batch * o.ra + m0) * o.k;
-  const _Float16* pb = o.b + (batch * o.rb + n0) * o.k;
-  const DirectSource<_Float16, B, NT, false> ah(pa, o.k, rows, o.k), al(pa + o.a_plane, o.k, rows, o.k), bh(pb, o.k, cols, o.k),
-      bl(pb + o.b_plane, o.k, cols, o.k);
+  const _Float16* pb = kSymmetric ? o.b + (batch * o.rb + n0) * o.k : o.b + batch * o.k_rows * o.ldb + n0;
+  const int ldb = kSymmetric ? o.k : o.ldb, in_b = kSymmetric ? cols : (h.lp - n0 < B ? h.lp - n0 : B), kb = kSymmetric ? o.k : o.k_rows;
+  const DirectSource<_Float16, B, NT, false> ah(pa, o.k, rows, o.k), al(pa + o.a_plane, o.k, rows, o.k);
+  const DirectSource<_Float16, B, NT, !kSymmetric> bh(pb, ldb, in_b, kb), bl(pb + o.b_plane, ldb, in_b, kb);
   auto load = [&](int k0, char* to) {
     ah.load(k0, to);
     al.load(k0, to + kPairPlane);
@@ -259,9 +283,9 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[p][j] = Tile::fragment(t + (2 + p) * kPairPlane, wn + j * 16, s);
+        for (int j = 0; j < NJ; ++j) fb[p][j] = TileB::fragment(t + (2 + p) * kPairPlane, wn + j * 16, s);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[p][i] = Tile::fragment(t + p * kPairPlane, wm + i * 16, s);
+        for (int i = 0; i < MI; ++i) fa[p][i] = TileA::fragment(t + p * kPairPlane, wm + i * 16, s);
       }
 #pragma unroll
       for (int i = 0; i < MI; ++i)
@@ -275,9 +299,11 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
     __syncthreads();
   }
   const float ratio = ratio_at(w.ratio[batch], step, c.grow);
-  // kPoly: a + b r^2 S^ + c r^4 S^ S^, formed in 64 bits: an error of a coefficient would be common to all entries and grow like a
-  // singular value's, and it is the small product of a step | kApply: over the step's growth of r | kLast: X = r X^
+  // kPoly: a + b r^2 S^ + c r^4 S^ S^ with the coefficients as pairs of floats: an error of a coefficient would be common to all entries and
+  // grow like a singular value's | kApply: over the step's growth of r | kLast: X = r X^
   const double r2 = (double)ratio * ratio, cb = c.b * r2 / kPlaneScale, cc = c.c * r2 * r2 * kProductScale;
+  const float cb_hi = (float)cb, cb_lo = (float)(cb - cb_hi), cc_hi = (float)cc, cc_lo = (float)(cc - cc_hi);
+  const float ca_hi = (float)c.a, ca_lo = (float)(c.a - ca_hi);
   const float out_scale = WHAT == kApply ? kProductScale * (ratio > 0.0f ? ratio / ratio_at(ratio, 1, c.grow) : 1.0f)
                                          : (WHAT == kLast ? kProductScale * ratio : kProductScale);
   const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
@@ -308,13 +334,17 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
         for (int q = 0; q < 4; ++q) {
           const float sum = acc[i][j][q] + fine[i][j][q];
           if constexpr (WHAT == kPoly) {
-            const double one = m0 + m == n0 + n + q && m < rows ? c.a : 0.0;  // (rows and columns of the padding stay zero)
-            split(cc * sum + (cb * ((double)(float)gh.v[q] + (double)(float)gl.v[q]) + one), hi.v[q], lo.v[q]);
+            const bool one = m0 + m == n0 + n + q && m < rows;  // (rows and columns of the padding stay zero)
+            const float was = (float)gh.v[q] + (float)gl.v[q];
+            const float small = fmaf(cc_lo, sum, fmaf(cb_lo, was, one ? ca_lo : 0.0f));
+            split(fmaf(cb_hi, was, one ? ca_hi : 0.0f) + fmaf(cc_hi, sum, small), hi.v[q], lo.v[q]);
           } else {
             split(sum * out_scale, hi.v[q], lo.v[q]);
           }
-          *reinterpret_cast<_Float16*>(lds + 2 * kOut + out_addr<_Float16>(n + q, m)) = hi.v[q];
-          *reinterpret_cast<_Float16*>(lds + 3 * kOut + out_addr<_Float16>(n + q, m)) = lo.v[q];
+          if constexpr (kSymmetric) {
+            *reinterpret_cast<_Float16*>(lds + 2 * kOut + out_addr<_Float16>(n + q, m)) = hi.v[q];
+            *reinterpret_cast<_Float16*>(lds + 3 * kOut + out_addr<_Float16>(n + q, m)) = lo.v[q];
+          }
         }
         store_pack(reinterpret_cast<_Float16*>(lds + out_addr<_Float16>(m, n)), hi);
         store_pack(reinterpret_cast<_Float16*>(lds + kOut + out_addr<_Float16>(m, n)), lo);
@@ -325,31 +355,49 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
   if constexpr (WHAT == kLast) {
     const int r0 = h.tall ? n0 : m0, c0 = h.tall ? m0 : n0, rn = h.tall ? cols : rows, cn = h.tall ? rows : cols;
     const int64_t base = batch * h.m * h.n + (int64_t)r0 * h.n + c0;
-    for (int id = threadIdx.x; id < B * B; id += NT) {
-      const int row = id / B, col = id % B;
+    // four at a time where rows and addresses allow it
+    const bool packed = h.n % 4 == 0 && ((uintptr_t)res.out & (4 * sizeof(T) - 1)) == 0;
+    for (int id = threadIdx.x; id < B * (B / 4); id += NT) {
+      const int row = id / (B / 4), col = id % (B / 4) * 4;
       if (row >= rn || col >= cn) continue;
-      const float v = *reinterpret_cast<const float*>(lds + out_addr<float>(row, col));
+      const f32x4 v = *reinterpret_cast<const f32x4*>(lds + out_addr<float>(row, col));
       const int64_t at = base + (int64_t)row * h.n + col;
       if (res.update) {
         float* p = reinterpret_cast<float*>(res.out) + at;
-        *p = res.keep * *p - res.rate * v;
+        if (packed) {
+          f32x4 old = *reinterpret_cast<f32x4*>(p);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) old[q] = res.keep * old[q] - res.rate * v[q];
+          *reinterpret_cast<f32x4*>(p) = old;
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (col + q < cn) p[q] = res.keep * p[q] - res.rate * v[q];
+        }
       } else {
-        reinterpret_cast<T*>(res.out)[at] = from_f32<T>(v);
+        T* p = reinterpret_cast<T*>(res.out) + at;
+        if (packed) {
+          Pack<T, 4> out;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) out.v[q] = from_f32<T>(v[q]);
+          store_pack(p, out);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (col + q < cn) p[q] = from_f32<T>(v[q]);
+        }
       }
     }
   } else {
-    _Float16* same = (WHAT == kGram ? w.gram : (WHAT == kPoly ? w.poly : w.x)) + batch * h.s * (kSymmetric ? h.sp : h.lp);
-    _Float16* turned = kSymmetric ? same : w.xt[(step + 1) & 1] + batch * h.l * h.sp;
-    const int64_t same_plane = kSymmetric ? w.s_plane : w.x_plane, turned_plane = kSymmetric ? w.s_plane : w.xt_plane;
-    const int same_ld = kSymmetric ? h.sp : h.lp, turned_ld = h.sp;
-    for (int id = threadIdx.x; id < 4 * B * (B / 8); id += NT) {
+    const int ld = kSymmetric ? h.sp : h.lp;
+    const int64_t plane = kSymmetric ? w.s_plane : w.x_plane;
+    _Float16* out = (WHAT == kGram ? w.gram : (WHAT == kPoly ? w.poly : w.x[(step + 1) & 1])) + batch * h.s * ld;
+    const int parts = kSymmetric && tm != tn ? 4 : 2;
+    for (int id = threadIdx.x; id < parts * B * (B / 8); id += NT) {
       const int part = id / (B * (B / 8)), row = id / (B / 8) % B, col = id % (B / 8) * 8;
       const u32x4 v = *reinterpret_cast<const u32x4*>(lds + part * kOut + out_addr<_Float16>(row, col));
-      if (part < 2) {
-        if (row < rows && n0 + col < same_ld) *reinterpret_cast<u32x4*>(same + (part & 1) * same_plane + (int64_t)(m0 + row) * same_ld + n0 + col) = v;
-      } else if (!kSymmetric || tm != tn) {
-        if (row < cols && m0 + col < turned_ld) *reinterpret_cast<u32x4*>(turned + (part & 1) * turned_plane + (int64_t)(n0 + row) * turned_ld + m0 + col) = v;
-      }
+      const int rn = part < 2 ? rows : cols, r0 = part < 2 ? m0 : n0, c0 = part < 2 ? n0 : m0;
+      if (row < rn && c0 + col < ld) *reinterpret_cast<u32x4*>(out + (part & 1) * plane + (int64_t)(r0 + row) * ld + c0 + col) = v;
     }
   }
 }
@@ -357,9 +405,9 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
 template <typename T, Product WHAT>
 void launch_product(const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res, hipStream_t s) {
   const int64_t m = (o.ra + kPairTile - 1) / kPairTile, n = (o.rb + kPairTile - 1) / kPairTile;
-  const int64_t blocks = WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : patched_blocks(m, n);
+  const int64_t blocks = xcd_blocks((WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : m * n) * B);
   hipFuncSetAttribute((const void*)ns_product_kernel<T, WHAT>, hipFuncAttributeMaxDynamicSharedMemorySize, kPairLds);
-  ns_product_kernel<T, WHAT><<<dim3((unsigned)blocks, (unsigned)B), kPairThreads, kPairLds, s>>>(o, h, w, step, c, res);
+  ns_product_kernel<T, WHAT><<<(unsigned)blocks, kPairThreads, kPairLds, s>>>(o, h, w, (int)B, step, c, res);
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -530,14 +578,20 @@ int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Pol
   }
   const Shape h = shape_of(m, n);
   const Work w = work_of(h, B, workspace);
-  ns_norm_kernel<T, MOMENTUM><<<dim3(kNormParts, (unsigned)B), 256, 0, s>>>(src, m * n, w.norms);
-  // (the columns cover both paddings: rows and columns as given, rounded up to the planes' tiles)
-  const int rows = h.tall ? h.lp : h.sp, cols = h.tall ? h.sp : h.lp;
-  ns_start_kernel<T, MOMENTUM><<<dim3((unsigned)(cols / 32), (unsigned)(rows / 32), (unsigned)B), 256, 0, s>>>(src, h, w, eps);
+  const dim3 norm_grid((unsigned)w.parts, (unsigned)B);
+  const dim3 start_grid((unsigned)((h.tall ? h.sp : h.lp) / 64), (unsigned)((h.tall ? h.lp : h.sp) / 64), (unsigned)B);
+  if (n % 4 == 0 && ((uintptr_t)src.g & (4 * sizeof(T) - 1)) == 0 && ((uintptr_t)src.buf & 15) == 0) {
+    ns_norm_kernel<T, MOMENTUM, 4><<<norm_grid, 256, 0, s>>>(src, m * n, w);
+    ns_start_kernel<T, MOMENTUM, 4><<<start_grid, 256, 0, s>>>(src, h, w, eps);
+  } else {
+    ns_norm_kernel<T, MOMENTUM, 1><<<norm_grid, 256, 0, s>>>(src, m * n, w);
+    ns_start_kernel<T, MOMENTUM, 1><<<start_grid, 256, 0, s>>>(src, h, w, eps);
+  }
   for (int i = 0; i < steps; ++i) {
-    launch_product<T, kGram>({w.x, w.x, w.x_plane, w.x_plane, h.s, h.s, h.lp}, h, w, B, i, c, res, s);
-    launch_product<T, kPoly>({w.gram, w.gram, w.s_plane, w.s_plane, h.s, h.s, h.sp}, h, w, B, i, c, res, s);
-    const Operands apply{w.poly, w.xt[i & 1], w.s_plane, w.xt_plane, h.s, h.l, h.sp};
+    const _Float16* x = w.x[i & 1];
+    launch_product<T, kGram>({x, x, w.x_plane, w.x_plane, h.s, h.s, h.lp, 0, 0}, h, w, B, i, c, res, s);
+    launch_product<T, kPoly>({w.gram, w.gram, w.s_plane, w.s_plane, h.s, h.s, h.sp, 0, 0}, h, w, B, i, c, res, s);
+    const Operands apply{w.poly, x, w.s_plane, w.x_plane, h.s, h.l, h.sp, h.s, h.lp};
     if (i + 1 < steps)
       launch_product<T, kApply>(apply, h, w, B, i, c, res, s);
     else
@@ -549,7 +603,8 @@ int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Pol
 constexpr int64_t kMaxSide = 1 << 20;
 
 bool sizes_ok(int64_t B, int64_t m, int64_t n, int steps) {
-  return B >= 0 && B <= 65535 && m >= 0 && n >= 0 && m <= kMaxSide && n <= kMaxSide && steps >= 1 && steps <= 64 && (m < n ? m : n) <= 16384;
+  return B >= 0 && B <= 65535 && m >= 0 && n >= 0 && m <= kMaxSide && n <= kMaxSide && steps >= 1 && steps <= 64 && (m < n ? m : n) <= 16384 &&
+         ((m + 127) / 128) * ((n + 127) / 128) * B < ((int64_t)1 << 30);
 }
 
 }  // namespace
