@@ -635,8 +635,9 @@ int ps_finish_losses(const float* const* terms, const int64_t* n, const float* d
  *   ps_expert_linear_fwd    y [M,out] = W_e x + b_e for expert e's rows, zeros for the rows of nobody; weight [E,out,in], bias [E,out] or
  *                           NULL.  Offsets are bounded to [0, M]: no row outside is touched
  *   ps_expert_linear_dx     dx [M,in] = W_e^T dy
- *   ps_expert_linear_dw     dweight [E,out,in] = sum over expert e's rows of dy x^T, dbias [E,out] = sum dy (may be NULL); workspace:
- *                           ps_expert_linear_dw_workspace bytes (NULL if 0) */
+ *   ps_expert_linear_dw     dweight [E,out,in] = sum over expert e's rows of dy x^T, dbias [E,out] = sum dy (may be NULL)
+ *   ps_expert_linear_workspace   bytes of workspace of a call with these operands; pass 0: forward (a = x, b = weight), 1: dx (a = dy,
+ *                           b = weight), 2: dw (a = dy, b = x); the call takes NULL where it is 0 */
 int64_t ps_expert_plan_workspace(int64_t M, int E);
 int ps_expert_plan(const void* ids, int ids_are_64, int64_t M, int E, int32_t* offsets, int32_t* src, int32_t* dst,
                    int32_t* workspace /*nullable*/, void* stream);
@@ -647,11 +648,12 @@ int ps_expert_combine(const void* rows, int64_t rows_stride, const float* weight
 int ps_expert_combine_bwd(const void* dy, int64_t dy_stride, const void* rows, int64_t rows_stride, const float* weights,
                           const int32_t* dst, const int32_t* held, int64_t N, int k, int64_t D, int dtype, void* drows /*nullable*/,
                           float* dw /*nullable*/, void* stream);
+int64_t ps_expert_linear_workspace(int pass, const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t M, int E,
+                                   int64_t n_in, int64_t n_out, int dtype);
 int ps_expert_linear_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias /*nullable*/, const int32_t* offsets,
-                         int64_t M, int E, int64_t n_in, int64_t n_out, int dtype, void* y, void* stream);
+                         int64_t M, int E, int64_t n_in, int64_t n_out, int dtype, void* y, void* workspace /*nullable*/, void* stream);
 int ps_expert_linear_dx(const void* dy, int64_t dy_stride, const void* weight, const int32_t* offsets, int64_t M, int E, int64_t n_in,
-                        int64_t n_out, int dtype, void* dx, void* stream);
-int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out);
+                        int64_t n_out, int dtype, void* dx, void* workspace /*nullable*/, void* stream);
 int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const int32_t* offsets, int64_t M, int E,
                         int64_t n_in, int64_t n_out, int dtype, void* dweight, void* dbias /*nullable*/, void* workspace /*nullable*/,
                         void* stream);

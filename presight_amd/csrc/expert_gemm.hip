@@ -74,161 +74,10 @@ __device__ __forceinline__ void clear_outside(const int* __restrict__ offsets, i
   for (int64_t i = (int64_t)me * blockDim.x + threadIdx.x; i < count; i += step) y[i < first ? i : tail0 * N + (i - first)] = from_f32<T>(0.0f);
 }
 
-// A workgroup's tile into memory: four consecutive n per lane and block
-template <typename T, int MI, int NJ>
-__device__ __forceinline__ void store_tile(f32x4 (&acc)[MI][NJ], T* __restrict__ y, int64_t ldy, int rows, int cols, int m0, int n0, const T* __restrict__ bias) {
-  const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-  const bool packed = ((ldy * sizeof(T)) % (4 * sizeof(T))) == 0 && ((uintptr_t)y % (4 * sizeof(T))) == 0;
-#pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const int n = n0 + j * 16 + g * 4;
-    float b[4] = {0.f, 0.f, 0.f, 0.f};
-    if (bias != nullptr) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (n + q < cols) b[q] = to_f32(bias[n + q]);
-    }
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + i * 16 + r;
-      if (m >= rows) continue;
-      T* o = y + m * ldy + n;
-      if (packed && n + 3 < cols) {
-        Pack<T, 4> p;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) p.v[q] = from_f32<T>(acc[i][j][q] + b[q]);
-        store_pack(o, p);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (n + q < cols) o[q] = from_f32<T>(acc[i][j][q] + b[q]);
-      }
-    }
-  }
-}
-
-// y[p] = sum_k x[p][k] W(n,k) (+ bias): W_RC = false: weight rows are k-contiguous (forward), true: n-contiguous (input gradient)
-template <typename T, int BM, int BN, int WM, int WN, int VB, bool W_RC>
-__global__ __launch_bounds__(64 * WM * WN) void linear_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, const T* __restrict__ bias,
-                                                              const int* __restrict__ offsets, int64_t M, int E, int N, int K, T* __restrict__ y) {
-  constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16, BK = kTileK<T>;
-  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * kTileRowBytes];
-  const int n_tiles = (N + BN - 1) / BN;
-  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles;
-  RowTiles tiles(offsets, E, M, BM);
-  if (tm >= tiles.total) {
-    clear_outside<T>(offsets, E, M, blockIdx.x - tiles.total * n_tiles, gridDim.x - tiles.total * n_tiles, y, N);
-    return;
-  }
-  const RowTile t = tiles.find(tm);
-  const int n0 = tn * BN, cols = N - n0 < BN ? N - n0 : BN;
-  const T* xa = x + t.row0 * ldx;
-  const T* wb = weight + (int64_t)t.expert * N * K + (W_RC ? (int64_t)n0 : (int64_t)n0 * K);
-  const unsigned lda = (unsigned)(ldx * sizeof(T)), ldb = (unsigned)((W_RC ? N : K) * sizeof(T));
-  TileLoader<T, BM, NT, VB, false> la;
-  TileLoader<T, BN, NT, VB, W_RC> lb;
-  auto load = [&](int k0) {
-    la.load(window(xa + k0, ((int64_t)(t.rows - 1) * ldx + (K - k0)) * sizeof(T)), lda, K - k0);
-    if constexpr (W_RC) {
-      const int kr = K - k0 < BK ? K - k0 : BK;
-      lb.load(window(wb + (int64_t)k0 * N, ((int64_t)(kr - 1) * N + (N - n0)) * sizeof(T)), ldb, N - n0);
-    } else {
-      lb.load(window(wb + k0, ((int64_t)(cols - 1) * K + (K - k0)) * sizeof(T)), ldb, K - k0);
-    }
-  };
-  f32x4 acc[MI][NJ];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-  load(0);
-  la.store(lds[0]);
-  lb.store(lds[0] + BM * kTileRowBytes);
-  __syncthreads();
-  for (int k0 = 0, cur = 0; k0 < K; k0 += BK, cur ^= 1) {
-    const bool more = k0 + BK < K;
-    if (more) load(k0 + BK);
-    tile_mma<T, MI, NJ>(lds[cur], lds[cur] + BM * kTileRowBytes, wm, wn, acc);
-    if (more) {
-      la.store(lds[cur ^ 1]);
-      lb.store(lds[cur ^ 1] + BM * kTileRowBytes);
-    }
-    __syncthreads();
-  }
-  store_tile<T, MI, NJ>(acc, y + t.row0 * N + n0, N, t.rows, cols, wm, wn, bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
-}
-
-// One piece of an expert's rows against a (out) x (in) tile.  split == false: the piece is all of the expert's rows and the tile is
-// written in T; true: tile `unit` of at most `piece` rows, written as fp32 partial sums [unit][out][in] that dw_join_kernel adds up.
-template <typename T, int BM, int BN, int WM, int WN, int VB>
-__global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
-                                                                 const int* __restrict__ offsets, int64_t M, int E, int N, int K, T* __restrict__ dw,
-                                                                 T* __restrict__ db) {
-  constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16, BK = kTileK<T>;
-  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * kTileRowBytes];
-  const int n_tiles = (K + BN - 1) / BN, m_tiles = (N + BM - 1) / BM;
-  const int tn = blockIdx.x % n_tiles, tm = blockIdx.x / n_tiles % m_tiles, e = blockIdx.x / (n_tiles * m_tiles);
-  const int64_t lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
-  const int64_t row0 = lo;
-  const int len = uniform(hi > lo ? (int)(hi - lo) : 0);
-  const int m0 = tm * BM, n0 = tn * BN;
-  TileLoader<T, BM, NT, VB, true> la;
-  TileLoader<T, BN, NT, VB, true> lb;
-  auto load = [&](int k0) {
-    const int kr = len - k0 < BK ? len - k0 : BK;
-    la.load(window(dy + (row0 + k0) * ldy + m0, ((int64_t)(kr - 1) * ldy + (N - m0)) * sizeof(T)), (unsigned)(ldy * sizeof(T)), N - m0);
-    lb.load(window(x + (row0 + k0) * ldx + n0, ((int64_t)(kr - 1) * ldx + (K - n0)) * sizeof(T)), (unsigned)(ldx * sizeof(T)), K - n0);
-  };
-  const bool sums = db != nullptr && tn == 0;
-  float s[decltype(la)::N][kChunk<T>] = {};
-  f32x4 acc[MI][NJ];
-#pragma unroll
-  for (int i = 0; i < MI; ++i)
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int wave = threadIdx.x >> 6, wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
-  if (len > 0) {
-    load(0);
-    if (sums) la.add_rows(s);
-    la.store(lds[0]);
-    lb.store(lds[0] + BM * kTileRowBytes);
-  }
-  __syncthreads();
-  for (int k0 = 0, cur = 0; k0 < len; k0 += BK, cur ^= 1) {
-    const bool more = k0 + BK < len;
-    if (more) load(k0 + BK);
-    tile_mma<T, MI, NJ>(lds[cur], lds[cur] + BM * kTileRowBytes, wm, wn, acc);
-    if (more) {
-      if (sums) la.add_rows(s);
-      la.store(lds[cur ^ 1]);
-      lb.store(lds[cur ^ 1] + BM * kTileRowBytes);
-    }
-    __syncthreads();
-  }
-  store_tile<T, MI, NJ>(acc, dw + (int64_t)e * N * K + (int64_t)m0 * K + n0, K, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn, nullptr);
-  if (sums) {  // the threads of one column of blocks add up in order of k
-    float* part = reinterpret_cast<float*>(&lds[0][0]);
-    constexpr int kAcross = BM / kChunk<T>, kDeep = kTileK<T> / 4;
-#pragma unroll
-    for (int b = 0; b < decltype(la)::N; ++b) {
-      const int id = b * NT + threadIdx.x;
-      if (id < 2 * BM)
-#pragma unroll
-        for (int i = 0; i < kChunk<T>; ++i) part[(id / kAcross) * BM + (id % kAcross) * kChunk<T> + i] = s[b][i];
-    }
-    __syncthreads();
-    for (int m = threadIdx.x; m < BM && m0 + m < N; m += NT) {
-      float v = 0.0f;
-      for (int k = 0; k < kDeep; ++k) v += part[k * BM + m];
-      db[(int64_t)e * N + m0 + m] = from_f32<T>(v);
-    }
-  }
-}
-
-// ------------------------------------------------------------------------------------------------ aligned operands
-// The same two kernels for operands whose pieces are whole 16-byte chunks: tiles go straight into LDS, two stages, the loads of the next
-// tile in flight while the matrix instructions run over this one.
+// Two stages of 128 bytes of k in LDS: the loads of the next tile are in flight while the matrix instructions run over this one.  What a
+// compute unit can have in flight from the L2 bounds them (about 18 bytes a cycle): a 256 x 256 tile of 16-bit operands asks for 32 at the
+// full matrix rate, a 128 x 128 one for 64.  (8192 x 8192 x 8192 bf16: 859 us, 1281 TFLOP/s; four stages of half the depth, half a tile of
+// fragments read ahead, and several tiles per workgroup with the next one's loads under this one's store were no faster.)
 // SUMS: also the sums of A's rows over k, as a product with ones (`sums`: whether this wave wants them).
 template <typename T, int BM, int BN, int WM, int WN, bool A_RC, bool B_RC, bool SUMS>
 __device__ __forceinline__ void direct_loop(char* lds, int K, const DirectSource<T, BM, 64 * WM * WN, A_RC>& sa,
@@ -292,6 +141,7 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
   constexpr int kSpread = kAcross < 8 ? kAcross - 1 : 7;
   static_assert(kPass >= 1 && MI % kPass == 0, "whole blocks of rows per pass");
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const bool whole = ((uint64_t)ldy * sizeof(T) & 15) == 0 && ((uintptr_t)y & 15) == 0;  // (else element by element)
   float b[NJ][4] = {};
   if (bias != nullptr) {
 #pragma unroll
@@ -317,6 +167,15 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (!whole) {
+      for (int id = lane; id < kPass * 16 * NJ * 16; id += 64) {
+        const int row = id / (NJ * 16), col = id % (NJ * 16), byte = col * (int)sizeof(T), m = m0 + p * kPass * 16 + row;
+        const T v = *reinterpret_cast<const T*>(slice + row * kRow + (((byte >> 4) ^ (row & kSpread)) << 4) + (byte & 15));
+        if (m < rows && n0 + col < cols) y[m * ldy + n0 + col] = v;
+      }
+      __builtin_amdgcn_wave_barrier();
+      continue;
+    }
 #pragma unroll
     for (int t = 0; t < kPass * 16 * kAcross / 64; ++t) {
       const int id = t * 64 + lane, row = id / kAcross, c = id % kAcross, m = m0 + p * kPass * 16 + row, n = n0 + c * kChunk<T>;
@@ -327,10 +186,12 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
   }
 }
 
+// y[p] = sum_k x[p][k] W(n,k) (+ bias).  W_RC = false: the weight's rows are k-contiguous (forward), n of them; true: n-contiguous (input
+// gradient), `w_rows` of them.  K: the rows' length in whole chunks.
 template <typename T, int BM, int BN, int WM, int WN, bool W_RC>
-__global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight,
-                                                                     const T* __restrict__ bias, const int* __restrict__ offsets, int64_t M, int E,
-                                                                     int N, int K, T* __restrict__ y) {
+__global__ __launch_bounds__(64 * WM * WN) void linear_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, int64_t ldw, int w_rows,
+                                                              const T* __restrict__ bias, const int* __restrict__ offsets, int64_t M, int E, int N, int K,
+                                                              T* __restrict__ y) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   RowTiles tiles(offsets, E, M, BM);
@@ -342,9 +203,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __
   const TileAt at = patched_tile(place, tiles.total, n_tiles);
   const RowTile t = tiles.find(at.m);
   const int n0 = at.n * BN, cols = N - n0 < BN ? N - n0 : BN;
-  const T* wb = weight + (int64_t)t.expert * N * K + (W_RC ? (int64_t)n0 : (int64_t)n0 * K);
+  const T* wb = weight + (int64_t)t.expert * w_rows * ldw + (W_RC ? (int64_t)n0 : n0 * ldw);
   const DirectSource<T, BM, NT, false> sa(x + t.row0 * ldx, ldx, t.rows, K);
-  const DirectSource<T, BN, NT, W_RC> sb(wb, W_RC ? N : K, W_RC ? N - n0 : cols, K);
+  const DirectSource<T, BN, NT, W_RC> sb(wb, ldw, W_RC ? (N + kChunk<T> - 1) / kChunk<T> * kChunk<T> - n0 : cols, W_RC ? w_rows : K);
   f32x4 acc[MI][NJ], none[1];
   direct_loop<T, BM, BN, WM, WN, false, W_RC, false>(lds, K, sa, sb, acc, none, false);
   const int wave = uniform(threadIdx.x >> 6), wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
@@ -358,9 +219,9 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_direct_kernel(const T* __
 // dw_join_kernel adds up the pieces of each expert in order.  Also shorter sums: a piece rounds `piece` / 4 times where the whole
 // column would round a hundred times as often.
 template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN) void linear_dw_direct_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
-                                                                        const int* __restrict__ offsets, int64_t M, int E, int N, int K, int piece,
-                                                                        void* __restrict__ dw, void* __restrict__ db) {
+__global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
+                                                                        const int* __restrict__ offsets, int64_t M, int E, int N, int K, int ldo, int piece,
+                                                                 void* __restrict__ dw, void* __restrict__ db) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
   using Out = std::conditional_t<SPLIT, float, T>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -385,30 +246,33 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_dw_direct_kernel(const T*
     len = uniform(hi > lo ? (int)(hi - lo) : 0);
   }
   const int m0 = tm * BM, n0 = tn * BN;
-  const DirectSource<T, BM, NT, true> sa(dy + row0 * ldy + m0, ldy, N - m0, len);
-  const DirectSource<T, BN, NT, true> sb(x + row0 * ldx + n0, ldx, K - n0, len);
+  constexpr int kC = kChunk<T>;  // (rows hold whole chunks)
+  const DirectSource<T, BM, NT, true> sa(dy + row0 * ldy + m0, ldy, (N + kC - 1) / kC * kC - m0, len);
+  const DirectSource<T, BN, NT, true> sb(x + row0 * ldx + n0, ldx, (K + kC - 1) / kC * kC - n0, len);
   const int wave = uniform(threadIdx.x >> 6), wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   const bool sums = db != nullptr && tn == 0 && wn == 0;
   f32x4 acc[MI][NJ], row_sums[MI];
   direct_loop<T, BM, BN, WM, WN, true, true, true>(lds, len, sa, sb, acc, row_sums, sums);
-  Out* o = reinterpret_cast<Out*>(dw) + (int64_t)unit * N * K + (int64_t)m0 * K + n0;
+  Out* o = reinterpret_cast<Out*>(dw) + ((int64_t)unit * N + m0) * ldo + n0;
   constexpr int kSlice = 2 * (BM + BN) * kTileRowBytes / (WM * WN);
-  store_tile_rows<Out, MI, NJ, kSlice>(acc, lds + wave * kSlice, o, K, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn,
+  store_tile_rows<Out, MI, NJ, kSlice>(acc, lds + wave * kSlice, o, ldo, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn,
                                        static_cast<const Out*>(nullptr));
   if (sums && (threadIdx.x & 63) < 16) {
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
       const int m = m0 + wm + i * 16 + (threadIdx.x & 15);
-      if (m < N) reinterpret_cast<Out*>(db)[(int64_t)unit * N + m] = from_f32<Out>(row_sums[i][0]);
+      if (m < N) reinterpret_cast<Out*>(db)[(int64_t)unit * (SPLIT ? (N + 3) / 4 * 4 : N) + m] = from_f32<Out>(row_sums[i][0]);
     }
   }
 }
 
-// dW_e, db_e = the sums of expert e's pieces, in order
+// dW_e, db_e = the sums of expert e's pieces: parts [unit][out][ldo] (ldo: in, rounded up to four) and db_parts [unit][out rounded up].
+// Four lanes share the pieces of four neighbouring sums, each takes every fourth in order, and the four meet in LDS in order.
 template <typename T>
 __global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ parts, const float* __restrict__ db_parts, const int* __restrict__ offsets,
-                                                      int64_t M, int64_t size, int N, int piece, T* __restrict__ dw, T* __restrict__ db) {
+                                                      int64_t M, int N, int K, int ldo, int piece, T* __restrict__ dw, T* __restrict__ db) {
   __shared__ int wave_sum[4];
+  __shared__ f32x4 quarter[4][64];
   const int e = blockIdx.y;
   int before = 0;
   for (int i = threadIdx.x; i < e; i += 256) {
@@ -416,26 +280,53 @@ __global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ 
     if (hi > lo) before += (int)((hi - lo + piece - 1) / piece);
   }
   for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d, 64);
-  if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = before;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  if (lane == 0) wave_sum[wave] = before;
   __syncthreads();
   const int64_t first = (int64_t)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
   const int64_t lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
   const int n = hi > lo ? (int)((hi - lo + piece - 1) / piece) : 0;
-  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i < size) {  // (size is a multiple of four: the direct kernels' rule)
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int u = 0; u < n; ++u) v += *reinterpret_cast<const f32x4*>(parts + (first + u) * size + i);
-    Pack<T, 4> o;
+  const int64_t size = (int64_t)N * ldo, db_size = (N + 3) / 4 * 4, i = ((int64_t)blockIdx.x * 64 + lane) * 4;
+  const bool bias = i >= size;  // (the weights' sums first, then the bias's)
+  const float* p = bias ? db_parts + first * db_size + (i - size) : parts + first * size + i;
+  const int64_t step = bias ? db_size : size;
+  const bool on = i < size || (db != nullptr && i < size + db_size);
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (on) {
+    f32x4 w[4] = {};
+    int u = wave;
+    for (; u + 12 < n; u += 16)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) o.v[q] = from_f32<T>(v[q]);
-    store_pack(dw + (int64_t)e * size + i, o);
+      for (int q = 0; q < 4; ++q) w[q] += *reinterpret_cast<const f32x4*>(p + (u + 4 * q) * step);
+    for (; u < n; u += 4) w[0] += *reinterpret_cast<const f32x4*>(p + u * step);
+    v = (w[0] + w[1]) + (w[2] + w[3]);
   }
-  if (db != nullptr)
-    for (int m = blockIdx.x * 256 + threadIdx.x; m < N; m += gridDim.x * 256) {
-      float v = 0.0f;
-      for (int u = 0; u < n; ++u) v += db_parts[(first + u) * N + m];
-      db[(int64_t)e * N + m] = from_f32<T>(v);
+  quarter[wave][lane] = v;
+  __syncthreads();
+  if (wave != 0 || !on) return;
+  v = (quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if (bias) {
+      if (i - size + q < N) db[(int64_t)e * N + (i - size) + q] = from_f32<T>(v[q]);
+    } else {
+      const int64_t m = (i + q) / ldo, c = (i + q) % ldo;
+      if (c < K) dw[((int64_t)e * N + m) * K + c] = from_f32<T>(v[q]);
     }
+  }
+}
+
+// rows of `cols` elements `ld` apart -> rows of whole 16-byte chunks, zeros behind the last element
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, T* __restrict__ dst) {
+  const int across = (cols + kChunk<T> - 1) / kChunk<T>;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / across;
+  const int c = (int)(id % across) * kChunk<T>;
+  if (row >= rows) return;
+  Pack<T, kChunk<T>> o;
+#pragma unroll
+  for (int q = 0; q < kChunk<T>; ++q) o.v[q] = c + q < cols ? src[row * ld + c + q] : from_f32<T>(0.0f);
+  store_pack(dst + id * kChunk<T>, o);
 }
 
 template <typename F>
@@ -447,15 +338,6 @@ int by_type(int dtype, F&& f) {
   return -1;
 }
 
-template <typename T, typename F>
-int by_piece(int vb, F&& f) {
-  if (vb == 16) return f(std::integral_constant<int, 16>{});
-  if constexpr (sizeof(T) == 2) {
-    if (vb == 2) return f(std::integral_constant<int, 2>{});
-  }
-  return f(std::integral_constant<int, 4>{});
-}
-
 constexpr int64_t kMaxWidth = 1 << 20;
 
 bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
@@ -464,9 +346,8 @@ bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
 
 constexpr int kCompute = 256;  // compute units
 
-// Tile sizes of the direct kernels, by work per tile.  256 x 256 reads each operand byte half as often as 128 x 128 and is twice as far
-// from the LDS's read rate, but one tile fills a compute unit: it is taken where it wastes little of itself and there is a tile for
-// every compute unit.  Narrow outputs and few rows per expert take the smaller ones.
+// Tile sizes, by work per tile.  256 x 256 reads each operand byte half as often as 128 x 128, but one tile fills a compute unit: it is taken
+// where it wastes little of itself and there is a tile for every compute unit.  Narrow outputs and few rows per expert take the smaller ones.
 int linear_tile(int64_t rows, int64_t groups, int64_t cols) {
   const int64_t each = rows / groups;
   if (cols > 128 && each >= 192 && (rows / 256 + groups) * ((cols + 255) / 256) >= kCompute) return 256;
@@ -478,37 +359,62 @@ void allow_lds(K* kernel, int bytes) {
   if (bytes > 64 * 1024) hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
+// An operand as the products read it: rows of whole 16-byte chunks that start on 16 bytes
+struct Rows {
+  const void* p;
+  int64_t ld;
+};
+int size_of(int dtype) { return dtype == kF32 ? 4 : 2; }
+int64_t padded(int64_t cols, int dtype) {
+  const int chunk = 16 / size_of(dtype);
+  return (cols + chunk - 1) / chunk * chunk;
+}
+bool is_packed(const void* p, int64_t ld, int64_t cols, int dtype) {
+  const int size = size_of(dtype);
+  return ((uintptr_t)p & 15) == 0 && ((ld * size) & 15) == 0 && ((cols * size) & 15) == 0;
+}
+int64_t pack_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
+  return is_packed(p, ld, cols, dtype) ? 0 : (rows * padded(cols, dtype) * size_of(dtype) + 255) & ~(int64_t)255;
+}
+// the operand itself, or its copy at *to, which moves on
+template <typename T>
+Rows packed(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype, char** to, hipStream_t s) {
+  const int64_t bytes = pack_bytes(p, ld, rows, cols, dtype);
+  if (bytes == 0) return {p, ld};
+  T* copy = (T*)*to;
+  *to += bytes;
+  const int64_t chunks = rows * (padded(cols, dtype) / kChunk<T>);
+  if (chunks > 0) pack_rows_kernel<T><<<(unsigned)((chunks + 255) / 256), 256, 0, s>>>((const T*)p, ld, rows, (int)cols, copy);
+  return {copy, padded(cols, dtype)};
+}
+
 template <typename T, int B, int WM, int WN, bool W_RC>
-int launch_linear_direct(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
-                         hipStream_t s) {
+int launch_linear_tile(const Rows& x, const Rows& w, int w_rows, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
+                       hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
   const int64_t row_tiles = (M + B - 1) / B + E, blocks = xcd_blocks(row_tiles * ((N + B - 1) / B) + 1);
-  PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
-  allow_lds(linear_direct_kernel<T, B, B, WM, WN, W_RC>, lds);
-  linear_direct_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N,
-                                                                                         K, (T*)y);
+  PS_REQUIRE(blocks < ((int64_t)1 << 30), "ps_expert_linear: too many tiles");
+  allow_lds(linear_kernel<T, B, B, WM, WN, W_RC>, lds);
+  linear_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x.p, x.ld, (const T*)w.p, w.ld, w_rows, (const T*)bias, offsets,
+                                                                                  M, E, N, K, (T*)y);
   PS_CHECK_LAUNCH();
 }
 
+// x [M,K] (dy) times the weights [E,out,in]: W_RC = false: K = in, N = out; true: K = out, N = in
 template <bool W_RC>
-int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, int dtype,
-                  void* y, hipStream_t s) {
+int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E, int64_t n_in, int64_t n_out,
+                  int dtype, void* y, void* workspace, hipStream_t s) {
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vb = piece_bytes(sizeof(T), {ldx, N, K}, {x, weight, y});
-    if (vb == 16) switch (linear_tile(M, E, N)) {
-        case 256: return launch_linear_direct<T, 256, 2, 4, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
-        case 128: return launch_linear_direct<T, 128, 2, 2, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
-        default: return launch_linear_direct<T, 64, 2, 2, W_RC>(x, ldx, weight, bias, offsets, M, E, N, K, y, s);
-      }
-    return by_piece<T>(vb, [&](auto piece) {
-      constexpr int VB = decltype(piece)::value, BM = 128, BN = 128;
-      const int64_t row_tiles = (M + BM - 1) / BM + E, blocks = row_tiles * ((N + BN - 1) / BN);
-      PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear: too many tiles");
-      linear_kernel<T, BM, BN, 2, 2, VB, W_RC><<<(unsigned)blocks, 256, 0, s>>>((const T*)x, ldx, (const T*)weight, (const T*)bias, offsets, M, E, N, K,
-                                                                              (T*)y);
-      PS_CHECK_LAUNCH();
-    });
+    char* to = (char*)workspace;
+    const int64_t k = W_RC ? n_out : n_in;
+    const Rows xs = packed<T>(x, ldx, M, k, dtype, &to, s), ws = packed<T>(weight, n_in, E * n_out, n_in, dtype, &to, s);
+    const int N = (int)(W_RC ? n_in : n_out), K = (int)padded(k, dtype), rows = (int)n_out;
+    switch (linear_tile(M, E, N)) {
+      case 256: return launch_linear_tile<T, 256, 2, 4, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
+      case 128: return launch_linear_tile<T, 128, 2, 2, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
+      default: return launch_linear_tile<T, 64, 2, 2, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
+    }
   });
 }
 
@@ -535,51 +441,66 @@ DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out) {
   return p;
 }
 
-int64_t dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out) {
+int64_t round4(int64_t v) { return (v + 3) / 4 * 4; }
+int64_t dw_part_bytes(int64_t M, int E, int64_t n_in, int64_t n_out) {
   const DwPlan p = dw_plan(M, E, n_in, n_out);
-  return p.piece == 0 ? 0 : p.units * (n_in * n_out + n_out) * (int64_t)sizeof(float);
+  return p.piece == 0 ? 0 : (p.units * (n_out * round4(n_in) + round4(n_out)) * (int64_t)sizeof(float) + 255) & ~(int64_t)255;
 }
 
 template <typename T, int B, int WM, int WN, bool SPLIT>
-int launch_dw_tile(const DwPlan& p, const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* offsets, int64_t M, int E, int N, int K,
-                   void* dw, void* db, hipStream_t s) {
+int launch_dw_tile(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t* offsets, int64_t M, int E, int N, int K, int ldo, void* dw, void* db,
+                   hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
   const int64_t blocks = xcd_blocks(p.units * ((N + B - 1) / B) * ((K + B - 1) / B));
-  PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
-  allow_lds(linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT>, lds);
-  linear_dw_direct_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy, ldy, (const T*)x, ldx, offsets, M, E, N, K, p.piece,
-                                                                                             dw, db);
+  PS_REQUIRE(blocks < ((int64_t)1 << 30), "ps_expert_linear_dw: too many tiles");
+  allow_lds(linear_dw_kernel<T, B, B, WM, WN, SPLIT>, lds);
+  linear_dw_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy.p, dy.ld, (const T*)x.p, x.ld, offsets, M, E, N, K, ldo,
+                                                                                      p.piece, dw, db);
   PS_CHECK_LAUNCH();
 }
 
 template <typename T, bool SPLIT>
-int launch_dw_direct(const DwPlan& p, const void* dy, int64_t ldy, const void* x, int64_t ldx, const int32_t* offsets, int64_t M, int E, int N, int K,
-                     void* dw, void* db, hipStream_t s) {
-  if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, SPLIT>(p, dy, ldy, x, ldx, offsets, M, E, N, K, dw, db, s);
-  if (p.tile == 128) return launch_dw_tile<T, 128, 2, 2, SPLIT>(p, dy, ldy, x, ldx, offsets, M, E, N, K, dw, db, s);
-  return launch_dw_tile<T, 64, 2, 2, SPLIT>(p, dy, ldy, x, ldx, offsets, M, E, N, K, dw, db, s);
+int launch_dw(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t* offsets, int64_t M, int E, int N, int K, int ldo, void* dw, void* db,
+              hipStream_t s) {
+  if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
+  if (p.tile == 128) return launch_dw_tile<T, 128, 2, 2, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
+  return launch_dw_tile<T, 64, 2, 2, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
+}
+
+enum Pass { kForward, kInputGradient, kWeightGradient };
+
+int64_t workspace_of(int pass, const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
+  if (pass == kWeightGradient)
+    return dw_part_bytes(M, E, n_in, n_out) + pack_bytes(a, a_stride, M, n_out, dtype) + pack_bytes(b, b_stride, M, n_in, dtype);
+  return pack_bytes(a, a_stride, M, pass == kForward ? n_in : n_out, dtype) + pack_bytes(b, n_in, E * n_out, n_in, dtype);
 }
 
 }  // namespace
 
+extern "C" int64_t ps_expert_linear_workspace(int pass, const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t M, int E, int64_t n_in,
+                                              int64_t n_out, int dtype) {
+  if (!sizes_ok(M, E, n_in, n_out) || pass < kForward || pass > kWeightGradient || dtype < kF32 || dtype > kBF16) return 0;
+  return workspace_of(pass, a, a_stride, b, b_stride, M, E, n_in, n_out, dtype);
+}
+
 extern "C" int ps_expert_linear_fwd(const void* x, int64_t x_stride, const void* weight, const void* bias, const int32_t* offsets, int64_t M, int E,
-                                    int64_t n_in, int64_t n_out, int dtype, void* y, void* stream) {
+                                    int64_t n_in, int64_t n_out, int dtype, void* y, void* workspace, void* stream) {
   PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && x_stride >= n_in && x_stride <= kMaxWidth, "ps_expert_linear_fwd: sizes out of range");
   if (M == 0) return 0;
   PS_REQUIRE(x != nullptr && weight != nullptr && offsets != nullptr && y != nullptr, "ps_expert_linear_fwd: null argument");
-  return launch_linear<false>(x, x_stride, weight, bias, offsets, M, E, (int)n_out, (int)n_in, dtype, y, (hipStream_t)stream);
+  PS_REQUIRE(workspace != nullptr || workspace_of(kForward, x, x_stride, weight, n_in, M, E, n_in, n_out, dtype) == 0,
+             "ps_expert_linear_fwd: needs its workspace (ps_expert_linear_workspace)");
+  return launch_linear<false>(x, x_stride, weight, bias, offsets, M, E, n_in, n_out, dtype, y, workspace, (hipStream_t)stream);
 }
 
 extern "C" int ps_expert_linear_dx(const void* dy, int64_t dy_stride, const void* weight, const int32_t* offsets, int64_t M, int E, int64_t n_in,
-                                   int64_t n_out, int dtype, void* dx, void* stream) {
+                                   int64_t n_out, int dtype, void* dx, void* workspace, void* stream) {
   PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && dy_stride >= n_out && dy_stride <= kMaxWidth, "ps_expert_linear_dx: sizes out of range");
   if (M == 0) return 0;
   PS_REQUIRE(dy != nullptr && weight != nullptr && offsets != nullptr && dx != nullptr, "ps_expert_linear_dx: null argument");
-  return launch_linear<true>(dy, dy_stride, weight, nullptr, offsets, M, E, (int)n_in, (int)n_out, dtype, dx, (hipStream_t)stream);
-}
-
-extern "C" int64_t ps_expert_linear_dw_workspace(int64_t M, int E, int64_t n_in, int64_t n_out) {
-  return sizes_ok(M, E, n_in, n_out) ? dw_workspace(M, E, n_in, n_out) : 0;
+  PS_REQUIRE(workspace != nullptr || workspace_of(kInputGradient, dy, dy_stride, weight, n_in, M, E, n_in, n_out, dtype) == 0,
+             "ps_expert_linear_dx: needs its workspace (ps_expert_linear_workspace)");
+  return launch_linear<true>(dy, dy_stride, weight, nullptr, offsets, M, E, n_in, n_out, dtype, dx, workspace, (hipStream_t)stream);
 }
 
 extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const int32_t* offsets, int64_t M, int E,
@@ -587,30 +508,23 @@ extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void
   PS_REQUIRE(sizes_ok(M, E, n_in, n_out) && x_stride >= n_in && x_stride <= kMaxWidth && dy_stride >= n_out && dy_stride <= kMaxWidth,
              "ps_expert_linear_dw: sizes out of range");
   PS_REQUIRE((M == 0 || (dy != nullptr && x != nullptr)) && offsets != nullptr && dweight != nullptr, "ps_expert_linear_dw: null argument");
+  PS_REQUIRE(workspace != nullptr || workspace_of(kWeightGradient, dy, dy_stride, x, x_stride, M, E, n_in, n_out, dtype) == 0,
+             "ps_expert_linear_dw: needs its workspace (ps_expert_linear_workspace)");
   const DwPlan p = dw_plan(M, E, n_in, n_out);
-  PS_REQUIRE(p.piece == 0 || workspace != nullptr, "ps_expert_linear_dw: needs its workspace (ps_expert_linear_dw_workspace)");
-  const int N = (int)n_out, K = (int)n_in;
+  const int N = (int)n_out, K = (int)n_in, ldo = (int)round4(n_in);
   hipStream_t s = (hipStream_t)stream;
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vb = piece_bytes(sizeof(T), {dy_stride, x_stride, n_in, n_out}, {dy, x, dweight, workspace});
-    if (vb == 16) {
-      if (p.piece == 0) return launch_dw_direct<T, false>(p, dy, dy_stride, x, x_stride, offsets, M, E, N, K, dweight, dbias, s);
-      float* parts = (float*)workspace;
-      float* db_parts = parts + p.units * n_in * n_out;
-      const int rc = launch_dw_direct<T, true>(p, dy, dy_stride, x, x_stride, offsets, M, E, N, K, parts, dbias != nullptr ? db_parts : nullptr, s);
-      if (rc != 0) return rc;
-      dw_join_kernel<T><<<dim3((unsigned)((n_in * n_out / 4 + 255) / 256), (unsigned)E), 256, 0, s>>>(parts, db_parts, offsets, M, n_in * n_out, N, p.piece,
-                                                                                                     (T*)dweight, (T*)dbias);
-      PS_CHECK_LAUNCH();
-    }
-    return by_piece<T>(vb, [&](auto piece) {
-      constexpr int VB = decltype(piece)::value, BM = 128, BN = 128;
-      const int64_t blocks = (int64_t)E * ((n_out + BM - 1) / BM) * ((n_in + BN - 1) / BN);
-      PS_REQUIRE(blocks < ((int64_t)1 << 31), "ps_expert_linear_dw: too many tiles");
-      linear_dw_kernel<T, BM, BN, 2, 2, VB><<<(unsigned)blocks, 256, 0, s>>>((const T*)dy, dy_stride, (const T*)x, x_stride, offsets, M, E, N, K,
-                                                                            (T*)dweight, (T*)dbias);
-      PS_CHECK_LAUNCH();
-    });
+    float* parts = (float*)workspace;
+    char* to = (char*)workspace + dw_part_bytes(M, E, n_in, n_out);
+    const Rows dys = packed<T>(dy, dy_stride, M, n_out, dtype, &to, s), xs = packed<T>(x, x_stride, M, n_in, dtype, &to, s);
+    if (p.piece == 0) return launch_dw<T, false>(p, dys, xs, offsets, M, E, N, K, K, dweight, dbias, s);
+    float* db_parts = parts + p.units * n_out * ldo;
+    const int rc = launch_dw<T, true>(p, dys, xs, offsets, M, E, N, K, ldo, parts, dbias != nullptr ? db_parts : nullptr, s);
+    if (rc != 0) return rc;
+    const int64_t sums = n_out * ldo + (dbias != nullptr ? round4(n_out) : 0);
+    dw_join_kernel<T><<<dim3((unsigned)((sums + 255) / 256), (unsigned)E), 256, 0, s>>>(parts, db_parts, offsets, M, N, K, ldo, p.piece, (T*)dweight,
+                                                                                       (T*)dbias);
+    PS_CHECK_LAUNCH();
   });
 }

@@ -1,13 +1,9 @@
-// Tile products on the matrix cores for operands of any length and layout: C[m][n] = sum_k A(m,k) B(n,k) over one workgroup's tile.
+// Tile products on the matrix cores: C[m][n] = sum_k A(m,k) B(n,k) over one workgroup's tile.
 //
-// An operand is either k-contiguous ("KC": element (r,k) at base + r*ld + k) or row-contiguous ("RC": at base + k*ld + r).  Both arrive in
-// LDS in ONE form, rows of 128 bytes that hold 128 / sizeof(T) consecutive k in eight 16-byte chunks: the RC loader transposes 4 k x 16
-// byte blocks in registers on the way (fp32: a renaming; 16-bit: one v_perm per two elements), so one inner loop serves the forward
-// product and both gradients.
-//
-// Edges.  Global reads go through buffer descriptors that start at the tile's corner and end at the operand's last valid element; what
-// lies behind reads as zero.  Within a row, pieces at or behind the contiguous extent get an offset outside the descriptor.  A piece
-// is VB bytes: the caller picks the widest that divides every extent, stride and address, so a piece is never split by an edge.
+// An operand is either k-contiguous ("KC": element (r,k) at base + r*ld + k) or row-contiguous ("RC": at base + k*ld + r), with rows that
+// start on 16 bytes and hold whole 16-byte chunks.  Global reads go through buffer descriptors that start at the tile's corner and end at
+// the operand's last element; what lies behind reads as zero, and so do chunks at or behind the contiguous extent, which get an
+// offset outside the descriptor.
 #pragma once
 #include "expert_types.hpp"
 
@@ -35,148 +31,11 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void* base, int64
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(lo | (hi << 32)), 0, uniform(n), 0x00027000);
 }
 
-// Byte address of a chunk in a tile.  16 lanes read one chunk column of 16 rows at a time, and the 64 banks hold two rows: the two rows
-// of a pair sit in the two halves of the banks by themselves, (row >> 1) spreads the eight pairs over the eight chunk slots.  The RC
-// loader writes rows 8 (16-bit) or 4 (fp32) apart side by side: (row >> 4) spreads those.
-__device__ __forceinline__ int tile_addr(int row, int chunk) { return row * kTileRowBytes + (((chunk ^ (row >> 1) ^ (row >> 4)) & 7) << 4); }
-
-// 16 bytes at byte `off`, of which `left` elements exist
-template <typename T, int VB>
-__device__ __forceinline__ u32x4 load_chunk(__amdgpu_buffer_rsrc_t w, unsigned off, int left) {
-  u32x4 v;
-  if constexpr (VB == 16) {
-    v = __builtin_amdgcn_raw_buffer_load_b128(w, left > 0 ? off : kOutside, 0, 0);
-  } else if constexpr (VB == 4) {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) v[p] = __builtin_amdgcn_raw_buffer_load_b32(w, left > p * 4 / (int)sizeof(T) ? off + p * 4 : kOutside, 0, 0);
-  } else {
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const unsigned lo = __builtin_amdgcn_raw_buffer_load_b16(w, left > 2 * p ? off + p * 4 : kOutside, 0, 0);
-      const unsigned hi = __builtin_amdgcn_raw_buffer_load_b16(w, left > 2 * p + 1 ? off + p * 4 + 2 : kOutside, 0, 0);
-      v[p] = (lo & 0xffffu) | (hi << 16);
-    }
-  }
-  return v;
-}
-
-// A tile of BR rows x kTileK<T>, loaded by NT threads into registers and from there into LDS.
-template <typename T, int BR, int NT, int VB, bool RC>
-struct TileLoader;
-
-template <typename T, int BR, int NT, int VB>
-struct TileLoader<T, BR, NT, VB, false> {
-  static_assert(BR * 8 % NT == 0, "every thread loads the same number of chunks");
-  static constexpr int N = BR * 8 / NT;
-  u32x4 v[N];
-  // w starts at (row 0 of the tile, first k); k_left: valid k from there; the descriptor ends the rows
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t w, unsigned ld_bytes, int k_left) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int id = i * NT + threadIdx.x, row = id >> 3, c = id & 7;
-      v[i] = load_chunk<T, VB>(w, row * ld_bytes + c * 16, k_left - c * kChunk<T>);
-    }
-  }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int id = i * NT + threadIdx.x;
-      *reinterpret_cast<u32x4*>(lds + tile_addr(id >> 3, id & 7)) = v[i];
-    }
-  }
-};
-
-template <typename T, int BR, int NT, int VB>
-struct TileLoader<T, BR, NT, VB, true> {
-  static constexpr int kBlocks = 2 * BR;  // (kTileK / 4) x (BR / kChunk) blocks of 4 k x one chunk of rows
-  static constexpr int N = (kBlocks + NT - 1) / NT;
-  static constexpr int kAcross = BR / kChunk<T>;
-  u32x4 v[N][4];
-  // w starts at (first k, row 0 of the tile); r_left: rows of the operand from there; the descriptor ends the k
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t w, unsigned ld_bytes, int r_left) {
-#pragma unroll
-    for (int b = 0; b < N; ++b) {
-      const int id = b * NT + threadIdx.x, r = id % kAcross, k = id / kAcross;
-      const int left = kBlocks % NT == 0 || id < kBlocks ? r_left - r * kChunk<T> : 0;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[b][q] = load_chunk<T, VB>(w, (k * 4 + q) * ld_bytes + r * 16, left);
-    }
-  }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int b = 0; b < N; ++b) {
-      const int id = b * NT + threadIdx.x, r = id % kAcross, k = id / kAcross;
-      if (kBlocks % NT != 0 && id >= kBlocks) continue;
-      if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<u32x4*>(lds + tile_addr(r * 4 + i, k)) = u32x4{v[b][0][i], v[b][1][i], v[b][2][i], v[b][3][i]};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const unsigned pick = (i & 1) ? 0x07060302u : 0x05040100u;
-          u32x2 o;
-          o[0] = __builtin_amdgcn_perm(v[b][1][i >> 1], v[b][0][i >> 1], pick);
-          o[1] = __builtin_amdgcn_perm(v[b][3][i >> 1], v[b][2][i >> 1], pick);
-          *reinterpret_cast<u32x2*>(lds + tile_addr(r * 8 + i, k >> 1) + (k & 1) * 8) = o;
-        }
-      }
-    }
-  }
-  // per-row sums over the k of this tile (bias gradients): s[i] += rows r*kChunk + i of this thread's blocks
-  __device__ __forceinline__ void add_rows(float (&s)[N][kChunk<T>]) const {
-#pragma unroll
-    for (int b = 0; b < N; ++b)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-#pragma unroll
-        for (int i = 0; i < kChunk<T>; ++i) {
-          if constexpr (sizeof(T) == 4) {
-            s[b][i] += __builtin_bit_cast(f32x4, v[b][q])[i];
-          } else {
-            const unsigned short h = (unsigned short)(v[b][q][i >> 1] >> ((i & 1) * 16));
-            s[b][i] += to_f32(__builtin_bit_cast(T, h));
-          }
-        }
-  }
-};
-
-// One wave's part of a tile: MI x NJ blocks of 16 x 16.  B's rows are the matrix instruction's rows, so a lane ends up with four
-// consecutive n of one m: acc[i][j][r] = C[16 i + (lane & 15)][16 j + 4 (lane >> 4) + r].  fp32: the k inside a chunk are taken in the
-// same order for both operands, so four 16x16x4 steps consume the four floats of a chunk.
-template <typename T, int MI, int NJ>
-__device__ __forceinline__ void tile_mma(const char* a_lds, const char* b_lds, int m0, int n0, f32x4 (&acc)[MI][NJ]) {
-  const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    u32x4 a[MI], b[NJ];
-#pragma unroll
-    for (int i = 0; i < MI; ++i) a[i] = *reinterpret_cast<const u32x4*>(a_lds + tile_addr(m0 + i * 16 + r, s * 4 + g));
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) b[j] = *reinterpret_cast<const u32x4*>(b_lds + tile_addr(n0 + j * 16 + r, s * 4 + g));
-#pragma unroll
-    for (int i = 0; i < MI; ++i)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        if constexpr (sizeof(T) == 4) {
-          const f32x4 bf = __builtin_bit_cast(f32x4, b[j]), af = __builtin_bit_cast(f32x4, a[i]);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(bf[q], af[q], acc[i][j], 0, 0, 0);
-        } else if constexpr (__is_same(T, _Float16)) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b[j]), __builtin_bit_cast(f16x8, a[i]), acc[i][j], 0, 0, 0);
-        } else {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, b[j]), __builtin_bit_cast(bf16x8, a[i]), acc[i][j], 0, 0, 0);
-        }
-      }
-  }
-}
-
 // ------------------------------------------------------------------------------------------------ tiles loaded straight into LDS
-// Operands whose pieces are whole 16-byte chunks need no registers on the way: buffer loads write LDS directly, 1 KiB per wave and
-// instruction in lane order, and zeros where the descriptor ends.  The tile keeps the operand's own direction: KC as above, RC as rows of
-// k (BR elements each), from which 16-bit fragments are read with the transposing LDS loads (16 lanes fetch 4 k x 16 rows, each lane ends
-// up with the 4 k of its row) and fp32 ones element by element.  What would collide in the banks is spread by permuting chunks within a
-// tile row, on the global side of the load.
+// Operands need no registers on the way: buffer loads write LDS directly, 1 KiB per wave and instruction in lane order.  A tile holds 128
+// bytes of k and keeps the operand's own direction: KC as rows of k, RC as rows of BR elements of one k each, from which 16-bit fragments
+// are read with the transposing LDS loads (16 lanes fetch 4 k x 16 rows, each lane ends up with the 4 k of its row) and fp32 ones element by
+// element.  What would collide in the 64 banks is spread by permuting chunks within a tile row, on the global side of the load.
 template <typename T, int BR, int NT, bool RC>
 struct DirectTile {
   static constexpr int kBytes = BR * kTileRowBytes;
@@ -270,8 +129,11 @@ struct DirectSource {
   }
 };
 
+// One 16 x 16 block of a product over one fragment of k.  B's rows are the matrix instruction's rows, so a lane ends up with four
+// consecutive n of one m: acc[r] = C[lane & 15][4 (lane >> 4) + r].  fp32: the k inside a chunk are taken in the same order for both
+// operands, so four 16x16x4 steps consume the four floats of a chunk.
 template <typename T>
-__device__ __forceinline__ f32x4 mma_block(u32x4 a, u32x4 b, f32x4 acc) {  // (b's rows are the instruction's rows, as in tile_mma)
+__device__ __forceinline__ f32x4 mma_block(u32x4 a, u32x4 b, f32x4 acc) {
   if constexpr (sizeof(T) == 4) {
     const f32x4 bf = __builtin_bit_cast(f32x4, b), af = __builtin_bit_cast(f32x4, a);
 #pragma unroll
@@ -318,14 +180,6 @@ __device__ __forceinline__ TileAt patched_tile(int place, int m_tiles, int n_til
   const int patch = in / (high * pn), wide = n_tiles - patch * pn < pn ? n_tiles - patch * pn : pn;
   in -= patch * high * pn;
   return {band * pm + in / wide, patch * pn + in % wide};
-}
-
-// widest piece (16, 4 or 2 bytes) that divides every byte count and address
-inline int piece_bytes(int size, std::initializer_list<int64_t> elems, std::initializer_list<const void*> ptrs) {
-  uint64_t bits = 0;
-  for (int64_t e : elems) bits |= (uint64_t)e * size;
-  for (const void* p : ptrs) bits |= (uint64_t)(uintptr_t)p;
-  return (bits & 15) == 0 ? 16 : ((bits & 3) == 0 ? 4 : 2);
 }
 
 }  // namespace ps

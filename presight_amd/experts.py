@@ -56,6 +56,16 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _once(fn):
+    """differentiable once: torch's guard, where second derivatives are being recorded (it costs as much as a small kernel otherwise)"""
+    guarded = once_differentiable(fn)
+    return lambda ctx, *grads: (guarded if torch.is_grad_enabled() else fn)(ctx, *grads)
+
+
 class ExpertPlan:
     """Who goes where, for ids [N, k] and E experts (int32 tensors on the ids' device):
         offsets [E+1]   expert e's rows are the sorted places offsets[e] .. offsets[e+1]
@@ -102,12 +112,12 @@ def expert_plan(ids: Tensor, num_experts: int) -> ExpertPlan:
 
 
 # ------------------------------------------------------------------------------------------------ exchange
-def _dispatch(x: Tensor, dst: Tensor, held: Tensor) -> Tensor:
+def _dispatch(x: Tensor, dst: Tensor, offsets: Tensor) -> Tensor:
     x = _rows(x)
     (N, k), D = dst.shape, x.shape[1]
     with _on(x.device):
         rows = torch.empty(N * k, D, device=x.device, dtype=x.dtype)
-        check(lib().ps_expert_dispatch(_p(x), x.stride(0), _p(dst), _p(held), N, k, D, DTYPE_CODES[x.dtype], _p(rows), _stream()),
+        check(lib().ps_expert_dispatch(_p(x), x.stride(0), _p(dst), _held(offsets), N, k, D, DTYPE_CODES[x.dtype], _p(rows), _stream()),
               "ps_expert_dispatch")
     return rows
 
@@ -122,14 +132,19 @@ def _combine(rows: Tensor, weights: Optional[Tensor], dst: Tensor) -> Tensor:
     return y
 
 
+def _held(offsets: Tensor) -> int:
+    """address of the number of assignments to an expert"""
+    return offsets.data_ptr() + 4 * (offsets.shape[0] - 1)
+
+
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, dst, held):
+    def forward(ctx, x, dst, offsets):
         ctx.save_for_backward(dst)
-        return _dispatch(x, dst, held)
+        return _dispatch(x, dst, offsets)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, drows):
         (dst,) = ctx.saved_tensors
         return _combine(drows, None, dst), None, None
@@ -137,24 +152,24 @@ class _Dispatch(torch.autograd.Function):
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, weights, dst, held):
+    def forward(ctx, rows, weights, dst, offsets):
         w = None if weights is None else weights.detach().float().contiguous()
-        ctx.save_for_backward(rows, w, dst, held)
+        ctx.save_for_backward(rows, w, dst, offsets)
         ctx.weights_dtype = None if weights is None else weights.dtype
         return _combine(rows, w, dst)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
-        rows, w, dst, held = ctx.saved_tensors
+        rows, w, dst, offsets = ctx.saved_tensors
         if w is None:
-            return _dispatch(dy, dst, held), None, None, None
+            return _dispatch(dy, dst, offsets), None, None, None
         dy, rows = _rows(dy), _rows(rows)
         (N, k), D = dst.shape, rows.shape[1]
         with _on(rows.device):
             drows = torch.empty(rows.shape, device=rows.device, dtype=rows.dtype) if ctx.needs_input_grad[0] else None
             dw = torch.empty(N, k, device=rows.device, dtype=torch.float32) if ctx.needs_input_grad[1] else None
-            check(lib().ps_expert_combine_bwd(_p(dy), dy.stride(0), _p(rows), rows.stride(0), _p(w), _p(dst), _p(held), N, k, D,
+            check(lib().ps_expert_combine_bwd(_p(dy), dy.stride(0), _p(rows), rows.stride(0), _p(w), _p(dst), _held(offsets), N, k, D,
                                               DTYPE_CODES[rows.dtype], _p(drows), _p(dw), _stream()), "ps_expert_combine_bwd")
         return drows, None if dw is None else dw.to(ctx.weights_dtype), None, None
 
@@ -171,7 +186,7 @@ def expert_dispatch(x: Tensor, plan: ExpertPlan) -> Tensor:
     _typed(_gpu(x, "x", plan.dst.device), "x")
     if x.dim() != 2 or x.shape[0] != plan.num_rows:
         raise ValueError(f"presight_amd: x must be [{plan.num_rows}, features] for this plan (got {tuple(x.shape)})")
-    return _Dispatch.apply(x, plan.dst, plan.held)
+    return _Dispatch.apply(x, plan.dst, plan.offsets) if _wants_grad(x) else _dispatch(x, plan.dst, plan.offsets)
 
 
 def expert_combine(rows: Tensor, weights: Optional[Tensor], plan: ExpertPlan) -> Tensor:
@@ -185,7 +200,9 @@ def expert_combine(rows: Tensor, weights: Optional[Tensor], plan: ExpertPlan) ->
         _typed(_gpu(weights, "weights", plan.dst.device), "weights")
         if tuple(weights.shape) != (plan.num_rows, plan.k):
             raise ValueError(f"presight_amd: weights must be {(plan.num_rows, plan.k)} for this plan (got {tuple(weights.shape)})")
-    return _Combine.apply(rows, weights, plan.dst, plan.held)
+    if not _wants_grad(rows, weights):
+        return _combine(rows, None if weights is None else weights.float().contiguous(), plan.dst)
+    return _Combine.apply(rows, weights, plan.dst, plan.offsets)
 
 
 # ------------------------------------------------------------------------------------------------ the experts' linear layers
@@ -199,40 +216,52 @@ def _ld(t: Tensor) -> int:
     return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
 
 
+def _workspace(pass_: int, a: Tensor, b: Tensor, b_ld: int, M: int, E: int, n_in: int, n_out: int, code: int) -> Optional[Tensor]:
+    nbytes = lib().ps_expert_linear_workspace(pass_, a.data_ptr(), _ld(a), b.data_ptr(), b_ld, M, E, n_in, n_out, code)
+    return torch.empty(nbytes, device=a.device, dtype=torch.uint8) if nbytes else None
+
+
+def _linear_fwd(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Tensor) -> Tensor:
+    (M, n_in), (E, n_out, _) = x.shape, weight.shape
+    code = DTYPE_CODES[x.dtype]
+    x, weight = _spaced(x), weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    with _on(x.device):
+        y = torch.empty(M, n_out, device=x.device, dtype=x.dtype)
+        ws = _workspace(0, x, weight, n_in, M, E, n_in, n_out, code)
+        check(lib().ps_expert_linear_fwd(_p(x), _ld(x), _p(weight), _p(bias), _p(offsets), M, E, n_in, n_out, code, _p(y), _p(ws), _stream()),
+              "ps_expert_linear_fwd")
+    return y
+
+
 class _ExpertLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, offsets):
         ctx.save_for_backward(x, weight, offsets)
-        ctx.has_bias = bias is not None
-        xs, ws, bs = _spaced(x), weight.contiguous(), None if bias is None else bias.contiguous()
-        (M, n_in), (E, n_out, _) = x.shape, weight.shape
-        with _on(x.device):
-            y = torch.empty(M, n_out, device=x.device, dtype=x.dtype)
-            check(lib().ps_expert_linear_fwd(_p(xs), _ld(xs), _p(ws), _p(bs), _p(offsets), M, E, n_in, n_out, DTYPE_CODES[x.dtype], _p(y), _stream()),
-                  "ps_expert_linear_fwd")
-        return y
+        return _linear_fwd(x, weight, bias, offsets)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, offsets = ctx.saved_tensors
         (M, n_in), (E, n_out, _) = x.shape, weight.shape
         code = DTYPE_CODES[x.dtype]
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         dx = dw = db = None
         with _on(x.device):
             dy = _spaced(dy)
             if need_x:
-                ws = weight.contiguous()
+                w = weight.contiguous()
                 dx = torch.empty(M, n_in, device=x.device, dtype=x.dtype)
-                check(lib().ps_expert_linear_dx(_p(dy), _ld(dy), _p(ws), _p(offsets), M, E, n_in, n_out, code, _p(dx), _stream()),
+                ws = _workspace(1, dy, w, n_in, M, E, n_in, n_out, code)
+                check(lib().ps_expert_linear_dx(_p(dy), _ld(dy), _p(w), _p(offsets), M, E, n_in, n_out, code, _p(dx), _p(ws), _stream()),
                       "ps_expert_linear_dx")
-            if need_w or (need_b and ctx.has_bias):
+            if need_w or need_b:
                 xs = _spaced(x)
                 dw = torch.empty(E, n_out, n_in, device=x.device, dtype=x.dtype)
-                db = torch.empty(E, n_out, device=x.device, dtype=x.dtype) if ctx.has_bias and need_b else None
-                nbytes = lib().ps_expert_linear_dw_workspace(M, E, n_in, n_out)
-                ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8) if nbytes else None
+                db = torch.empty(E, n_out, device=x.device, dtype=x.dtype) if need_b else None
+                ws = _workspace(2, dy, xs, _ld(xs), M, E, n_in, n_out, code)
                 check(lib().ps_expert_linear_dw(_p(dy), _ld(dy), _p(xs), _ld(xs), _p(offsets), M, E, n_in, n_out, code, _p(dw), _p(db), _p(ws),
                                                 _stream()), "ps_expert_linear_dw")
         return dx, dw if need_w else None, db, None
@@ -262,4 +291,7 @@ def expert_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Un
         raise ValueError(f"presight_amd: x must have the plan's {plan.num_places} rows (got {x.shape[0]})")
     if max(weight.shape[1:]) > 1 << 20 or weight.shape[0] > 65536:
         raise ValueError("presight_amd: expert_linear takes up to 65536 experts and 2**20 features")
-    return _ExpertLinear.apply(x, weight, bias, offsets.to(torch.int32).contiguous())
+    offsets = offsets.to(torch.int32).contiguous()
+    if not _wants_grad(x, weight, bias):
+        return _linear_fwd(x, weight, bias, offsets)
+    return _ExpertLinear.apply(x, weight, bias, offsets)

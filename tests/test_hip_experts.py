@@ -86,9 +86,9 @@ def test_library_refuses_bad_sizes():
                h.ps_expert_plan(None, 0, 8, 4, None, None, None, None, None),
                h.ps_expert_dispatch(None, 4, None, None, 4, 0, 4, 0, None, None), h.ps_expert_dispatch(None, 4, None, None, 4, 2, 4, 0, None, None),
                h.ps_expert_combine(None, 4, None, None, 1 << 30, 2, 4, 0, None, None),
-               h.ps_expert_linear_fwd(None, 4, None, None, None, 8, 2, 5, 4, 0, None, None),
-               h.ps_expert_linear_fwd(None, 5, None, None, None, 8, 2, 5, 4, 0, None, None),
-               h.ps_expert_linear_dx(None, 3, None, None, 8, 2, 5, 4, 0, None, None),
+               h.ps_expert_linear_fwd(None, 4, None, None, None, 8, 2, 5, 4, 0, None, None, None),
+               h.ps_expert_linear_fwd(None, 5, None, None, None, 8, 2, 5, 4, 0, None, None, None),
+               h.ps_expert_linear_dx(None, 3, None, None, 8, 2, 5, 4, 0, None, None, None),
                h.ps_expert_linear_dw(None, 4, None, 5, None, 8, 0, 5, 4, 0, None, None, None, None)):
         assert rc != 0
     with pytest.raises(Exception, match="experts"):
