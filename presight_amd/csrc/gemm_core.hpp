@@ -36,9 +36,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void* base, int64
 // bytes of k and keeps the operand's own direction: KC as rows of k, RC as rows of BR elements of one k each, from which 16-bit fragments
 // are read with the transposing LDS loads (16 lanes fetch 4 k x 16 rows, each lane ends up with the 4 k of its row) and fp32 ones element by
 // element.  What would collide in the 64 banks is spread by permuting chunks within a tile row, on the global side of the load.
-template <typename T, int BR, int NT, bool RC>
+template <typename T, int BR, int NT, bool RC, int KR = kTileK<T>>  // KR: k of an RC tile
 struct DirectTile {
-  static constexpr int kBytes = BR * kTileRowBytes;
+  static constexpr int kBytes = RC ? KR * BR * (int)sizeof(T) : BR * kTileRowBytes;
   static constexpr int N = kBytes / 16 / NT;                    // chunks per thread
   static constexpr int kRow = RC ? BR * (int)sizeof(T) : kTileRowBytes;  // bytes of a tile row
   static constexpr int kAcross = kRow / 16;
@@ -110,9 +110,9 @@ struct DirectTile {
 };
 
 // An operand's tiles along k: `rows` rows (KC) or elements of a row (RC) from the tile's corner `base` on, K of k
-template <typename T, int BR, int NT, bool RC>
+template <typename T, int BR, int NT, bool RC, int KR = kTileK<T>>
 struct DirectSource {
-  DirectTile<T, BR, NT, RC> tile;
+  DirectTile<T, BR, NT, RC, KR> tile;
   const T* base;
   int64_t ld;
   int rows, K;
@@ -121,13 +121,24 @@ struct DirectSource {
   }
   __device__ __forceinline__ void load(int k0, char* to) const {
     if constexpr (RC) {
-      const int kr = K - k0 < kTileK<T> ? K - k0 : kTileK<T>;
+      const int kr = K - k0 < KR ? K - k0 : KR;
       tile.load(window(base + k0 * ld, ((int64_t)(kr - 1) * ld + rows) * sizeof(T)), rows, to);
     } else {
       tile.load(window(base + k0, ((int64_t)(rows - 1) * ld + (K - k0)) * sizeof(T)), K - k0, to);
     }
   }
 };
+
+// A barrier behind which all but the last `keep` of every wave's loads have landed in LDS, and every wave has read what it read before.
+// (The compiler's own barrier would wait for all of them; it does not know that LDS changes here, hence the empty statements.)
+template <int keep>
+__device__ __forceinline__ void tile_barrier() {
+  static_assert(keep >= 0 && keep < 64, "six bits");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((keep & 15) | 7 << 4 | 0 << 8 | (keep >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 
 // One 16 x 16 block of a product over one fragment of k.  B's rows are the matrix instruction's rows, so a lane ends up with four
 // consecutive n of one m: acc[r] = C[lane & 15][4 (lane >> 4) + r].  fp32: the k inside a chunk are taken in the same order for both

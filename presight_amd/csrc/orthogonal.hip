@@ -11,6 +11,7 @@
 // multiplies r by the power of two `grow` that bounds a + b t + c t^2, until r passes 1/2, and keeps it from then on.  The caller
 // checks that the iterates' squared singular values and the polynomial stay under 15: with X^ <= 2 X all entries are below 64, the
 // planes' end, and 1024 * entry keeps the low half normal down to entries of 2^-12.
+#include <type_traits>
 #include "gemm_core.hpp"
 
 namespace {
@@ -28,10 +29,14 @@ __device__ __forceinline__ void split(V v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(float)(t - (V)(float)hi);
 }
 
+// The two planes lie side by side, 32 columns of hi and then the same 32 of lo: 128 bytes, a cache line and a tile row.  Rows are padded to
+// whole lines of 64 columns.
+__host__ __device__ inline int64_t pair_at(int col, int plane) { return (int64_t)(col >> 5) * 64 + plane * 32 + (col & 31); }
+
 struct Shape {  // of one matrix
   int64_t m, n;      // as given
   int s, l;          // short and long side
-  int sp, lp;        // rounded up to whole tiles of k (zeros there)
+  int sp, lp;        // rounded up to 64 (zeros there); rows of a pair are twice as long
   bool tall;         // m > n: X = G^T
 };
 Shape shape_of(int64_t m, int64_t n) {
@@ -45,18 +50,17 @@ Shape shape_of(int64_t m, int64_t n) {
   return h;
 }
 
-// Workspace of a batch: pairs of planes (hi, then lo, for all matrices)
+// Workspace of a batch
 struct Work {
-  _Float16 *x[2], *gram, *poly;  // [B][s][lp] twice, [B][s][sp], [B][s][sp]
+  _Float16 *x[2], *gram, *poly;  // pairs: [B][s][2 lp] twice, [B][s][2 sp], [B][s][2 sp]
   double* norms;                 // [B][parts]
   float* ratio;                  // [B] r at the start
   int parts;
-  int64_t x_plane, s_plane, bytes;
+  int64_t bytes;
 };
 Work work_of(const Shape& h, int64_t B, void* base) {
   Work w;
-  w.x_plane = B * h.s * (int64_t)h.lp;
-  w.s_plane = B * h.s * (int64_t)h.sp;
+  const int64_t x_bytes = B * h.s * (int64_t)h.lp * 4, s_bytes = B * h.s * (int64_t)h.sp * 4;
   char* p = (char*)base;
   auto take = [&](int64_t bytes) {
     char* q = p;
@@ -67,10 +71,10 @@ Work work_of(const Shape& h, int64_t B, void* base) {
   w.parts = (int)(parts < 1 ? 1 : (parts > kNormParts ? kNormParts : parts));
   w.norms = (double*)take(B * kNormParts * 8);
   w.ratio = (float*)take(B * 4);
-  w.x[0] = (_Float16*)take(w.x_plane * 4);
-  w.x[1] = (_Float16*)take(w.x_plane * 4);
-  w.gram = (_Float16*)take(w.s_plane * 4);
-  w.poly = (_Float16*)take(w.s_plane * 4);
+  w.x[0] = (_Float16*)take(x_bytes);
+  w.x[1] = (_Float16*)take(x_bytes);
+  w.gram = (_Float16*)take(s_bytes);
+  w.poly = (_Float16*)take(s_bytes);
   w.bytes = p - (char*)base;
   return w;
 }
@@ -180,7 +184,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work
   for (int id = threadIdx.x; id < 2 * 64 * 8; id += 256) {
     const int p = id >> 9, row = (id >> 3) & 63, col = (id & 7) * 8;
     if (m0 + row < h.s && n0 + col < h.lp)
-      *reinterpret_cast<u32x4*>(w.x[0] + p * w.x_plane + (b * h.s + m0 + row) * h.lp + n0 + col) = *reinterpret_cast<const u32x4*>(&tile[p][row][col]);
+      *reinterpret_cast<u32x4*>(w.x[0] + (b * h.s + m0 + row) * 2 * h.lp + pair_at(n0 + col, p)) = *reinterpret_cast<const u32x4*>(&tile[p][row][col]);
   }
 }
 
@@ -203,101 +207,114 @@ struct Poly {
   float grow;
 };
 
-struct Operands {
-  const _Float16 *a, *b;  // [B][ra][k]; [B][rb][k], or for kApply and kLast [B][k_rows][ldb]; the lo planes are a_plane / b_plane behind
-  int64_t a_plane, b_plane;
-  int ra, rb, k;  // k: padded, and the rows' distance
+struct Operands {  // pairs
+  const _Float16 *a, *b;  // [B][ra][2 k]; [B][rb][2 k], or for kApply and kLast [B][k_rows][2 ldb]
+  int ra, rb, k;          // k: padded, and half the rows' distance
   int k_rows, ldb;
 };
 
-// A workgroup's tile: 128 x 128, eight waves of 64 x 32.  Two tiles of 64 k of all four planes (hi and lo of either operand, 64 KiB) in
-// LDS: the loads of the next tile run beside this one's 384 matrix instructions, three on every pair of fragments.  The two small
-// products add up apart from the large one: each of their additions to it would cost it another rounding.
+// A workgroup's tile: BM x BN; a stage is 32 k of both planes of either operand, one tile row of 128 bytes for a row of k (KC).  A compute
+// unit can have about 17 bytes per cycle of the L2's in flight, so the tile decides how fast the matrix instructions are fed: at their full
+// rate 256 x 128 asks for 32 bytes per cycle, 128 x 128 for 43 and 64 x 64 for 85, and a step of k takes as long as its stage of 48, 32 or
+// 16 KiB takes to arrive.  256 rows are taken where that still makes a tile for every second compute unit (2048 x 4096, P X: 131 -> 113 us;
+// 8 x 1024 x 2048: 150 -> 122), else 64 x 64 while no compute unit gets more than the two that fit its LDS (all five steps: 3 x 385 x 129
+// 229 -> 132 us, 1024 x 1024 479 -> 273, 1536 x 1536 671 -> 517; with more of them 2048 x 4096 would go from 1236 to 1317), else 128 x 128.
+// The two small products add up apart from the large one: each of their additions to it would cost it another rounding.
 //
-// The result leaves through LDS as rows of 256 bytes; of a symmetric one only the tiles on and below the diagonal are computed, and leave
-// turned as well.
-constexpr int kPairTile = 128, kPairThreads = 512, kPairPlane = kPairTile * kTileRowBytes;  // bytes of one plane's tile
-constexpr int kPairLds = 2 * 4 * kPairPlane;
+// The result leaves through LDS as rows of whole lines.  Of a symmetric one only what lies on and below the diagonal's BN x BN blocks is
+// computed and written, and then written turned.
+constexpr int kPairK = 32;
+template <int BM>
+struct PairTile {
+  static constexpr int kN = BM == 64 ? 64 : 128, kThreads = BM == 64 ? 256 : 512;
+  static constexpr int kWaveM = BM == 64 ? 32 : 64, kWavesN = kThreads / 64 / (BM / kWaveM), kWaveN = kN / kWavesN;
+  static constexpr int kStages = BM == 256 ? 3 : 4, kGroup = BM == 256 ? 1 : 2;  // in LDS; per barrier
+  static constexpr int kStage = (BM + kN) * kTileRowBytes, kLds = kStages * kStage;
+};
 
-// byte of element `col` (fp16 or fp32) in row `row` of a turned-out tile: 16-byte chunks spread so that the 16 rows that a wave writes at a
-// time and the 4 columns of a lane meet different banks
-template <typename V>
-__device__ __forceinline__ int out_addr(int row, int col) {
-  const int byte = col * (int)sizeof(V);
-  return row * kPairTile * (int)sizeof(V) + (((byte >> 4) ^ (row & 15)) << 4) + (byte & 15);
+// a tile on its way out: rows of `bytes`, 16-byte chunks spread so that 16 rows at a time meet different banks
+__device__ __forceinline__ int out_addr(int row, int bytes, int byte) { return row * bytes + (((byte >> 4) ^ (row & 15)) << 4) + (byte & 15); }
+
+// tiles of a symmetric product in the row of tiles tm: those that reach the diagonal or below
+__host__ __device__ inline int symmetric_tiles(int tm, int across, int n_tiles) {  // across: tiles' height over their width
+  const int n = (tm + 1) * across;
+  return n < n_tiles ? n : n_tiles;
 }
 
-template <typename T, Product WHAT>
-__global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Shape h, Work w, int batches, int step, Poly c, Result res) {
-  constexpr int B = kPairTile, NT = kPairThreads, MI = 4, NJ = 2;
+template <typename T, Product WHAT, int BM>
+__global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Operands o, Shape h, Work w, int batches, int tiles, int step, Poly c, Result res) {
+  using Tile = PairTile<BM>;
+  constexpr int BN = Tile::kN, NT = Tile::kThreads, WN = Tile::kWavesN, MI = Tile::kWaveM / 16, NJ = Tile::kWaveN / 16, kStages = Tile::kStages,
+                kStage = Tile::kStage, kGroup = Tile::kGroup;
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
-  using TileA = DirectTile<_Float16, B, NT, false>;
-  using TileB = DirectTile<_Float16, B, NT, !kSymmetric>;
+  using SourceA = DirectSource<_Float16, BM, NT, false>;
+  using SourceB = std::conditional_t<kSymmetric, DirectSource<_Float16, BN, NT, false>, DirectSource<_Float16, 2 * BN, NT, true, kPairK>>;
+  constexpr int kLoads = decltype(SourceA::tile)::N + decltype(SourceB::tile)::N;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  const int m_tiles = (o.ra + B - 1) / B, n_tiles = (o.rb + B - 1) / B;
-  // (the batch's matrices one under the other; of a symmetric result the tiles tm >= tn, row by row)
-  const int tiles = kSymmetric ? m_tiles * (m_tiles + 1) / 2 : m_tiles * n_tiles, place = xcd_place(blockIdx.x, tiles * batches);
+  const int m_tiles = (o.ra + BM - 1) / BM, n_tiles = (o.rb + BN - 1) / BN;
+  // (the batch's matrices one under the other; `tiles`: of one of them)
+  const int place = xcd_place(blockIdx.x, tiles * batches);
   if (place < 0) return;
-  int tm, tn;
+  int tm = 0, tn;
   int64_t batch;
   if constexpr (kSymmetric) {
     batch = place / tiles;
-    const int in = place % tiles;
-    tm = (int)((sqrtf(8.0f * in + 1.0f) - 1.0f) * 0.5f);
-    while (tm * (tm + 1) / 2 > in) --tm;
-    while ((tm + 1) * (tm + 2) / 2 <= in) ++tm;
-    tm = uniform(tm);
-    tn = in - tm * (tm + 1) / 2;
+    tn = place % tiles;
+    for (int n; tn >= (n = symmetric_tiles(tm, BM / BN, n_tiles)); ++tm) tn -= n;
   } else {
     const TileAt at = patched_tile(place, batches * m_tiles, n_tiles);
     batch = at.m / m_tiles;
     tm = at.m % m_tiles, tn = at.n;
   }
-  const int m0 = tm * B, n0 = tn * B;
-  const int rows = o.ra - m0 < B ? o.ra - m0 : B, cols = o.rb - n0 < B ? o.rb - n0 : B;
-  const _Float16* pa = o.a + (batch * o.ra + m0) * o.k;
-  const _Float16* pb = kSymmetric ? o.b + (batch * o.rb + n0) * o.k : o.b + batch * o.k_rows * o.ldb + n0;
-  const int ldb = kSymmetric ? o.k : o.ldb, in_b = kSymmetric ? cols : (h.lp - n0 < B ? h.lp - n0 : B), kb = kSymmetric ? o.k : o.k_rows;
-  const DirectSource<_Float16, B, NT, false> ah(pa, o.k, rows, o.k), al(pa + o.a_plane, o.k, rows, o.k);
-  const DirectSource<_Float16, B, NT, !kSymmetric> bh(pb, ldb, in_b, kb), bl(pb + o.b_plane, ldb, in_b, kb);
-  auto load = [&](int k0, char* to) {
-    ah.load(k0, to);
-    al.load(k0, to + kPairPlane);
-    bh.load(k0, to + 2 * kPairPlane);
-    bl.load(k0, to + 3 * kPairPlane);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int rows = o.ra - m0 < BM ? o.ra - m0 : BM, cols = o.rb - n0 < BN ? o.rb - n0 : BN;
+  const SourceA sa(o.a + (batch * o.ra + m0) * 2 * o.k, 2 * o.k, rows, 2 * o.k);
+  const SourceB sb = kSymmetric ? SourceB(o.b + (batch * o.rb + n0) * 2 * o.k, 2 * o.k, cols, 2 * o.k)
+                                : SourceB(o.b + batch * o.k_rows * 2 * o.ldb + 2 * n0, 2 * o.ldb, 2 * (o.ldb - n0), o.k_rows);
+  auto load = [&](int stage) {  // stage by stage of k; KC counts both planes
+    char* to = lds + stage % kStages * kStage;
+    sa.load(stage * 2 * kPairK, to);
+    sb.load(stage * (kSymmetric ? 2 : 1) * kPairK, to + BM * kTileRowBytes);
   };
-  const int wave = threadIdx.x >> 6, wm = (wave >> 2) * 64, wn = (wave & 3) * 32;
+  const int wave = threadIdx.x >> 6, wm = wave / WN * Tile::kWaveM, wn = wave % WN * Tile::kWaveN;
   f32x4 acc[MI][NJ], fine[MI][NJ];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = fine[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  load(0, lds);
-  __syncthreads();
-  for (int k0 = 0, cur = 0; k0 < o.k; k0 += kTileK<_Float16>, cur ^= 1) {
-    const char* t = lds + cur * 4 * kPairPlane;
-    if (k0 + kTileK<_Float16> < o.k) load(k0 + kTileK<_Float16>, lds + (cur ^ 1) * 4 * kPairPlane);
+  const int steps = o.k / kPairK;  // (even)
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+  for (int i = 0; i < kStages - kGroup; ++i) load(i);
+  for (int i = 0; i < steps; i += kGroup) {
+    tile_barrier<(kStages - 2 * kGroup) * kLoads>();
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) load(i + u + kStages - kGroup);  // (where the stages before i were; zeros behind the last)
+#pragma unroll
+    for (int u = 0; u < kGroup; ++u) {
+      const char* t = lds + (i + u) % kStages * kStage;
       u32x4 fa[2][MI], fb[2][NJ];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[p][j] = TileB::fragment(t + (2 + p) * kPairPlane, wn + j * 16, s);
+        for (int j = 0; j < NJ; ++j) {
+          const int n = wn + j * 16;
+          fb[p][j] = kSymmetric ? decltype(sb.tile)::fragment(t + BM * kTileRowBytes, n, p)
+                                : decltype(sb.tile)::fragment(t + BM * kTileRowBytes, (int)pair_at(n, p), 0);
+        }
 #pragma unroll
-        for (int i = 0; i < MI; ++i) fa[p][i] = TileA::fragment(t + p * kPairPlane, wm + i * 16, s);
+        for (int q = 0; q < MI; ++q) fa[p][q] = decltype(sa.tile)::fragment(t, wm + q * 16, p);
       }
 #pragma unroll
-      for (int i = 0; i < MI; ++i)
+      for (int q = 0; q < MI; ++q)
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-          acc[i][j] = mma_block<_Float16>(fa[0][i], fb[0][j], acc[i][j]);
-          fine[i][j] = mma_block<_Float16>(fa[0][i], fb[1][j], fine[i][j]);
-          fine[i][j] = mma_block<_Float16>(fa[1][i], fb[0][j], fine[i][j]);
+          acc[q][j] = mma_block<_Float16>(fa[0][q], fb[0][j], acc[q][j]);
+          fine[q][j] = mma_block<_Float16>(fa[0][q], fb[1][j], fine[q][j]);
+          fine[q][j] = mma_block<_Float16>(fa[1][q], fb[0][j], fine[q][j]);
         }
     }
-    __syncthreads();
   }
+  __syncthreads();
   const float ratio = ratio_at(w.ratio[batch], step, c.grow);
   // kPoly: a + b r^2 S^ + c r^4 S^ S^ with the coefficients as pairs of floats: an error of a coefficient would be common to all entries and
   // grow like a singular value's | kApply: over the step's growth of r | kLast: X = r X^
@@ -307,60 +324,30 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
   const float out_scale = WHAT == kApply ? kProductScale * (ratio > 0.0f ? ratio / ratio_at(ratio, 1, c.grow) : 1.0f)
                                          : (WHAT == kLast ? kProductScale * ratio : kProductScale);
   const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-  constexpr int kOut = B * B * 2;  // bytes of a plane's tile: hi, lo, then hi and lo turned
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
-    const int m = wm + i * 16 + r;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int n = wn + j * 16 + g * 4;
-      if constexpr (WHAT == kLast) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float v = (acc[i][j][q] + fine[i][j][q]) * out_scale;
-          *reinterpret_cast<float*>(lds + (h.tall ? out_addr<float>(n + q, m) : out_addr<float>(m, n + q))) = v;
-        }
-      } else {
-        Pack<_Float16, 4> hi, lo, gh, gl;
-        if constexpr (WHAT == kPoly) {
-          gh = gl = Pack<_Float16, 4>{};
-          if (m < rows && n < cols) {  // (rows are padded to 64: whole packs)
-            const int64_t at = (batch * h.s + m0 + m) * h.sp + n0 + n;
-            gh = load_pack<_Float16, 4>(w.gram + at);
-            gl = load_pack<_Float16, 4>(w.gram + w.s_plane + at);
-          }
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float sum = acc[i][j][q] + fine[i][j][q];
-          if constexpr (WHAT == kPoly) {
-            const bool one = m0 + m == n0 + n + q && m < rows;  // (rows and columns of the padding stay zero)
-            const float was = (float)gh.v[q] + (float)gl.v[q];
-            const float small = fmaf(cc_lo, sum, fmaf(cb_lo, was, one ? ca_lo : 0.0f));
-            split(fmaf(cb_hi, was, one ? ca_hi : 0.0f) + fmaf(cc_hi, sum, small), hi.v[q], lo.v[q]);
-          } else {
-            split(sum * out_scale, hi.v[q], lo.v[q]);
-          }
-          if constexpr (kSymmetric) {
-            *reinterpret_cast<_Float16*>(lds + 2 * kOut + out_addr<_Float16>(n + q, m)) = hi.v[q];
-            *reinterpret_cast<_Float16*>(lds + 3 * kOut + out_addr<_Float16>(n + q, m)) = lo.v[q];
-          }
-        }
-        store_pack(reinterpret_cast<_Float16*>(lds + out_addr<_Float16>(m, n)), hi);
-        store_pack(reinterpret_cast<_Float16*>(lds + kOut + out_addr<_Float16>(m, n)), lo);
-      }
-    }
-  }
-  __syncthreads();
   if constexpr (WHAT == kLast) {
+    const int image = (h.tall ? BM : BN) * 4;  // bytes of a row of G's direction
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int m = wm + i * 16 + r, n = wn + j * 16 + g * 4;
+        const f32x4 v = (acc[i][j] + fine[i][j]) * out_scale;
+        if (h.tall) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) *reinterpret_cast<float*>(lds + out_addr(n + q, image, m * 4)) = v[q];
+        } else {
+          *reinterpret_cast<f32x4*>(lds + out_addr(m, image, n * 4)) = v;
+        }
+      }
+    __syncthreads();
     const int r0 = h.tall ? n0 : m0, c0 = h.tall ? m0 : n0, rn = h.tall ? cols : rows, cn = h.tall ? rows : cols;
     const int64_t base = batch * h.m * h.n + (int64_t)r0 * h.n + c0;
     // four at a time where rows and addresses allow it
     const bool packed = h.n % 4 == 0 && ((uintptr_t)res.out & (4 * sizeof(T) - 1)) == 0;
-    for (int id = threadIdx.x; id < B * (B / 4); id += NT) {
-      const int row = id / (B / 4), col = id % (B / 4) * 4;
+    for (int id = threadIdx.x; id < BM * BN / 4; id += NT) {
+      const int row = id / (image / 16), col = id % (image / 16) * 4;
       if (row >= rn || col >= cn) continue;
-      const f32x4 v = *reinterpret_cast<const f32x4*>(lds + out_addr<float>(row, col));
+      const f32x4 v = *reinterpret_cast<const f32x4*>(lds + out_addr(row, image, col * 4));
       const int64_t at = base + (int64_t)row * h.n + col;
       if (res.update) {
         float* p = reinterpret_cast<float*>(res.out) + at;
@@ -390,24 +377,83 @@ __global__ __launch_bounds__(kPairThreads) void ns_product_kernel(Operands o, Sh
     }
   } else {
     const int ld = kSymmetric ? h.sp : h.lp;
-    const int64_t plane = kSymmetric ? w.s_plane : w.x_plane;
-    _Float16* out = (WHAT == kGram ? w.gram : (WHAT == kPoly ? w.poly : w.x[(step + 1) & 1])) + batch * h.s * ld;
-    const int parts = kSymmetric && tm != tn ? 4 : 2;
-    for (int id = threadIdx.x; id < parts * B * (B / 8); id += NT) {
-      const int part = id / (B * (B / 8)), row = id / (B / 8) % B, col = id % (B / 8) * 8;
-      const u32x4 v = *reinterpret_cast<const u32x4*>(lds + part * kOut + out_addr<_Float16>(row, col));
-      const int rn = part < 2 ? rows : cols, r0 = part < 2 ? m0 : n0, c0 = part < 2 ? n0 : m0;
-      if (row < rn && c0 + col < ld) *reinterpret_cast<u32x4*>(out + (part & 1) * plane + (int64_t)(r0 + row) * ld + c0 + col) = v;
+    _Float16* out = (WHAT == kGram ? w.gram : (WHAT == kPoly ? w.poly : w.x[(step + 1) & 1])) + batch * h.s * 2 * ld;
+#pragma unroll
+    for (int turned = 0; turned < (kSymmetric ? 2 : 1); ++turned) {
+      if (turned) __syncthreads();
+      const int image = (turned ? BM : BN) * 4;  // bytes of a row
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const int m = wm + i * 16 + r, n = wn + j * 16 + g * 4;
+          Pack<_Float16, 4> hi, lo, gh{}, gl{};
+          if (WHAT == kPoly && m < rows && n < cols) {  // (rows are padded to 64: whole packs)
+            const _Float16* was = w.gram + (batch * h.s + m0 + m) * 2 * ld;
+            gh = load_pack<_Float16, 4>(was + pair_at(n0 + n, 0));
+            gl = load_pack<_Float16, 4>(was + pair_at(n0 + n, 1));
+          }
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float sum = acc[i][j][q] + fine[i][j][q];
+            if constexpr (WHAT == kPoly) {
+              const bool one = m0 + m == n0 + n + q && m < rows;  // (rows and columns of the padding stay zero)
+              const float was = (float)gh.v[q] + (float)gl.v[q];
+              const float small = fmaf(cc_lo, sum, fmaf(cb_lo, was, one ? ca_lo : 0.0f));
+              split(fmaf(cb_hi, was, one ? ca_hi : 0.0f) + fmaf(cc_hi, sum, small), hi.v[q], lo.v[q]);
+            } else {
+              split(sum * out_scale, hi.v[q], lo.v[q]);
+            }
+            if (turned) {
+              *reinterpret_cast<_Float16*>(lds + out_addr(n + q, image, (int)pair_at(m, 0) * 2)) = hi.v[q];
+              *reinterpret_cast<_Float16*>(lds + out_addr(n + q, image, (int)pair_at(m, 1) * 2)) = lo.v[q];
+            }
+          }
+          if (!turned) {
+            store_pack(reinterpret_cast<_Float16*>(lds + out_addr(m, image, (int)pair_at(n, 0) * 2)), hi);
+            store_pack(reinterpret_cast<_Float16*>(lds + out_addr(m, image, (int)pair_at(n, 1) * 2)), lo);
+          }
+        }
+      __syncthreads();
+      const int r0 = turned ? n0 : m0, c0 = turned ? m0 : n0, rn = turned ? cols : rows;
+      for (int id = threadIdx.x; id < BM * BN * 4 / 16; id += NT) {
+        const int row = id / (image / 16), chunk = id % (image / 16), col = c0 + (chunk >> 3) * 32;
+        if (row >= rn || col >= ld) continue;
+        if (kSymmetric) {  // blocks on and below the diagonal as they are, those below turned
+          const int low = turned ? col / BN : (r0 + row) / BN, high = turned ? r0 / BN : n0 / BN;
+          if (turned ? low <= high : low < high) continue;
+        }
+        *reinterpret_cast<u32x4*>(out + (int64_t)(r0 + row) * 2 * ld + 2 * c0 + chunk * 8) = *reinterpret_cast<const u32x4*>(lds + out_addr(row, image, chunk * 16));
+      }
     }
   }
 }
 
+template <typename T, Product WHAT, int BM>
+int product_tiles(const Operands& o) {
+  constexpr int BN = PairTile<BM>::kN;
+  const int m = (o.ra + BM - 1) / BM, n = (o.rb + BN - 1) / BN;
+  if (WHAT == kApply || WHAT == kLast) return m * n;
+  int all = 0;
+  for (int t = 0; t < m; ++t) all += symmetric_tiles(t, BM / BN, n);
+  return all;
+}
+
+template <typename T, Product WHAT, int BM>
+void launch_product_tile(const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res, hipStream_t s) {
+  const int tiles = product_tiles<T, WHAT, BM>(o);
+  hipFuncSetAttribute((const void*)ns_product_kernel<T, WHAT, BM>, hipFuncAttributeMaxDynamicSharedMemorySize, PairTile<BM>::kLds);
+  ns_product_kernel<T, WHAT, BM><<<(unsigned)xcd_blocks(tiles * B), PairTile<BM>::kThreads, PairTile<BM>::kLds, s>>>(o, h, w, (int)B, tiles, step, c, res);
+}
+
 template <typename T, Product WHAT>
 void launch_product(const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res, hipStream_t s) {
-  const int64_t m = (o.ra + kPairTile - 1) / kPairTile, n = (o.rb + kPairTile - 1) / kPairTile;
-  const int64_t blocks = xcd_blocks((WHAT == kGram || WHAT == kPoly ? m * (m + 1) / 2 : m * n) * B);
-  hipFuncSetAttribute((const void*)ns_product_kernel<T, WHAT>, hipFuncAttributeMaxDynamicSharedMemorySize, kPairLds);
-  ns_product_kernel<T, WHAT><<<(unsigned)blocks, kPairThreads, kPairLds, s>>>(o, h, w, (int)B, step, c, res);
+  if (product_tiles<T, WHAT, 256>(o) * B >= 128)
+    launch_product_tile<T, WHAT, 256>(o, h, w, B, step, c, res, s);
+  else if (product_tiles<T, WHAT, 64>(o) * B <= 512)
+    launch_product_tile<T, WHAT, 64>(o, h, w, B, step, c, res, s);
+  else
+    launch_product_tile<T, WHAT, 128>(o, h, w, B, step, c, res, s);
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -589,9 +635,9 @@ int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Pol
   }
   for (int i = 0; i < steps; ++i) {
     const _Float16* x = w.x[i & 1];
-    launch_product<T, kGram>({x, x, w.x_plane, w.x_plane, h.s, h.s, h.lp, 0, 0}, h, w, B, i, c, res, s);
-    launch_product<T, kPoly>({w.gram, w.gram, w.s_plane, w.s_plane, h.s, h.s, h.sp, 0, 0}, h, w, B, i, c, res, s);
-    const Operands apply{w.poly, x, w.s_plane, w.x_plane, h.s, h.l, h.sp, h.s, h.lp};
+    launch_product<T, kGram>({x, x, h.s, h.s, h.lp, 0, 0}, h, w, B, i, c, res, s);
+    launch_product<T, kPoly>({w.gram, w.gram, h.s, h.s, h.sp, 0, 0}, h, w, B, i, c, res, s);
+    const Operands apply{w.poly, x, h.s, h.l, h.sp, h.s, h.lp};
     if (i + 1 < steps)
       launch_product<T, kApply>(apply, h, w, B, i, c, res, s);
     else
