@@ -20,6 +20,9 @@ struct RowTile {
 
 __device__ __forceinline__ int64_t bounded(int v, int64_t M) { return v < 0 ? 0 : (v > M ? M : v); }
 
+// what M rows of E experts can make at most
+__host__ __device__ inline int64_t row_tiles_at_most(int64_t M, int E, int piece) { return (M + piece - 1) / piece + E; }
+
 // The tiles of `piece` rows that the experts' rows make: a prefix sum over the experts, one per lane, 64 at a time.  Up to 64 experts the
 // lanes keep what they have read.
 struct RowTiles {
@@ -47,7 +50,11 @@ struct RowTiles {
     return __builtin_amdgcn_readlane(incl, 63);
   }
   __device__ __forceinline__ RowTiles(const int* offsets_, int E_, int64_t M_, int piece_) : offsets(offsets_), M(M_), E(E_), piece(piece_), total(0) {
-    for (int e0 = 0; e0 < E; e0 += 64) total += scan(e0);
+    const int64_t most = row_tiles_at_most(M, E, piece);  // (offsets that do not ascend could ask for more than there is room for)
+    for (int e0 = 0; e0 < E; e0 += 64) {
+      const int64_t sum = (int64_t)total + scan(e0);
+      total = (int)(sum < most ? sum : most);
+    }
   }
   // tile t < total, uniform over the wave
   __device__ __forceinline__ RowTile find(int t) {
@@ -283,9 +290,10 @@ __global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ 
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   if (lane == 0) wave_sum[wave] = before;
   __syncthreads();
-  const int64_t first = (int64_t)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
-  const int64_t lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
-  const int n = hi > lo ? (int)((hi - lo + piece - 1) / piece) : 0;
+  const int64_t most = row_tiles_at_most(M, gridDim.y, piece), all = (int64_t)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+  const int64_t first = all < most ? all : most, lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
+  const int64_t mine = hi > lo ? (hi - lo + piece - 1) / piece : 0;
+  const int n = (int)(mine < most - first ? mine : most - first);
   const int64_t size = (int64_t)N * ldo, db_size = (N + 3) / 4 * 4, i = ((int64_t)blockIdx.x * 64 + lane) * 4;
   const bool bias = i >= size;  // (the weights' sums first, then the bias's)
   const float* p = bias ? db_parts + first * db_size + (i - size) : parts + first * size + i;
@@ -320,13 +328,14 @@ __global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ 
 template <typename T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, T* __restrict__ dst) {
   const int across = (cols + kChunk<T> - 1) / kChunk<T>;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, row = id / across;
-  const int c = (int)(id % across) * kChunk<T>;
-  if (row >= rows) return;
-  Pack<T, kChunk<T>> o;
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < rows * across; id += (int64_t)gridDim.x * 256) {
+    const int64_t row = id / across;
+    const int c = (int)(id % across) * kChunk<T>;
+    Pack<T, kChunk<T>> o;
 #pragma unroll
-  for (int q = 0; q < kChunk<T>; ++q) o.v[q] = c + q < cols ? src[row * ld + c + q] : from_f32<T>(0.0f);
-  store_pack(dst + id * kChunk<T>, o);
+    for (int q = 0; q < kChunk<T>; ++q) o.v[q] = c + q < cols ? src[row * ld + c + q] : from_f32<T>(0.0f);
+    store_pack(dst + id * kChunk<T>, o);
+  }
 }
 
 template <typename F>
@@ -384,7 +393,7 @@ Rows packed(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype, ch
   T* copy = (T*)*to;
   *to += bytes;
   const int64_t chunks = rows * (padded(cols, dtype) / kChunk<T>);
-  if (chunks > 0) pack_rows_kernel<T><<<(unsigned)((chunks + 255) / 256), 256, 0, s>>>((const T*)p, ld, rows, (int)cols, copy);
+  if (chunks > 0) pack_rows_kernel<T><<<blocks_of_256(chunks), 256, 0, s>>>((const T*)p, ld, rows, (int)cols, copy);
   return {copy, padded(cols, dtype)};
 }
 
@@ -392,8 +401,8 @@ template <typename T, int B, int WM, int WN, bool W_RC>
 int launch_linear_tile(const Rows& x, const Rows& w, int w_rows, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
                        hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t row_tiles = (M + B - 1) / B + E, blocks = xcd_blocks(row_tiles * ((N + B - 1) / B) + 1);
-  PS_REQUIRE(blocks < ((int64_t)1 << 30), "ps_expert_linear: too many tiles");
+  const int64_t blocks = xcd_blocks(row_tiles_at_most(M, E, B) * ((N + B - 1) / B) + 1);
+  PS_REQUIRE(blocks * 64 * WM * WN < kMaxThreads, "ps_expert_linear: too many tiles");
   allow_lds(linear_kernel<T, B, B, WM, WN, W_RC>, lds);
   linear_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x.p, x.ld, (const T*)w.p, w.ld, w_rows, (const T*)bias, offsets,
                                                                                   M, E, N, K, (T*)y);
@@ -436,7 +445,7 @@ DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out) {
     const int64_t want = (4 * kCompute + t - 1) / t;
     int64_t piece = ((each + want - 1) / want + 63) & ~(int64_t)63;
     p.piece = (int)(piece < 256 ? 256 : piece);
-    p.units = (M + p.piece - 1) / p.piece + E;
+    p.units = row_tiles_at_most(M, E, p.piece);
   }
   return p;
 }
@@ -452,7 +461,7 @@ int launch_dw_tile(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t
                    hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
   const int64_t blocks = xcd_blocks(p.units * ((N + B - 1) / B) * ((K + B - 1) / B));
-  PS_REQUIRE(blocks < ((int64_t)1 << 30), "ps_expert_linear_dw: too many tiles");
+  PS_REQUIRE(blocks * 64 * WM * WN < kMaxThreads, "ps_expert_linear_dw: too many tiles");
   allow_lds(linear_dw_kernel<T, B, B, WM, WN, SPLIT>, lds);
   linear_dw_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy.p, dy.ld, (const T*)x.p, x.ld, offsets, M, E, N, K, ldo,
                                                                                       p.piece, dw, db);

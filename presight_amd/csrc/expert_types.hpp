@@ -15,6 +15,10 @@ __device__ __forceinline__ T from_f32(float v) {  // round to nearest even
   return (T)v;
 }
 
+// A launch holds fewer than 2^32 threads: workgroups of 256 for n of them, which take more than one each beyond 2^31
+constexpr int64_t kMaxThreads = (int64_t)1 << 32;
+inline unsigned blocks_of_256(int64_t n) { return (unsigned)((n < kMaxThreads / 2 ? n + 255 : kMaxThreads / 2) / 256); }
+
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];

@@ -140,22 +140,22 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const void* __
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void dispatch_kernel(const T* __restrict__ x, int64_t x_stride, const int* __restrict__ dst,
                                                        const int* __restrict__ held, int64_t N, int k, int D, int G, T* __restrict__ rows) {
-  const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
-  if (n >= N) return;
   const int l = threadIdx.x & (G - 1);
-  const int total = *held;
-  const int* d = dst + n * k;
-  for (int c = l * VEC; c < D; c += G * VEC) {
-    const Pack<T, VEC> v = load_pack<T, VEC>(x + n * x_stride + c);
-    for (int j = 0; j < k; ++j) {
-      const int p = d[j];
-      if (p >= 0) store_pack(rows + (int64_t)p * D + c, v);
+  const int64_t places = N * k, total = *held;
+  for (int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G; n < N; n += (int64_t)gridDim.x * 256 / G) {
+    const int* d = dst + n * k;
+    for (int c = l * VEC; c < D; c += G * VEC) {
+      const Pack<T, VEC> v = load_pack<T, VEC>(x + n * x_stride + c);
+      for (int j = 0; j < k; ++j) {
+        const int p = d[j];
+        if (p >= 0 && p < places) store_pack(rows + (int64_t)p * D + c, v);
+      }
     }
-  }
-  for (int j = 0; j < k; ++j) {  // the places behind the last expert's rows are shared out over the same lanes
-    const int64_t p = n * k + j;
-    if (p >= total)
-      for (int c = l * VEC; c < D; c += G * VEC) store_pack(rows + p * D + c, Pack<T, VEC>{});
+    for (int j = 0; j < k; ++j) {  // the places behind the last expert's rows are shared out over the same lanes
+      const int64_t p = n * k + j;
+      if (p >= total)
+        for (int c = l * VEC; c < D; c += G * VEC) store_pack(rows + p * D + c, Pack<T, VEC>{});
+    }
   }
 }
 
@@ -164,24 +164,25 @@ __global__ __launch_bounds__(256) void dispatch_kernel(const T* __restrict__ x, 
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ rows, int64_t r_stride, const float* __restrict__ w,
                                                       const int* __restrict__ dst, int64_t N, int k, int D, int G, T* __restrict__ y) {
-  const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
-  if (n >= N) return;
   const int l = threadIdx.x & (G - 1);
-  const int* d = dst + n * k;
-  for (int c = l * VEC; c < D; c += G * VEC) {
-    float acc[VEC] = {};
-    for (int j = 0; j < k; ++j) {
-      const int p = d[j];
-      if (p < 0) continue;
-      const Pack<T, VEC> v = load_pack<T, VEC>(rows + p * r_stride + c);
-      const float wj = w != nullptr ? w[n * k + j] : 1.0f;
+  const int64_t places = N * k;
+  for (int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G; n < N; n += (int64_t)gridDim.x * 256 / G) {
+    const int* d = dst + n * k;
+    for (int c = l * VEC; c < D; c += G * VEC) {
+      float acc[VEC] = {};
+      for (int j = 0; j < k; ++j) {
+        const int p = d[j];
+        if (p < 0 || p >= places) continue;
+        const Pack<T, VEC> v = load_pack<T, VEC>(rows + p * r_stride + c);
+        const float wj = w != nullptr ? w[n * k + j] : 1.0f;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) acc[i] = fmaf(wj, to_f32(v.v[i]), acc[i]);
+        for (int i = 0; i < VEC; ++i) acc[i] = fmaf(wj, to_f32(v.v[i]), acc[i]);
+      }
+      Pack<T, VEC> o;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(acc[i]);
+      store_pack(y + n * D + c, o);
     }
-    Pack<T, VEC> o;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(acc[i]);
-    store_pack(y + n * D + c, o);
   }
 }
 
@@ -190,37 +191,37 @@ template <typename T, int VEC>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ rows, int64_t r_stride,
                                                           const float* __restrict__ w, const int* __restrict__ dst, const int* __restrict__ held,
                                                           int64_t N, int k, int D, int G, T* __restrict__ drows, float* __restrict__ dw) {
-  const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G;
-  const bool live = n < N;  // (no early return: the lanes of a row's group add up below)
   const int l = threadIdx.x & (G - 1);
-  const int total = *held;
-  for (int j = 0; j < k; ++j) {
-    const int p = live ? dst[n * k + j] : -1;
-    float dot = 0.0f;
-    if (p >= 0) {
-      const float wj = w[n * k + j];
-      for (int c = l * VEC; c < D; c += G * VEC) {
-        const Pack<T, VEC> g = load_pack<T, VEC>(dy + n * dy_stride + c);
-        if (dw != nullptr) {
-          const Pack<T, VEC> r = load_pack<T, VEC>(rows + p * r_stride + c);
+  const int64_t places = N * k, total = *held;
+  for (int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G; n < N; n += (int64_t)gridDim.x * 256 / G) {  // (a row's lanes stay together)
+    for (int j = 0; j < k; ++j) {
+      const int p = dst[n * k + j];
+      float dot = 0.0f;
+      if (p >= 0 && p < places) {
+        const float wj = w[n * k + j];
+        for (int c = l * VEC; c < D; c += G * VEC) {
+          const Pack<T, VEC> g = load_pack<T, VEC>(dy + n * dy_stride + c);
+          if (dw != nullptr) {
+            const Pack<T, VEC> r = load_pack<T, VEC>(rows + p * r_stride + c);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) dot = fmaf(to_f32(g.v[i]), to_f32(r.v[i]), dot);
-        }
-        if (drows != nullptr) {
-          Pack<T, VEC> o;
+            for (int i = 0; i < VEC; ++i) dot = fmaf(to_f32(g.v[i]), to_f32(r.v[i]), dot);
+          }
+          if (drows != nullptr) {
+            Pack<T, VEC> o;
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(wj * to_f32(g.v[i]));
-          store_pack(drows + (int64_t)p * D + c, o);
+            for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(wj * to_f32(g.v[i]));
+            store_pack(drows + (int64_t)p * D + c, o);
+          }
         }
       }
+      if (dw != nullptr) {
+        for (int s = G >> 1; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64);
+        if (l == 0) dw[n * k + j] = dot;
+      }
+      const int64_t q = n * k + j;
+      if (drows != nullptr && q >= total)
+        for (int c = l * VEC; c < D; c += G * VEC) store_pack(drows + q * D + c, Pack<T, VEC>{});
     }
-    if (dw != nullptr) {
-      for (int s = G >> 1; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64);
-      if (live && l == 0) dw[n * k + j] = dot;
-    }
-    const int64_t q = n * k + j;
-    if (live && drows != nullptr && q >= total)
-      for (int c = l * VEC; c < D; c += G * VEC) store_pack(drows + q * D + c, Pack<T, VEC>{});
   }
 }
 
@@ -280,6 +281,7 @@ extern "C" int ps_expert_plan(const void* ids, int ids_are_64, int64_t M, int E,
   int bits = 0;
   while ((1 << bits) < E) ++bits;
   const size_t lds = (size_t)(kPlanWaves + 2) * E * sizeof(int);
+  if (lds > 64 * 1024) hipFuncSetAttribute((const void*)plan_place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (M <= kPlanOneBlock) {
     const int64_t chunk = ((M + kPlanThreads - 1) / kPlanThreads) * kPlanThreads;
     plan_place_kernel<<<1, kPlanThreads, lds, s>>>(ids, ids_are_64, M, E, bits, chunk, nullptr, offsets, src, dst);
@@ -301,7 +303,7 @@ extern "C" int ps_expert_dispatch(const void* x, int64_t x_stride, const int32_t
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const int vec = vec_elems(sizeof(T), D, {x_stride}, {x, rows}), G = lanes_per_row(D, vec);
-    const unsigned blocks = (unsigned)((N * G + 255) / 256);
+    const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (dispatch_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)x, x_stride, dst, held, N, k, (int)D, G, (T*)rows)));
     PS_CHECK_LAUNCH();
   });
@@ -315,7 +317,7 @@ extern "C" int ps_expert_combine(const void* rows, int64_t rows_stride, const fl
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const int vec = vec_elems(sizeof(T), D, {rows_stride}, {rows, y}), G = lanes_per_row(D, vec);
-    const unsigned blocks = (unsigned)((N * G + 255) / 256);
+    const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (combine_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)rows, rows_stride, weights, dst, N, k, (int)D, G, (T*)y)));
     PS_CHECK_LAUNCH();
   });
@@ -330,7 +332,7 @@ extern "C" int ps_expert_combine_bwd(const void* dy, int64_t dy_stride, const vo
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     const int vec = vec_elems(sizeof(T), D, {dy_stride, rows_stride}, {dy, rows, drows}), G = lanes_per_row(D, vec);
-    const unsigned blocks = (unsigned)((N * G + 255) / 256);
+    const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (combine_bwd_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)dy, dy_stride, (const T*)rows, rows_stride, weights,
                                                                                            dst, held, N, k, (int)D, G, (T*)drows, dw)));
     PS_CHECK_LAUNCH();

@@ -28,6 +28,7 @@ from .ops import _p, _stream
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 MAX_EXPERTS = 1024
+MAX_WIDTH = 1 << 20
 
 
 def _on(device: torch.device):
@@ -67,12 +68,19 @@ def _once(fn):
 
 
 class ExpertPlan:
-    """Who goes where, for ids [N, k] and E experts (int32 tensors on the ids' device):
+    """Who goes where, for ids [N, k] and E experts (contiguous int32 tensors on the ids' device):
         offsets [E+1]   expert e's rows are the sorted places offsets[e] .. offsets[e+1]
         src     [N*k]   sorted place -> assignment n*k + j, in order of (expert, assignment); -1 behind offsets[E]
-        dst     [N, k]  assignment -> sorted place; -1: to no expert"""
+        dst     [N, k]  assignment -> sorted place; -1: to no expert
+    One made by hand has to hold what expert_plan would: every place once.  (Places outside [0, N*k) count as no expert.)"""
 
     def __init__(self, offsets: Tensor, src: Tensor, dst: Tensor, num_experts: int):
+        if dst.dim() != 2 or offsets.shape != (num_experts + 1,) or src.shape != (dst.numel(),):
+            raise ValueError(f"presight_amd: a plan for {num_experts} experts holds offsets [{num_experts + 1}], src [rows * k] and dst [rows, k] "
+                             f"(got {tuple(offsets.shape)}, {tuple(src.shape)}, {tuple(dst.shape)})")
+        for t in (offsets, src, dst):
+            if t.dtype != torch.int32 or t.device != dst.device or not t.is_contiguous():
+                raise TypeError("presight_amd: a plan holds contiguous int32 tensors on one device")
         self.offsets, self.src, self.dst, self.num_experts = offsets, src, dst, num_experts
         self.num_rows, self.k = dst.shape
 
@@ -207,9 +215,9 @@ def expert_combine(rows: Tensor, weights: Optional[Tensor], plan: ExpertPlan) ->
 
 # ------------------------------------------------------------------------------------------------ the experts' linear layers
 def _spaced(t: Tensor) -> Tensor:
-    """rows that do not overlap (an expanded gradient is copied)"""
+    """rows that neither overlap nor lie further apart than the products' tiles can address (an expanded gradient is copied)"""
     t = _rows(t)
-    return t if t.shape[0] <= 1 or t.stride(0) >= t.shape[1] else t.contiguous()
+    return t if t.shape[0] <= 1 or t.shape[1] <= t.stride(0) <= MAX_WIDTH else t.contiguous()
 
 
 def _ld(t: Tensor) -> int:
@@ -269,8 +277,8 @@ class _ExpertLinear(torch.autograd.Function):
 
 def expert_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Union[Tensor, ExpertPlan]) -> Tensor:
     """x [M, in] sorted by expert, weight [E, out, in], bias [E, out] or None -> y [M, out], y[p] = weight[e] x[p] + bias[e] for the rows
-    p in offsets[e] .. offsets[e+1].  offsets: an ExpertPlan, or int32 / int64 [E+1], ascending; a piece of a longer plan's offsets
-    takes the experts of that piece.  Rows that belong to none of them are zero in y and in x's gradient and do not enter the others;
+    p in offsets[e] .. offsets[e+1].  offsets: an ExpertPlan, or int32 / int64 [E+1], ascending (others give undefined rows, within the
+    results); a piece of a longer plan's offsets takes the experts of that piece.  Rows that belong to none of them are zero in y and in x's gradient and do not enter the others;
     experts without rows have zero gradients."""
     plan = offsets
     offsets = plan.offsets if isinstance(plan, ExpertPlan) else plan
@@ -289,7 +297,7 @@ def expert_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Un
         raise ValueError(f"presight_amd: offsets must be int32 or int64 [{weight.shape[0] + 1}] (got {offsets.dtype} {tuple(offsets.shape)})")
     if isinstance(plan, ExpertPlan) and x.shape[0] != plan.num_places:
         raise ValueError(f"presight_amd: x must have the plan's {plan.num_places} rows (got {x.shape[0]})")
-    if max(weight.shape[1:]) > 1 << 20 or weight.shape[0] > 65536:
+    if max(weight.shape[1:]) > MAX_WIDTH or weight.shape[0] > 65536:
         raise ValueError("presight_amd: expert_linear takes up to 65536 experts and 2**20 features")
     offsets = offsets.to(torch.int32).contiguous()
     if not _wants_grad(x, weight, bias):

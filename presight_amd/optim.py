@@ -342,7 +342,8 @@ class HipMuon:
         p   <- (1 - lr * weight_decay) * p - lr * scale * newton_schulz(u)
     scale: "spectral": sqrt(max(1, out / in)), an update whose effect on activations does not depend on the width;
            "rms": 0.2 * sqrt(max(out, in)), an update of the size Adam's has (its learning rates carry over).
-    Parameters are contiguous fp32; one without a gradient is skipped, its momentum included.  lr may be changed between steps.
+    Parameters are contiguous fp32; one without a gradient is skipped, its momentum included.  lr may be changed between steps; a captured
+    step keeps the lr, weight_decay and set of parameters it was captured with.
     Gradients held by a FlatGrads are read where it keeps them (a parameter counts as without a gradient until the backward pass has
     reached it); parameters of its device-decided groups are refused."""
 
@@ -354,6 +355,8 @@ class HipMuon:
             if not p.is_cuda or p.dtype != torch.float32 or not p.is_contiguous():
                 raise RuntimeError("HipMuon: parameters must be contiguous fp32 CUDA tensors")
             _matrices(p, "a parameter")
+        if len({id(p) for p in self.params}) != len(self.params):
+            raise ValueError("HipMuon: a parameter appears more than once")
         if not 0.0 <= momentum < 1.0:
             raise ValueError(f"HipMuon: 0 <= momentum < 1 (got {momentum})")
         if scale not in ("spectral", "rms"):
@@ -377,7 +380,9 @@ class HipMuon:
                 continue
             if getattr(p, "_ps_group", None) is not None:
                 raise RuntimeError("HipMuon: whether this parameter has a gradient is decided on the device; it belongs to HipAdam")
-            if g.dtype != torch.float32 or g.device != p.device or g.shape != p.shape:
+            if p.device != buf.device or not p.is_contiguous() or p.dtype != torch.float32 or p.shape != buf.shape:
+                raise RuntimeError("HipMuon: a parameter has changed its device, type, shape or layout since the optimizer was made")
+            if g.layout != torch.strided or g.dtype != torch.float32 or g.device != p.device or g.shape != p.shape:
                 raise RuntimeError("HipMuon: gradients must be dense fp32 tensors on their parameter's device")
             by_device.setdefault(p.device, []).append((p, g.contiguous(), buf))
         for device, stacks in by_device.items():

@@ -95,6 +95,17 @@ def test_library_refuses_bad_sizes():
         check(h.ps_expert_plan(None, 0, 8, 0, None, None, None, None, None), "ps_expert_plan")
 
 
+def test_plan_made_by_hand_is_checked():
+    i32 = lambda *shape: torch.zeros(*shape, dtype=torch.int32)  # noqa: E731
+    experts.ExpertPlan(i32(4), i32(8), i32(4, 2), 3)
+    for bad in ((i32(5), i32(8), i32(4, 2)), (i32(4), i32(7), i32(4, 2)), (i32(4), i32(8), i32(8))):
+        with pytest.raises(ValueError):
+            experts.ExpertPlan(*bad, 3)
+    for bad in ((i32(4).long(), i32(8), i32(4, 2)), (i32(4), i32(8), i32(2, 4).t()), (i32(8)[::2], i32(8), i32(4, 2))):
+        with pytest.raises(TypeError):
+            experts.ExpertPlan(*bad, 3)
+
+
 @pytest.mark.gpu
 def test_refusals(dev):
     ids = torch.zeros(6, 2, dtype=torch.int64, device=dev)
@@ -273,6 +284,41 @@ def test_places_behind_32_bits(dev):
     assert torch.equal(y, x)
 
 
+@pytest.mark.gpu
+def test_places_of_a_plan_made_by_hand_are_bounded(dev):
+    """places outside the sorted rows count as no expert"""
+    N, k = 50, 2
+    ids = some_ids(N, k, 4, 1, "dropped")
+    plan = experts.expert_plan(ids.to(dev), 4)
+    dst = plan.dst.clone()
+    dst[dst < 0] = N * k
+    dst[0, 0], dst[1, 1] = 2 ** 30, -(2 ** 30)  # (rows that nobody takes)
+    other = experts.ExpertPlan(plan.offsets, plan.src, dst, 4)
+    x, gates = torch.randn(N, 7, device=dev, requires_grad=True), torch.rand(N, k, device=dev, requires_grad=True)
+    rows = [experts.expert_dispatch(x, p) for p in (plan, other)]
+    y = [experts.expert_combine(r, gates, p) for r, p in zip(rows, (plan, other))]
+    assert torch.equal(rows[0], rows[1]) and torch.equal(y[0], y[1])
+    dy = torch.randn(N, 7, device=dev)
+    for a, b in zip(*[torch.autograd.grad(v, [x, gates], dy) for v in y]):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_more_lanes_than_a_launch_holds(dev):
+    """rows whose lanes number more than 2^32: every workgroup takes several; values are whole numbers, so all results are exact"""
+    N, D = (1 << 26) + 1000, 33
+    x = torch.randint(-128, 128, (N, D), device=dev, dtype=torch.int8).to(torch.bfloat16)
+    plan = experts.expert_plan((torch.arange(N, device=dev, dtype=torch.int32) % 7)[:, None], 7)
+    rows = experts.expert_dispatch(x, plan).requires_grad_(True)
+    w = torch.ones(N, 1, device=dev, requires_grad=True)
+    y = experts.expert_combine(rows, w, plan)
+    assert torch.equal(y, x)
+    drows, dw = torch.autograd.grad(y, [rows, w], x)
+    assert torch.equal(drows, rows)
+    for part in range(0, N, 1 << 22):
+        assert torch.equal(dw[part:part + (1 << 22), 0], x[part:part + (1 << 22)].float().square().sum(1))
+
+
 # ------------------------------------------------------------------------------------------------ the experts' linear layers
 def lengths(M, E, kind, seed):
     """offsets [E+1] of M rows"""
@@ -332,6 +378,45 @@ def check_linear(dev, M, E, n_in, n_out, dtype, kind, bias=True, seed=0):
                                                  (9, 4, 1030, 66, "even")])
 def test_linear_and_gradients(dev, M, E, n_in, n_out, kind, dtype):
     check_linear(dev, M, E, n_in, n_out, dtype, kind, bias=(M + E) % 2 == 0 or kind == "nobody")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,E,n_in,n_out,kind", [(40000, 8, 264, 300, "ragged"), (33000, 64, 301, 265, "ragged"), (6500, 64, 264, 300, "even"),
+                                                 (5000, 64, 201, 130, "ragged")])
+def test_linear_of_every_tile(dev, M, E, n_in, n_out, kind, dtype):
+    """sizes that take the largest tiles, whole weights' gradients and gradients in pieces, rows of whole 16 bytes and others"""
+    check_linear(dev, M, E, n_in, n_out, dtype, kind, bias=True)
+
+
+@pytest.mark.gpu
+def test_linear_of_rows_far_apart(dev):
+    """rows more than 2^20 elements apart are copied first"""
+    x = torch.zeros(5, (1 << 20) + 4, device=dev)
+    x[:, :40] = torch.randn(5, 40, generator=torch.Generator().manual_seed(1)).to(dev)
+    w = torch.randn(2, 24, 40, generator=torch.Generator().manual_seed(2)).to(dev).requires_grad_(True)
+    offsets = torch.tensor([0, 2, 5], device=dev)
+    results = []
+    for t in (x[:, :40], x[:, :40].contiguous()):
+        t.requires_grad_(True)
+        y = experts.expert_linear(t, w, None, offsets)
+        results.append((y,) + torch.autograd.grad(y, [t, w], x[:, 8:32]))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,E", [(300, 4), (3000, 64), (4000, 4), (2000, 100)])
+def test_linear_of_offsets_that_do_not_ascend(dev, M, E):
+    """ask for more tiles and pieces than the rows make: every access stays inside, what follows is right"""
+    x, w = torch.ones(M, 40, device=dev, requires_grad=True), torch.ones(E, 72, 40, device=dev, requires_grad=True)
+    for first, second in ((0, M), (M, 0), (M + 7, -9)):
+        offsets = torch.tensor([first, second] * E, dtype=torch.int32, device=dev)[: E + 1]
+        y = experts.expert_linear(x, w, None, offsets)
+        torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    offsets = torch.tensor([0] * E + [M], device=dev)
+    y = experts.expert_linear(x, w, None, offsets)
+    dx, dw = torch.autograd.grad(y, [x, w], torch.ones_like(y))
+    assert (y == 40).all() and (dx == 72).all() and (dw[-1] == M).all() and not dw[:-1].any()
 
 
 @pytest.mark.gpu

@@ -177,6 +177,20 @@ def test_a_large_matrix(dev):
     assert float((optim.newton_schulz(x).double() - ref).norm()) <= bound
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(12, 600, 700), (12, 701, 603), (3, 700, 1100), (40, 130, 65)])
+def test_every_tile(dev, shape, dtype):
+    """stacks that take the largest tiles and others, wide and tall, odd rows; against 64 bits on the GPU, matrix by matrix"""
+    x = (torch.randn(shape, generator=torch.Generator().manual_seed(14)) * 1e-2).to(TYPES[dtype]).to(dev)
+    y = optim.newton_schulz(x)
+    f = torch.finfo(y.dtype)
+    for got, g in zip(y, x):
+        ref, plain = iterate(g.double()), iterate(g.float())
+        rounding = 0.0 if dtype == "f32" else float(ref.norm()) * f.eps / 2
+        assert float((got.double() - ref).norm()) <= max(4 * float((plain.double() - ref).norm()), 16 * 2.0 ** -24 * float(ref.norm())) + rounding
+
+
 # ------------------------------------------------------------------------------------------------ the optimizer
 def muon_ref(p, g, buf, lr, mu, nesterov, wd, scale):
     buf = mu * buf + (1 - mu) * g
@@ -216,6 +230,44 @@ def test_muon_steps(dev, shapes, nesterov, scale):
         bound = 1e-4 * size[i] * 1.3 * math.sqrt(many * min(p.shape[-2:])) + 6 * 2.0 ** -24 * 2 * float(ref[i][0].norm())
         assert float((p.detach().cpu().double() - ref[i][0]).norm()) <= bound
         torch.testing.assert_close(buf.cpu().double(), ref[i][1], rtol=0, atol=8 * 2.0 ** -24 * float(ref[i][1].abs().max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(12, 600, 700), (12, 701, 603), (3, 704, 500), (2, 31, 33)])
+def test_muon_applies_the_orthogonalised_momentum(dev, shape):
+    """the first step's u is the same bits computed outside (two products and a sum, each rounded), so its orthogonalised form is too; the
+    parameter then carries two roundings of about its own size and one of the product's"""
+    g = torch.Generator().manual_seed(15)
+    p, grad = torch.randn(shape, generator=g).to(dev), torch.randn(shape, generator=g).to(dev)
+    q = torch.nn.Parameter(p.clone())
+    q.grad = grad
+    opt = optim.HipMuon([q], lr=0.05, momentum=0.9, weight_decay=0.2)
+    opt.step()
+    buf = (1.0 - 0.9) * grad
+    assert torch.equal(opt.momentum_buffers[0], buf)
+    y = optim.newton_schulz(0.9 * buf + (1.0 - 0.9) * grad).double()
+    rate = 0.05 * math.sqrt(max(1.0, shape[1] / shape[2]))
+    ref = (1 - 0.05 * 0.2) * p.double() - rate * y
+    bound = 3 * 2.0 ** -24 * (p.double().abs() + rate * y.abs()) + 2.0 ** -24 * (p.double().abs() + rate * y.abs())  # (and those of keep and rate)
+    assert ((q.detach().double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+def test_muon_refuses_parameters_twice_and_changed(dev):
+    p = torch.nn.Parameter(torch.randn(2, 40, 30, device=dev))
+    with pytest.raises(ValueError, match="more than once"):
+        optim.HipMuon([p, p])
+    opt = optim.HipMuon([p])
+    kept = p.detach().clone()
+    for data in (p.data.double(), p.data.transpose(1, 2), p.data[:1]):
+        q = p.data
+        p.data = data
+        p.grad = torch.ones_like(p)
+        with pytest.raises(RuntimeError):
+            opt.step()
+        p.grad = None
+        p.data = q
+    assert torch.equal(p, kept) and not opt.momentum_buffers[0].any()
 
 
 @pytest.mark.gpu
