@@ -282,6 +282,20 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
   for (int i = 0; i < MI; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = fine[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // what the result needs besides the sums is asked for before them (S of a small tile: there are registers for it)
+  const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+  const float start_ratio = w.ratio[batch];
+  constexpr bool kEarly = WHAT == kPoly && BM == 64;
+  Pack<_Float16, 4> early[2][kEarly ? MI : 1][kEarly ? NJ : 1];
+  auto gram_at = [&](int i, int j, int plane) {  // (rows are padded to 64: whole packs)
+    const int m = wm + i * 16 + r, n = wn + j * 16 + g * 4;
+    return m < rows && n < cols ? load_pack<_Float16, 4>(w.gram + (batch * h.s + m0 + m) * 2 * h.sp + pair_at(n0 + n, plane)) : Pack<_Float16, 4>{};
+  };
+  if constexpr (kEarly)
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) early[0][i][j] = gram_at(i, j, 0), early[1][i][j] = gram_at(i, j, 1);
   const int steps = o.k / kPairK;  // (even)
 #pragma unroll
   for (int i = 0; i < kStages - kGroup; ++i) load(i);
@@ -315,7 +329,7 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
     }
   }
   __syncthreads();
-  const float ratio = ratio_at(w.ratio[batch], step, c.grow);
+  const float ratio = ratio_at(start_ratio, step, c.grow);
   // kPoly: a + b r^2 S^ + c r^4 S^ S^ with the coefficients as pairs of floats: an error of a coefficient would be common to all entries and
   // grow like a singular value's | kApply: over the step's growth of r | kLast: X = r X^
   const double r2 = (double)ratio * ratio, cb = c.b * r2 / kPlaneScale, cc = c.c * r2 * r2 * kProductScale;
@@ -323,7 +337,6 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
   const float ca_hi = (float)c.a, ca_lo = (float)(c.a - ca_hi);
   const float out_scale = WHAT == kApply ? kProductScale * (ratio > 0.0f ? ratio / ratio_at(ratio, 1, c.grow) : 1.0f)
                                          : (WHAT == kLast ? kProductScale * ratio : kProductScale);
-  const int r = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
   if constexpr (WHAT == kLast) {
     const int image = (h.tall ? BM : BN) * 4;  // bytes of a row of G's direction
 #pragma unroll
@@ -388,11 +401,10 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
         for (int j = 0; j < NJ; ++j) {
           const int m = wm + i * 16 + r, n = wn + j * 16 + g * 4;
           Pack<_Float16, 4> hi, lo, gh{}, gl{};
-          if (WHAT == kPoly && m < rows && n < cols) {  // (rows are padded to 64: whole packs)
-            const _Float16* was = w.gram + (batch * h.s + m0 + m) * 2 * ld;
-            gh = load_pack<_Float16, 4>(was + pair_at(n0 + n, 0));
-            gl = load_pack<_Float16, 4>(was + pair_at(n0 + n, 1));
-          }
+          if constexpr (kEarly)
+            gh = early[0][i][j], gl = early[1][i][j];
+          else if constexpr (WHAT == kPoly)
+            gh = gram_at(i, j, 0), gl = gram_at(i, j, 1);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const float sum = acc[i][j][q] + fine[i][j][q];
