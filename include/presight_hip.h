@@ -623,7 +623,9 @@ int ps_finish_losses(const float* const* terms, const int64_t* n, const float* d
 
 /* ---- experts: rows sorted by expert and back, and the experts' linear layers on the sorted rows --------------------------------
  * dtype of rows, weights and their gradients: 0 fp32, 1 fp16, 2 bf16; sums in fp32, one rounding.  k experts per row, E experts,
- * M = N*k assignments f = n*k + j.  Strides are in elements between rows; the elements of a row are consecutive.
+ * M = N*k assignments f = n*k + j.  Strides are in elements between rows; the elements of a row are consecutive.  dst outside [0, M) is
+ * nobody's.  The linear layers take rows up to 2^20 elements long and apart, and offsets that ascend (others: undefined rows, no access
+ * outside the operands).
  *   ps_expert_plan          ids [N,k] int32, or int64 (ids_are_64); an id outside [0, E) assigns to nobody.  offsets [E+1]: expert e's
  *                           rows are the sorted places offsets[e] .. offsets[e+1]; src [M]: place -> assignment, by (expert, f), -1
  *                           behind offsets[E]; dst [M]: assignment -> place or -1.  workspace: ps_expert_plan_workspace ints.  E <= 1024

@@ -31,5 +31,16 @@ template <typename T, int VEC>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) {
   *reinterpret_cast<Pack<T, VEC>*>(p) = v;
 }
+// ... at any element's address (one access all the same: the memory takes 16 bytes at any address, and splits what crosses a line)
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_any(const T* p) {
+  Pack<T, VEC> v;
+  __builtin_memcpy(&v, p, sizeof v);
+  return v;
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_any(T* p, const Pack<T, VEC>& v) {
+  __builtin_memcpy(p, &v, sizeof v);
+}
 
 }  // namespace ps

@@ -6,7 +6,10 @@
 //     dispatch   rows[dst[n,j]] = x[n]                              gradient   dx[n] = sum_j drows[dst[n,j]]      (= combine, w = 1)
 //     combine    y[n] = sum_j w[n,j] * rows[dst[n,j]]               gradient   drows[dst[n,j]] = w[n,j] * dy[n],  dw[n,j] = <dy[n], rows[dst[n,j]]>
 // All four run over n: x / dy / y are streamed once in order, the k sorted rows are touched as whole rows.  Nothing is computed that
-// is not moved, so all of them are bound by HBM.
+// is not moved, so all of them are bound by HBM.  16384 rows to 8 of 128 experts each, 2048 bf16 features (a large copy reaches 4.9 TB/s):
+//     dispatch 604 MB 127 us, 4.8 TB/s | combine 604 MB 180 us, 3.4 TB/s (mostly reads; rows fetched four or eight ahead were no faster) |
+//     combine's gradients 1141 MB 243 us, 4.7 TB/s | the plan of 131072 assignments 14 us
+// 65536 rows to 2 of 16, 64 fp32 features: 10 us and less for 50 MB, 17 us for 84; one row: 2 us each and 4 for its plan, all latency.
 #include "common.hpp"
 #include "expert_types.hpp"
 
@@ -48,6 +51,8 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const void* __
   for (int e = threadIdx.x; e < E; e += kPlanThreads) hist[(int64_t)blockIdx.x * E + e] = cnt[e];
 }
 
+// 131072 assignments: 4 us to count and 9 to place them, neither near a limit of the memory: a workgroup's two passes over its ids, the
+// second one's ranks, and the scans between them wait for each other.
 // One workgroup places the assignments [f0, f0 + chunk).  Each wave owns a contiguous run of them and counts it by itself (cnt[wave][e],
 // ballots instead of atomics: the rank inside a 64-wide round is a popcount), the counts become first places by a scan over waves, the
 // workgroups before this one (hist) and the experts, and a second pass over the same ids hands the places out in order.
@@ -135,8 +140,11 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place_kernel(const void* __
 }
 
 // ------------------------------------------------------------------------------------------------ rows
-// G lanes work on one row in steps of VEC elements (16 bytes where the row length, the strides and the addresses allow it): a 256-byte
-// row keeps 16 lanes busy, so 4 rows share a wave; long rows take a whole wave.
+// G lanes work on one row in steps of VEC elements (16 bytes, of rows that have them): a 256-byte row keeps 16 lanes busy, so 4 rows share a
+// wave; long rows take a whole wave.  Rows may start at any element; the last step of one that is no whole number of them starts early,
+// over elements that come out the same twice.  (10007 rows to 3 of 37, 195 fp16, with gradients: 28 us; 64 element by element.)
+__device__ __forceinline__ int step_at(int c, int D, int vec) { return c + vec <= D ? c : D - vec; }
+
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void dispatch_kernel(const T* __restrict__ x, int64_t x_stride, const int* __restrict__ dst,
                                                        const int* __restrict__ held, int64_t N, int k, int D, int G, T* __restrict__ rows) {
@@ -144,17 +152,18 @@ __global__ __launch_bounds__(256) void dispatch_kernel(const T* __restrict__ x, 
   const int64_t places = N * k, total = *held;
   for (int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G; n < N; n += (int64_t)gridDim.x * 256 / G) {
     const int* d = dst + n * k;
-    for (int c = l * VEC; c < D; c += G * VEC) {
-      const Pack<T, VEC> v = load_pack<T, VEC>(x + n * x_stride + c);
+    for (int u = l * VEC; u < D; u += G * VEC) {
+      const int c = step_at(u, D, VEC);
+      const Pack<T, VEC> v = load_any<T, VEC>(x + n * x_stride + c);
       for (int j = 0; j < k; ++j) {
         const int p = d[j];
-        if (p >= 0 && p < places) store_pack(rows + (int64_t)p * D + c, v);
+        if (p >= 0 && p < places) store_any(rows + (int64_t)p * D + c, v);
       }
     }
     for (int j = 0; j < k; ++j) {  // the places behind the last expert's rows are shared out over the same lanes
       const int64_t p = n * k + j;
       if (p >= total)
-        for (int c = l * VEC; c < D; c += G * VEC) store_pack(rows + p * D + c, Pack<T, VEC>{});
+        for (int u = l * VEC; u < D; u += G * VEC) store_any(rows + p * D + step_at(u, D, VEC), Pack<T, VEC>{});
     }
   }
 }
@@ -168,12 +177,13 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ rows
   const int64_t places = N * k;
   for (int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) / G; n < N; n += (int64_t)gridDim.x * 256 / G) {
     const int* d = dst + n * k;
-    for (int c = l * VEC; c < D; c += G * VEC) {
+    for (int u = l * VEC; u < D; u += G * VEC) {
+      const int c = step_at(u, D, VEC);
       float acc[VEC] = {};
       for (int j = 0; j < k; ++j) {
         const int p = d[j];
         if (p < 0 || p >= places) continue;
-        const Pack<T, VEC> v = load_pack<T, VEC>(rows + p * r_stride + c);
+        const Pack<T, VEC> v = load_any<T, VEC>(rows + p * r_stride + c);
         const float wj = w != nullptr ? w[n * k + j] : 1.0f;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[i] = fmaf(wj, to_f32(v.v[i]), acc[i]);
@@ -181,7 +191,7 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ rows
       Pack<T, VEC> o;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(acc[i]);
-      store_pack(y + n * D + c, o);
+      store_any(y + n * D + c, o);
     }
   }
 }
@@ -199,18 +209,22 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(const T* __restrict__ 
       float dot = 0.0f;
       if (p >= 0 && p < places) {
         const float wj = w[n * k + j];
-        for (int c = l * VEC; c < D; c += G * VEC) {
-          const Pack<T, VEC> g = load_pack<T, VEC>(dy + n * dy_stride + c);
+        for (int u = l * VEC; u < D; u += G * VEC) {
+          const int c = step_at(u, D, VEC);
+          const Pack<T, VEC> g = load_any<T, VEC>(dy + n * dy_stride + c);
           if (dw != nullptr) {
-            const Pack<T, VEC> r = load_pack<T, VEC>(rows + p * r_stride + c);
+            const Pack<T, VEC> r = load_any<T, VEC>(rows + p * r_stride + c);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) dot = fmaf(to_f32(g.v[i]), to_f32(r.v[i]), dot);
+            for (int i = 0; i < VEC; ++i) {
+              const float sum = fmaf(to_f32(g.v[i]), to_f32(r.v[i]), dot);
+              dot = c + i >= u ? sum : dot;  // (once each)
+            }
           }
           if (drows != nullptr) {
             Pack<T, VEC> o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) o.v[i] = from_f32<T>(wj * to_f32(g.v[i]));
-            store_pack(drows + (int64_t)p * D + c, o);
+            store_any(drows + (int64_t)p * D + c, o);
           }
         }
       }
@@ -220,20 +234,15 @@ __global__ __launch_bounds__(256) void combine_bwd_kernel(const T* __restrict__ 
       }
       const int64_t q = n * k + j;
       if (drows != nullptr && q >= total)
-        for (int c = l * VEC; c < D; c += G * VEC) store_pack(drows + q * D + c, Pack<T, VEC>{});
+        for (int u = l * VEC; u < D; u += G * VEC) store_any(drows + q * D + step_at(u, D, VEC), Pack<T, VEC>{});
     }
   }
 }
 
-// elements a lane moves at a time: the largest power of two that divides the row length and every stride and keeps every address
-// aligned, up to 16 bytes
-int vec_elems(int size, int64_t D, std::initializer_list<int64_t> strides, std::initializer_list<const void*> ptrs) {
-  int64_t bits = D;
-  for (int64_t s : strides) bits |= s;
-  uintptr_t addr = 0;
-  for (const void* p : ptrs) addr |= (uintptr_t)p;
+// elements a lane moves at a time: 16 bytes, fewer where a row has not got them
+int vec_elems(int size, int64_t D) {
   int v = 16 / size;
-  while (v > 1 && ((bits & (v - 1)) != 0 || (addr & (uintptr_t)(v * size - 1)) != 0)) v >>= 1;
+  while (v > 1 && v > D) v >>= 1;
   return v;
 }
 
@@ -302,7 +311,7 @@ extern "C" int ps_expert_dispatch(const void* x, int64_t x_stride, const int32_t
   PS_REQUIRE(x != nullptr && dst != nullptr && held != nullptr && rows != nullptr, "ps_expert_dispatch: null argument");
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vec = vec_elems(sizeof(T), D, {x_stride}, {x, rows}), G = lanes_per_row(D, vec);
+    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec);
     const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (dispatch_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)x, x_stride, dst, held, N, k, (int)D, G, (T*)rows)));
     PS_CHECK_LAUNCH();
@@ -316,7 +325,7 @@ extern "C" int ps_expert_combine(const void* rows, int64_t rows_stride, const fl
   PS_REQUIRE(rows != nullptr && dst != nullptr && y != nullptr, "ps_expert_combine: null argument");
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vec = vec_elems(sizeof(T), D, {rows_stride}, {rows, y}), G = lanes_per_row(D, vec);
+    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec);
     const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (combine_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)rows, rows_stride, weights, dst, N, k, (int)D, G, (T*)y)));
     PS_CHECK_LAUNCH();
@@ -331,7 +340,7 @@ extern "C" int ps_expert_combine_bwd(const void* dy, int64_t dy_stride, const vo
   PS_REQUIRE(weights != nullptr && dst != nullptr && held != nullptr && (D == 0 || (dy != nullptr && rows != nullptr)), "ps_expert_combine_bwd: null argument");
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vec = vec_elems(sizeof(T), D, {dy_stride, rows_stride}, {dy, rows, drows}), G = lanes_per_row(D, vec);
+    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec);
     const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (combine_bwd_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)dy, dy_stride, (const T*)rows, rows_stride, weights,
                                                                                            dst, held, N, k, (int)D, G, (T*)drows, dw)));

@@ -5,7 +5,7 @@
 // Arithmetic.  The polynomial multiplies what rounding leaves in the small singular directions by up to a^steps, so one 16-bit rounding
 // per step is not enough for an fp32 result.  Every matrix is kept as a PAIR of fp16 planes, value = (hi + lo) / 1024: 22 bits and the
 // sign, and a product is three matrix instructions, hi hi + hi lo + lo hi, summed in fp32 (lo lo, 2^-24 of the product, is left out).
-// That is fp32's own precision at a third of the fp16 rate, five times the fp32 matrix rate.
+// That is fp32's own precision at a third of the fp16 rate, three times the fp32 matrix rate (large products: 1463 and 154 TFLOP/s).
 //
 // Range.  The planes hold X^ = X / r with r = norm / (norm + eps) at the start, so an input far below eps loses nothing; a step
 // multiplies r by the power of two `grow` that bounds a + b t + c t^2, until r passes 1/2, and keeps it from then on.  The caller
@@ -103,33 +103,36 @@ __device__ __forceinline__ float source_value(const Source& src, int64_t i) {
   if constexpr (MOMENTUM && UPDATE) src.buf[i] = b;
   return v;
 }
-// V consecutive values (V > 1: aligned to their size)
-template <typename T, bool MOMENTUM, bool UPDATE, int V>
-__device__ __forceinline__ void source_pack(const Source& src, int64_t i, float (&v)[V]) {
-  const Pack<T, V> g = load_pack<T, V>(reinterpret_cast<const T*>(src.g) + i);
-  Pack<float, V> b{};
-  if constexpr (MOMENTUM) b = load_pack<float, V>(src.buf + i);
+// four consecutive values, zeros from the `left`th on
+template <typename T, bool MOMENTUM, bool UPDATE>
+__device__ __forceinline__ void source_pack(const Source& src, int64_t i, int64_t left, float (&v)[4]) {
+  if (left < 4) {
 #pragma unroll
-  for (int k = 0; k < V; ++k) v[k] = source_step<MOMENTUM, UPDATE>(src, to_f32(g.v[k]), b.v[k]);
-  if constexpr (MOMENTUM && UPDATE) store_pack(src.buf + i, b);
+    for (int k = 0; k < 4; ++k) v[k] = k < left ? source_value<T, MOMENTUM, UPDATE>(src, i + k) : 0.0f;
+    return;
+  }
+  const Pack<T, 4> g = load_any<T, 4>(reinterpret_cast<const T*>(src.g) + i);
+  Pack<float, 4> b{};
+  if constexpr (MOMENTUM) b = load_any<float, 4>(src.buf + i);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = source_step<MOMENTUM, UPDATE>(src, to_f32(g.v[k]), b.v[k]);
+  if constexpr (MOMENTUM && UPDATE) store_any(src.buf + i, b);
 }
 
-// partial sums of squares, in 64 bits: entries of any fp32 size neither overflow nor vanish.  V elements at a time (V = 4: every matrix
-// starts and ends on a pack).
-template <typename T, bool MOMENTUM, int V>
+// 2048 x 4096 fp32: 11 us for 34 MB; with the momentum, 8 x 1024 x 2048: 35 us for 201 MB (5.7 TB/s, some of it from the last-level cache).
+// partial sums of squares, in 64 bits: entries of any fp32 size neither overflow nor vanish
+template <typename T, bool MOMENTUM>
 __global__ __launch_bounds__(256) void ns_norm_kernel(Source src, int64_t size, Work w) {
   __shared__ double part[4];
   const int64_t base = (int64_t)blockIdx.y * size;
-  double sum[V] = {};
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; i < size; i += (int64_t)gridDim.x * 256 * V) {
-    float v[V];
-    source_pack<T, MOMENTUM, true, V>(src, base + i, v);
+  double sum[4] = {};
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < size; i += (int64_t)gridDim.x * 256 * 4) {
+    float v[4];
+    source_pack<T, MOMENTUM, true>(src, base + i, size - i, v);
 #pragma unroll
-    for (int k = 0; k < V; ++k) sum[k] += (double)v[k] * v[k];
+    for (int k = 0; k < 4; ++k) sum[k] += (double)v[k] * v[k];
   }
-  double all = 0.0;
-#pragma unroll
-  for (int k = 0; k < V; ++k) all += sum[k];
+  double all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = all;
   __syncthreads();
@@ -148,9 +151,9 @@ __device__ __forceinline__ float ratio_at(float r, int i, float grow) {
   return r;
 }
 
-// X^ = G / norm as planes [s][lp], 64 x 64 elements at a time (turned in LDS where G is tall); zeros in the padding.  V as above, of the
-// rows as given.
-template <typename T, bool MOMENTUM, int V>
+// 2048 x 4096 fp32: 25 us for 67 MB; 8 x 1024 x 2048 with the momentum: 45 us for 201 MB.
+// X^ = G / norm as pairs [s][2 lp], 64 x 64 elements at a time (turned in LDS where G is tall); zeros in the padding
+template <typename T, bool MOMENTUM>
 __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work w, float eps) {
   __shared__ _Float16 tile[2][64][72];  // (rows of 144 bytes: 16-byte chunks, 36 banks apart)
   __shared__ double inv_of;
@@ -169,12 +172,13 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work
   const double inv = inv_of;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;  // of G
   const int64_t base = b * h.m * h.n;
-  for (int id = threadIdx.x; id < 64 * 64 / V; id += 256) {
-    const int r = id / (64 / V), c = id % (64 / V) * V;
-    float v[V] = {};
-    if (r0 + r < h.m && c0 + c < h.n) source_pack<T, MOMENTUM, false, V>(src, base + (int64_t)(r0 + r) * h.n + c0 + c, v);
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
+  for (int id = threadIdx.x; id < 64 * 64 / 4; id += 256) {
+    const int r = id / 16, c = id % 16 * 4;
+    float v[4] = {};
+    if (r0 + r < h.m && c0 + c < h.n) source_pack<T, MOMENTUM, false>(src, base + (int64_t)(r0 + r) * h.n + c0 + c, h.n - (c0 + c), v);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
       const int row = h.tall ? c + k : r, col = h.tall ? r : c + k;
       split(v[k] * inv, tile[0][row][col], tile[1][row][col]);
     }
@@ -220,6 +224,10 @@ struct Operands {  // pairs
 // 8 x 1024 x 2048: 150 -> 122), else 64 x 64 while no compute unit gets more than the two that fit its LDS (all five steps: 3 x 385 x 129
 // 229 -> 132 us, 1024 x 1024 479 -> 273, 1536 x 1536 671 -> 517; with more of them 2048 x 4096 would go from 1236 to 1317), else 128 x 128.
 // The two small products add up apart from the large one: each of their additions to it would cost it another rounding.
+//
+// 2048 x 4096: S 90 us, a I + b S + c S S 56, times X 115: 573, 464 and 897 TFLOP/s of pairs' products (half of S and S S by symmetry, three
+// products per pair), where a large fp16 product reaches 1463; 8 x 1024 x 2048: 87, 62 and 122 us.  A few tiles:
+// 3 x 385 x 129 takes 7 to 9 us a product, most of it the launch, the first loads from memory that another XCD wrote, and the way out.
 //
 // The result leaves through LDS as rows of whole lines.  Of a symmetric one only what lies on and below the diagonal's BN x BN blocks is
 // computed and written, and then written turned.
@@ -355,20 +363,19 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
     __syncthreads();
     const int r0 = h.tall ? n0 : m0, c0 = h.tall ? m0 : n0, rn = h.tall ? cols : rows, cn = h.tall ? rows : cols;
     const int64_t base = batch * h.m * h.n + (int64_t)r0 * h.n + c0;
-    // four at a time where rows and addresses allow it
-    const bool packed = h.n % 4 == 0 && ((uintptr_t)res.out & (4 * sizeof(T) - 1)) == 0;
     for (int id = threadIdx.x; id < BM * BN / 4; id += NT) {
       const int row = id / (image / 16), col = id % (image / 16) * 4;
       if (row >= rn || col >= cn) continue;
       const f32x4 v = *reinterpret_cast<const f32x4*>(lds + out_addr(row, image, col * 4));
       const int64_t at = base + (int64_t)row * h.n + col;
+      const bool whole = col + 4 <= cn;
       if (res.update) {
         float* p = reinterpret_cast<float*>(res.out) + at;
-        if (packed) {
-          f32x4 old = *reinterpret_cast<f32x4*>(p);
+        if (whole) {
+          Pack<float, 4> old = load_any<float, 4>(p);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) old[q] = res.keep * old[q] - res.rate * v[q];
-          *reinterpret_cast<f32x4*>(p) = old;
+          for (int q = 0; q < 4; ++q) old.v[q] = res.keep * old.v[q] - res.rate * v[q];
+          store_any(p, old);
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -376,11 +383,11 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
         }
       } else {
         T* p = reinterpret_cast<T*>(res.out) + at;
-        if (packed) {
+        if (whole) {
           Pack<T, 4> out;
 #pragma unroll
           for (int q = 0; q < 4; ++q) out.v[q] = from_f32<T>(v[q]);
-          store_pack(p, out);
+          store_any(p, out);
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
@@ -473,6 +480,8 @@ void launch_product(const Operands& o, const Shape& h, const Work& w, int64_t B,
 // products on the fp32 matrix instructions, which at these sizes wait for the LDS rather than for each other, and ONE launch for every
 // small matrix of a whole list of stacks, where the planes' path needs three launches a step.  Eight waves: a wave takes two of the (up to)
 // 16 blocks of S and of P, and half the rows of a 16-column block of X.
+// 80 matrices of 64 x 64 and smaller in five stacks, momentum and parameters included: 36 us, five steps of three products each behind the
+// one before it in the same LDS.
 // LDS rows are 64 i + 4 floats apart: 16 rows x 4 k (chunk reads of A and B) and 4 k x 16 columns (the reads of X as B) both meet all 64
 // banks once.
 constexpr int kSmallSide = 64;
@@ -638,13 +647,8 @@ int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Pol
   const Work w = work_of(h, B, workspace);
   const dim3 norm_grid((unsigned)w.parts, (unsigned)B);
   const dim3 start_grid((unsigned)((h.tall ? h.sp : h.lp) / 64), (unsigned)((h.tall ? h.lp : h.sp) / 64), (unsigned)B);
-  if (n % 4 == 0 && ((uintptr_t)src.g & (4 * sizeof(T) - 1)) == 0 && ((uintptr_t)src.buf & 15) == 0) {
-    ns_norm_kernel<T, MOMENTUM, 4><<<norm_grid, 256, 0, s>>>(src, m * n, w);
-    ns_start_kernel<T, MOMENTUM, 4><<<start_grid, 256, 0, s>>>(src, h, w, eps);
-  } else {
-    ns_norm_kernel<T, MOMENTUM, 1><<<norm_grid, 256, 0, s>>>(src, m * n, w);
-    ns_start_kernel<T, MOMENTUM, 1><<<start_grid, 256, 0, s>>>(src, h, w, eps);
-  }
+  ns_norm_kernel<T, MOMENTUM><<<norm_grid, 256, 0, s>>>(src, m * n, w);
+  ns_start_kernel<T, MOMENTUM><<<start_grid, 256, 0, s>>>(src, h, w, eps);
   for (int i = 0; i < steps; ++i) {
     const _Float16* x = w.x[i & 1];
     launch_product<T, kGram>({x, x, h.s, h.s, h.lp, 0, 0}, h, w, B, i, c, res, s);
