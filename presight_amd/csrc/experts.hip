@@ -246,10 +246,12 @@ int vec_elems(int size, int64_t D) {
   return v;
 }
 
-int lanes_per_row(int64_t D, int vec) {
+// most: 64 where a row's lanes add up (one wave), else a workgroup: a row of 4 KiB is fetched whole rather than in four visits (combine,
+// 16384 rows of 8 x 2048 bf16: 156 -> 127 us)
+int lanes_per_row(int64_t D, int vec, int most) {
   const int64_t units = (D + vec - 1) / vec;
   int g = 1;
-  while (g < 64 && g < units) g <<= 1;
+  while (g < most && g < units) g <<= 1;
   return g;
 }
 
@@ -311,7 +313,7 @@ extern "C" int ps_expert_dispatch(const void* x, int64_t x_stride, const int32_t
   PS_REQUIRE(x != nullptr && dst != nullptr && held != nullptr && rows != nullptr, "ps_expert_dispatch: null argument");
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec);
+    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec, 256);
     const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (dispatch_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)x, x_stride, dst, held, N, k, (int)D, G, (T*)rows)));
     PS_CHECK_LAUNCH();
@@ -325,7 +327,7 @@ extern "C" int ps_expert_combine(const void* rows, int64_t rows_stride, const fl
   PS_REQUIRE(rows != nullptr && dst != nullptr && y != nullptr, "ps_expert_combine: null argument");
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec);
+    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec, 256);
     const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (combine_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)rows, rows_stride, weights, dst, N, k, (int)D, G, (T*)y)));
     PS_CHECK_LAUNCH();
@@ -340,7 +342,7 @@ extern "C" int ps_expert_combine_bwd(const void* dy, int64_t dy_stride, const vo
   PS_REQUIRE(weights != nullptr && dst != nullptr && held != nullptr && (D == 0 || (dy != nullptr && rows != nullptr)), "ps_expert_combine_bwd: null argument");
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec);
+    const int vec = vec_elems(sizeof(T), D), G = lanes_per_row(D, vec, 64);
     const unsigned blocks = blocks_of_256(N * G);
     PS_BY_VEC(T, vec, (combine_bwd_kernel<T, VEC><<<blocks, 256, 0, (hipStream_t)stream>>>((const T*)dy, dy_stride, (const T*)rows, rows_stride, weights,
                                                                                            dst, held, N, k, (int)D, G, (T*)drows, dw)));
