@@ -7,8 +7,9 @@
 //     combine    y[n] = sum_j w[n,j] * rows[dst[n,j]]               gradient   drows[dst[n,j]] = w[n,j] * dy[n],  dw[n,j] = <dy[n], rows[dst[n,j]]>
 // All four run over n: x / dy / y are streamed once in order, the k sorted rows are touched as whole rows.  Nothing is computed that
 // is not moved, so all of them are bound by HBM.  16384 rows to 8 of 128 experts each, 2048 bf16 features (a large copy reaches 4.9 TB/s):
-//     dispatch 604 MB 127 us, 4.8 TB/s | combine 604 MB 180 us, 3.4 TB/s (mostly reads; rows fetched four or eight ahead were no faster) |
-//     combine's gradients 1141 MB 243 us, 4.7 TB/s | the plan of 131072 assignments 14 us
+//     dispatch 604 MB 119 us, 5.1 TB/s | combine 604 MB 127 us, 4.7 TB/s | combine's gradients 1141 MB 245 us, 4.7 TB/s |
+//     the plan of 131072 assignments 14 us
+// One row after the other, each fetched whole, is best: four or eight rows of an assignment's at once were a tenth to a half slower.
 // 65536 rows to 2 of 16, 64 fp32 features: 10 us and less for 50 MB, 17 us for 84; one row: 2 us each and 4 for its plan, all latency.
 #include "common.hpp"
 #include "expert_types.hpp"
@@ -196,7 +197,8 @@ __global__ __launch_bounds__(256) void combine_kernel(const T* __restrict__ rows
   }
 }
 
-// both gradients of combine in one pass over the sorted rows; drows / dw may be null (not asked for)
+// both gradients of combine in one pass over the sorted rows; drows / dw may be null (not asked for).  (More than a wave on one row, its
+// products joined in LDS: 260 us for 245.)
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void combine_bwd_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ rows, int64_t r_stride,
                                                           const float* __restrict__ w, const int* __restrict__ dst, const int* __restrict__ held,
