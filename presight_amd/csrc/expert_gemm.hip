@@ -365,11 +365,13 @@ bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
 constexpr int kCompute = 256;  // compute units
 
 // Tile sizes, by work per tile.  256 x 256 reads each operand byte half as often as 128 x 128, but one tile fills a compute unit: it is taken
-// where it wastes little of itself and there is a tile for every compute unit.  Narrow outputs and few rows per expert take the smaller ones.
+// where it wastes little of itself and there is a tile for every compute unit (bf16: 65536 rows, 32 experts of 2048 x 1024 316 us, with 128
+// 375; 16384, 8 of 1024 x 1024 35 and 42).  Narrow outputs and few rows per expert take the smaller ones (128 rows each, 64 experts of 1024 x
+// 1024: tiles of 128 28 us, of 64 32; 64 rows each, 512 x 512: 11.2 and 9.4).
 int linear_tile(int64_t rows, int64_t groups, int64_t cols) {
   const int64_t each = rows / groups;
   if (cols > 128 && each >= 192 && (rows / 256 + groups) * ((cols + 255) / 256) >= kCompute) return 256;
-  return cols > 64 && each >= 64 ? 128 : 64;
+  return cols > 64 && each >= 96 ? 128 : 64;
 }
 
 template <typename K>
@@ -441,27 +443,44 @@ struct DwPlan {
   int tile, piece;
   int64_t units;
 };
-DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out) {
-  DwPlan p;
-  const int64_t least = n_in < n_out ? n_in : n_out;
-  auto tiles = [&](int64_t b) { return ((n_in + b - 1) / b) * ((n_out + b - 1) / b) * E; };
-  p.tile = least > 128 && tiles(256) >= kCompute ? 256 : (least > 64 && tiles(128) >= kCompute ? 128 : 64);
-  if (p.tile == 64 && least > 64) p.tile = 128;
-  p.piece = 0;
-  p.units = E;
-  const int64_t each = M / E, t = tiles(p.tile);
-  if (t < 2 * kCompute && each >= 512) {  // pieces for about four workgroups per compute unit, of at least 256 rows
-    const int64_t want = (4 * kCompute + t - 1) / t;
-    int64_t piece = ((each + want - 1) / want + 63) & ~(int64_t)63;
-    p.piece = (int)(piece < 256 ? 256 : piece);
-    p.units = row_tiles_at_most(M, E, p.piece);
+// The cheapest by what was measured: a step of k (128 bytes of it) of a 64, 128 or 256 tile takes its compute unit .27, .73 or 2.1 us in 16 bits,
+// of a 64 or 128 tile .44 or 1.75 in fp32 (bound by the matrix instructions: a larger one gains nothing), and no less than .45, .8 or 2.1
+// (.8 or 1.75) from its start to its end.  Pieces shorten the longest run of
+// steps and cost 5 us and the way of their fp32 sums through the memory, 4.5 TB/s; without them an expert may well have twice its
+// share of the rows.
+//     16 experts, fp32:  131072 rows of 64 x 64 in pieces 22 us, whole 191 | 32768 rows of 128 x 128 in pieces, tiles of 64 21, of 128 30
+//     bf16:  8192 rows, 16 experts of 512 x 512 whole 12, in pieces 45 | 65536 rows, 32 experts of 2048 x 1024 tiles of 256 307, of 128 374
+DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
+  const bool wide = dtype == kF32;
+  const double busy_us[3] = {wide ? 0.44 : 0.27, wide ? 1.75 : 0.73, 2.1}, least_us[3] = {wide ? 0.8 : 0.45, wide ? 1.75 : 0.8, 2.1};
+  const int64_t least = n_in < n_out ? n_in : n_out, step_rows = wide ? 32 : 64, each = M / E;
+  DwPlan best{64, 0, E};
+  double best_us = 1e30;
+  for (int i = 0; i < (wide ? 2 : 3); ++i) {
+    const int tile = 64 << i;
+    if (i > 0 && least <= tile / 2) break;
+    const double tiles = (double)((n_in + tile - 1) / tile) * ((n_out + tile - 1) / tile);
+    for (int64_t pieces = 1; pieces == 1 || each / pieces >= 192; pieces *= 2) {
+      DwPlan p{tile, 0, E};
+      int64_t rows = each, longest = E > 1 ? 2 * each : each;
+      if (pieces > 1) {
+        rows = ((each + pieces - 1) / pieces + 63) & ~(int64_t)63;
+        longest = rows = rows < 256 ? 256 : rows;
+        p.piece = (int)rows;
+        p.units = row_tiles_at_most(M, E, p.piece);
+      }
+      const double shared = tiles * (pieces > 1 ? (double)M / rows + 0.5 * E : (double)E) / kCompute;  // workgroups per compute unit
+      const double steps = (double)((rows + step_rows - 1) / step_rows), all = busy_us[i] * (shared > 1 ? shared : 1) * (steps > 1 ? steps : 1);
+      const double run = least_us[i] * (double)((longest + step_rows - 1) / step_rows);
+      const double us = (all > run ? all : run) + (pieces > 1 ? 5.0 + 8e-6 / 4.5 * p.units * n_in * n_out : 0.0);
+      if (us < best_us) best = p, best_us = us;
+    }
   }
-  return p;
+  return best;
 }
 
 int64_t round4(int64_t v) { return (v + 3) / 4 * 4; }
-int64_t dw_part_bytes(int64_t M, int E, int64_t n_in, int64_t n_out) {
-  const DwPlan p = dw_plan(M, E, n_in, n_out);
+int64_t dw_part_bytes(const DwPlan& p, int64_t n_in, int64_t n_out) {
   return p.piece == 0 ? 0 : (p.units * (n_out * round4(n_in) + round4(n_out)) * (int64_t)sizeof(float) + 255) & ~(int64_t)255;
 }
 
@@ -480,7 +499,8 @@ int launch_dw_tile(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t
 template <typename T, bool SPLIT>
 int launch_dw(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t* offsets, int64_t M, int E, int N, int K, int ldo, void* dw, void* db,
               hipStream_t s) {
-  if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
+  if constexpr (sizeof(T) == 2)
+    if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
   if (p.tile == 128) return launch_dw_tile<T, 128, 2, 2, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
   return launch_dw_tile<T, 64, 2, 2, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
 }
@@ -489,7 +509,7 @@ enum Pass { kForward, kInputGradient, kWeightGradient };
 
 int64_t workspace_of(int pass, const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
   if (pass == kWeightGradient)
-    return dw_part_bytes(M, E, n_in, n_out) + pack_bytes(a, a_stride, M, n_out, dtype) + pack_bytes(b, b_stride, M, n_in, dtype);
+    return dw_part_bytes(dw_plan(M, E, n_in, n_out, dtype), n_in, n_out) + pack_bytes(a, a_stride, M, n_out, dtype) + pack_bytes(b, b_stride, M, n_in, dtype);
   return pack_bytes(a, a_stride, M, pass == kForward ? n_in : n_out, dtype) + pack_bytes(b, n_in, E * n_out, n_in, dtype);
 }
 
@@ -528,13 +548,13 @@ extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void
   PS_REQUIRE((M == 0 || (dy != nullptr && x != nullptr)) && offsets != nullptr && dweight != nullptr, "ps_expert_linear_dw: null argument");
   PS_REQUIRE(workspace != nullptr || workspace_of(kWeightGradient, dy, dy_stride, x, x_stride, M, E, n_in, n_out, dtype) == 0,
              "ps_expert_linear_dw: needs its workspace (ps_expert_linear_workspace)");
-  const DwPlan p = dw_plan(M, E, n_in, n_out);
+  const DwPlan p = dw_plan(M, E, n_in, n_out, dtype);
   const int N = (int)n_out, K = (int)n_in, ldo = (int)round4(n_in);
   hipStream_t s = (hipStream_t)stream;
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     float* parts = (float*)workspace;
-    char* to = (char*)workspace + dw_part_bytes(M, E, n_in, n_out);
+    char* to = (char*)workspace + dw_part_bytes(p, n_in, n_out);
     const Rows dys = packed<T>(dy, dy_stride, M, n_out, dtype, &to, s), xs = packed<T>(x, x_stride, M, n_in, dtype, &to, s);
     if (p.piece == 0) return launch_dw<T, false>(p, dys, xs, offsets, M, E, N, K, K, dweight, dbias, s);
     float* db_parts = parts + p.units * n_out * ldo;

@@ -390,6 +390,14 @@ def test_linear_of_every_tile(dev, M, E, n_in, n_out, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M,E,n_in,n_out", [(4200, 64, 512, 520), (24000, 1, 776, 1000)])
+def test_gradients_of_the_largest_tiles(dev, M, E, n_in, n_out, dtype):
+    """weights' gradients by 256 x 256, whole and in pieces"""
+    check_linear(dev, M, E, n_in, n_out, dtype, "even", bias=True)
+
+
+@pytest.mark.gpu
 def test_linear_of_rows_far_apart(dev):
     """rows more than 2^20 elements apart are copied first"""
     x = torch.zeros(5, (1 << 20) + 4, device=dev)
