@@ -81,8 +81,12 @@ class ExpertPlan:
         for t in (offsets, src, dst):
             if t.dtype != torch.int32 or t.device != dst.device or not t.is_contiguous():
                 raise TypeError("presight_amd: a plan holds contiguous int32 tensors on one device")
+        self._set(offsets, src, dst, num_experts)
+
+    def _set(self, offsets: Tensor, src: Tensor, dst: Tensor, num_experts: int) -> "ExpertPlan":
         self.offsets, self.src, self.dst, self.num_experts = offsets, src, dst, num_experts
         self.num_rows, self.k = dst.shape
+        return self
 
     @property
     def num_places(self) -> int:
@@ -116,7 +120,7 @@ def expert_plan(ids: Tensor, num_experts: int) -> ExpertPlan:
         ws = torch.empty(ints, device=dev, dtype=torch.int32) if ints else None
         check(lib().ps_expert_plan(_p(ids), int(ids.dtype == torch.int64), M, num_experts, _p(offsets), _p(src), _p(dst), _p(ws), _stream()),
               "ps_expert_plan")
-    return ExpertPlan(offsets, src, dst, num_experts)
+    return ExpertPlan.__new__(ExpertPlan)._set(offsets, src, dst, num_experts)
 
 
 # ------------------------------------------------------------------------------------------------ exchange

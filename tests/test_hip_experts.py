@@ -398,6 +398,14 @@ def test_gradients_of_the_largest_tiles(dev, M, E, n_in, n_out, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("M,E,kind", [(16, 1000, "ragged"), (700, 65, "ragged"), (700, 129, "even"), (2000, 5000, "ragged"), (9, 8200, "even"), (40, 4097, "one")])
+def test_linear_of_many_experts(dev, M, E, kind, dtype):
+    """more experts than lanes, and than lanes times lanes"""
+    check_linear(dev, M, E, 24, 40, dtype, kind, bias=True)
+
+
+@pytest.mark.gpu
 def test_linear_of_rows_far_apart(dev):
     """rows more than 2^20 elements apart are copied first"""
     x = torch.zeros(5, (1 << 20) + 4, device=dev)
