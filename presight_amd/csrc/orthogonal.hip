@@ -20,6 +20,7 @@ using namespace ps;
 
 constexpr float kPlaneScale = 1024.0f;                       // fp16 planes hold 1024 * value
 constexpr float kProductScale = 1.0f / (1024.0f * 1024.0f);  // of a product of two
+constexpr int kCompute = 256;                                // compute units
 constexpr int kNormParts = 256;                              // partial sums of squares per matrix, at most
 
 template <typename V>  // float or double
@@ -55,30 +56,10 @@ struct Work {
   _Float16 *x[2], *gram, *poly;  // pairs: [B][s][2 lp] twice, [B][s][2 sp], [B][s][2 sp]
   double* norms;                 // [B][parts]
   float* ratio;                  // [B] r at the start
+  f32x4* shares;                 // [parts][B][tiles][64 x 64] fp32 sums, where a product's k is shared out
   int parts;
   int64_t bytes;
 };
-Work work_of(const Shape& h, int64_t B, void* base) {
-  Work w;
-  const int64_t x_bytes = B * h.s * (int64_t)h.lp * 4, s_bytes = B * h.s * (int64_t)h.sp * 4;
-  char* p = (char*)base;
-  auto take = [&](int64_t bytes) {
-    char* q = p;
-    p += (bytes + 255) & ~(int64_t)255;
-    return q;
-  };
-  const int64_t parts = h.m * h.n / 8192;  // (at least a few thousand elements each)
-  w.parts = (int)(parts < 1 ? 1 : (parts > kNormParts ? kNormParts : parts));
-  w.norms = (double*)take(B * kNormParts * 8);
-  w.ratio = (float*)take(B * 4);
-  w.x[0] = (_Float16*)take(x_bytes);
-  w.x[1] = (_Float16*)take(x_bytes);
-  w.gram = (_Float16*)take(s_bytes);
-  w.poly = (_Float16*)take(s_bytes);
-  w.bytes = p - (char*)base;
-  return w;
-}
-
 // Where the matrix comes from: G itself, or an optimizer's momentum buf <- mu buf + (1 - mu) g, taken as it is or (nesterov) as
 // mu buf + (1 - mu) g once more
 struct Source {
@@ -220,9 +201,7 @@ struct Operands {  // pairs
 // A workgroup's tile: BM x BN; a stage is 32 k of both planes of either operand, one tile row of 128 bytes for a row of k (KC).  A compute
 // unit can have about 17 bytes per cycle of the L2's in flight, so the tile decides how fast the matrix instructions are fed: at their full
 // rate 256 x 128 asks for 32 bytes per cycle, 128 x 128 for 43 and 64 x 64 for 85, and a step of k takes as long as its stage of 48, 32 or
-// 16 KiB takes to arrive.  256 rows are taken where that still makes a tile for every second compute unit (2048 x 4096, P X: 131 -> 113 us;
-// 8 x 1024 x 2048: 150 -> 122), else 64 x 64 while no compute unit gets more than the two that fit its LDS (all five steps: 3 x 385 x 129
-// 229 -> 132 us, 1024 x 1024 479 -> 273, 1536 x 1536 671 -> 517; with more of them 2048 x 4096 would go from 1236 to 1317), else 128 x 128.
+// 16 KiB takes to arrive.
 // The two small products add up apart from the large one: each of their additions to it would cost it another rounding.
 //
 // 2048 x 4096: S 90 us, a I + b S + c S S 56, times X 115: 573, 464 and 897 TFLOP/s of pairs' products (half of S and S S by symmetry, three
@@ -231,6 +210,10 @@ struct Operands {  // pairs
 //
 // The result leaves through LDS as rows of whole lines.  Of a symmetric one only what lies on and below the diagonal's BN x BN blocks is
 // computed and written, and then written turned.
+// Few tiles and a long k, as of S of a wide matrix: k is shared out over several workgroups per tile (kShare), their fp32 sums go through memory,
+// and a second launch (kJoin) adds them up in order and takes the way out.  (All five steps: 512 x 8192 612 -> 301 us.)
+enum Part { kAllOfK, kShare, kJoin };
+
 constexpr int kPairK = 32;
 template <int BM>
 struct PairTile {
@@ -249,8 +232,9 @@ __host__ __device__ inline int symmetric_tiles(int tm, int across, int n_tiles) 
   return n < n_tiles ? n : n_tiles;
 }
 
-template <typename T, Product WHAT, int BM>
-__global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Operands o, Shape h, Work w, int batches, int tiles, int step, Poly c, Result res) {
+template <typename T, Product WHAT, int BM, Part PART>
+__global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Operands o, Shape h, Work w, int batches, int tiles, int parts, int step, Poly c,
+                                                                            Result res) {
   using Tile = PairTile<BM>;
   constexpr int BN = Tile::kN, NT = Tile::kThreads, WN = Tile::kWavesN, MI = Tile::kWaveM / 16, NJ = Tile::kWaveN / 16, kStages = Tile::kStages,
                 kStage = Tile::kStage, kGroup = Tile::kGroup;
@@ -261,8 +245,13 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int m_tiles = (o.ra + BM - 1) / BM, n_tiles = (o.rb + BN - 1) / BN;
   // (the batch's matrices one under the other; `tiles`: of one of them)
-  const int place = xcd_place(blockIdx.x, tiles * batches);
+  const int shares = PART == kShare ? parts : 1;
+  int place = xcd_place(blockIdx.x, tiles * batches * shares), part = 0;
   if (place < 0) return;
+  if constexpr (PART == kShare) {  // (a part's tiles share their operands)
+    part = place / (tiles * batches);
+    place -= part * tiles * batches;
+  }
   int tm = 0, tn;
   int64_t batch;
   if constexpr (kSymmetric) {
@@ -276,8 +265,10 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
   }
   const int m0 = tm * BM, n0 = tn * BN;
   const int rows = o.ra - m0 < BM ? o.ra - m0 : BM, cols = o.rb - n0 < BN ? o.rb - n0 : BN;
-  const SourceA sa(o.a + (batch * o.ra + m0) * 2 * o.k, 2 * o.k, rows, 2 * o.k);
-  const SourceB sb = kSymmetric ? SourceB(o.b + (batch * o.rb + n0) * 2 * o.k, 2 * o.k, cols, 2 * o.k)
+  // this part's steps, even numbers of them; the loads behind the last one bring zeros
+  const int steps = o.k / kPairK, first = PART == kShare ? steps / 2 * part / parts * 2 : 0, end = PART == kShare ? steps / 2 * (part + 1) / parts * 2 : steps;
+  const SourceA sa(o.a + (batch * o.ra + m0) * 2 * o.k, 2 * o.k, rows, 2 * kPairK * end);
+  const SourceB sb = kSymmetric ? SourceB(o.b + (batch * o.rb + n0) * 2 * o.k, 2 * o.k, cols, 2 * kPairK * end)
                                 : SourceB(o.b + batch * o.k_rows * 2 * o.ldb + 2 * n0, 2 * o.ldb, 2 * (o.ldb - n0), o.k_rows);
   auto load = [&](int stage) {  // stage by stage of k; KC counts both planes
     char* to = lds + stage % kStages * kStage;
@@ -304,11 +295,11 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
     for (int i = 0; i < MI; ++i)
 #pragma unroll
       for (int j = 0; j < NJ; ++j) early[0][i][j] = gram_at(i, j, 0), early[1][i][j] = gram_at(i, j, 1);
-  const int steps = o.k / kPairK;  // (even)
-  __builtin_assume(steps > 0);     // (no way past the loop to prepare for: 3 x 385 x 129 124 -> 121 us)
+  if constexpr (PART != kJoin) {
+  __builtin_assume(first < end);  // (no way past the loop to prepare for: 3 x 385 x 129 124 -> 121 us)
 #pragma unroll
-  for (int i = 0; i < kStages - kGroup; ++i) load(i);
-  for (int i = 0; i < steps; i += kGroup) {
+  for (int i = 0; i < kStages - kGroup; ++i) load(first + i);
+  for (int i = first; i < end; i += kGroup) {
     tile_barrier<(kStages - 2 * kGroup) * kLoads>();
 #pragma unroll
     for (int u = 0; u < kGroup; ++u) load(i + u + kStages - kGroup);  // (where the stages before i were; zeros behind the last)
@@ -336,6 +327,24 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
           fine[q][j] = mma_block<_Float16>(fa[1][q], fb[0][j], fine[q][j]);
         }
     }
+  }
+  }
+  if constexpr (PART == kShare) {
+    f32x4* mine = w.shares + ((int64_t)(part * batches + batch) * tiles + place % tiles) * (NT * MI * NJ) + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) mine[(i * NJ + j) * NT] = acc[i][j] + fine[i][j];
+    tile_barrier<0>();  // (no load is left on its way into LDS)
+    return;
+  }
+  if constexpr (PART == kJoin) {
+    const f32x4* from = w.shares + (batch * tiles + place % tiles) * (NT * MI * NJ) + threadIdx.x;
+    for (int q = 0; q < parts; ++q, from += (int64_t)batches * tiles * (NT * MI * NJ))
+#pragma unroll
+      for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] += from[(i * NJ + j) * NT];
   }
   __syncthreads();
   const float ratio = ratio_at(start_ratio, step, c.grow);
@@ -449,31 +458,84 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
   }
 }
 
-template <typename T, Product WHAT, int BM>
-int product_tiles(const Operands& o) {
-  constexpr int BN = PairTile<BM>::kN;
-  const int m = (o.ra + BM - 1) / BM, n = (o.rb + BN - 1) / BN;
-  if (WHAT == kApply || WHAT == kLast) return m * n;
-  int all = 0;
-  for (int t = 0; t < m; ++t) all += symmetric_tiles(t, BM / BN, n);
+// tiles of a product of ra x rb
+int64_t product_tiles(int bm, int ra, int rb, bool symmetric) {
+  const int bn = bm == 64 ? 64 : 128;
+  const int64_t m = (ra + bm - 1) / bm, n = (rb + bn - 1) / bn;
+  if (!symmetric) return m * n;
+  int64_t all = 0;
+  for (int t = 0; t < m; ++t) all += symmetric_tiles(t, bm / bn, (int)n);
   return all;
 }
 
-template <typename T, Product WHAT, int BM>
-void launch_product_tile(const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res, hipStream_t s) {
-  const int tiles = product_tiles<T, WHAT, BM>(o);
-  hipFuncSetAttribute((const void*)ns_product_kernel<T, WHAT, BM>, hipFuncAttributeMaxDynamicSharedMemorySize, PairTile<BM>::kLds);
-  ns_product_kernel<T, WHAT, BM><<<(unsigned)xcd_blocks(tiles * B), PairTile<BM>::kThreads, PairTile<BM>::kLds, s>>>(o, h, w, (int)B, tiles, step, c, res);
+// How a product is cut: the cheapest of what a step of k of a round of tiles, one per compute unit, takes: .42 us (64 x 64, of which two or more
+// share a compute unit; alone .55), .95 (128 x 128) or 1.65 (256 x 128).  All five steps: 2048 x 4096 with tiles of 256 and 128 1236 us, 128
+// alone about 1330, 64 alone 1489; 1024 x 1024 with 64 273, with 128 479; 300 x 128 x 128 with 64 269, with 256 499.  Then the parts of k
+// of S: as many as two workgroups per compute unit allow, where they save more steps than they and the second launch cost (1024 x 1024,
+// 22 of 32 steps saved: 266 -> 278).
+struct ProductPlan {
+  int tile, parts;
+  int64_t tiles;
+};
+ProductPlan product_plan(Product what, int ra, int rb, int k, int64_t B) {
+  const bool gram = what == kGram, symmetric = gram || what == kPoly;
+  ProductPlan best{64, 1, 0};
+  double best_cost = 1e30;
+  for (int tile = 64; tile <= 256; tile *= 2) {
+    const int64_t tiles = product_tiles(tile, ra, rb, symmetric), rounds = (tiles * B + kCompute - 1) / kCompute;
+    const double cost = tile == 64 ? (rounds > 1 ? 0.42 * (double)rounds : 0.55) : (tile == 128 ? 0.95 : 1.65) * (double)rounds;
+    if (cost < best_cost) best_cost = cost, best.tile = tile, best.tiles = tiles;
+  }
+  if (best.tile == 64 && gram) {
+    const int64_t steps = k / kPairK, room = 2 * kCompute / (best.tiles * B), parts = room < steps / 8 ? room : steps / 8;
+    if (parts > 1 && steps - steps / parts > 32) best.parts = (int)parts;
+  }
+  return best;
+}
+
+Work work_of(const Shape& h, int64_t B, void* base) {
+  Work w;
+  const int64_t x_bytes = B * h.s * (int64_t)h.lp * 4, s_bytes = B * h.s * (int64_t)h.sp * 4;
+  char* p = (char*)base;
+  auto take = [&](int64_t bytes) {
+    char* q = p;
+    p += (bytes + 255) & ~(int64_t)255;
+    return q;
+  };
+  const int64_t parts = h.m * h.n / 8192;  // (at least a few thousand elements each)
+  w.parts = (int)(parts < 1 ? 1 : (parts > kNormParts ? kNormParts : parts));
+  w.norms = (double*)take(B * kNormParts * 8);
+  w.ratio = (float*)take(B * 4);
+  w.x[0] = (_Float16*)take(x_bytes);
+  w.x[1] = (_Float16*)take(x_bytes);
+  w.gram = (_Float16*)take(s_bytes);
+  w.poly = (_Float16*)take(s_bytes);
+  const ProductPlan gram = product_plan(kGram, h.s, h.s, h.lp, B);
+  w.shares = (f32x4*)take(gram.parts > 1 ? gram.parts * gram.tiles * B * 64 * 64 * 4 : 0);
+  w.bytes = p - (char*)base;
+  return w;
+}
+
+template <typename T, Product WHAT, int BM, Part PART>
+void launch_product_tile(const ProductPlan& p, const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res,
+                         hipStream_t s) {
+  const int64_t blocks = xcd_blocks(p.tiles * B * (PART == kShare ? p.parts : 1));
+  hipFuncSetAttribute((const void*)ns_product_kernel<T, WHAT, BM, PART>, hipFuncAttributeMaxDynamicSharedMemorySize, PairTile<BM>::kLds);
+  ns_product_kernel<T, WHAT, BM, PART>
+      <<<(unsigned)blocks, PairTile<BM>::kThreads, PairTile<BM>::kLds, s>>>(o, h, w, (int)B, (int)p.tiles, p.parts, step, c, res);
 }
 
 template <typename T, Product WHAT>
 void launch_product(const Operands& o, const Shape& h, const Work& w, int64_t B, int step, const Poly& c, const Result& res, hipStream_t s) {
-  if (product_tiles<T, WHAT, 256>(o) * B >= 128)
-    launch_product_tile<T, WHAT, 256>(o, h, w, B, step, c, res, s);
-  else if (product_tiles<T, WHAT, 64>(o) * B <= 512)
-    launch_product_tile<T, WHAT, 64>(o, h, w, B, step, c, res, s);
-  else
-    launch_product_tile<T, WHAT, 128>(o, h, w, B, step, c, res, s);
+  const ProductPlan p = product_plan(WHAT, o.ra, o.rb, o.k, B);
+  if constexpr (WHAT == kGram)
+    if (p.parts > 1) {
+      launch_product_tile<T, WHAT, 64, kShare>(p, o, h, w, B, step, c, res, s);
+      return launch_product_tile<T, WHAT, 64, kJoin>(p, o, h, w, B, step, c, res, s);
+    }
+  if (p.tile == 256) return launch_product_tile<T, WHAT, 256, kAllOfK>(p, o, h, w, B, step, c, res, s);
+  if (p.tile == 128) return launch_product_tile<T, WHAT, 128, kAllOfK>(p, o, h, w, B, step, c, res, s);
+  return launch_product_tile<T, WHAT, 64, kAllOfK>(p, o, h, w, B, step, c, res, s);
 }
 
 // ------------------------------------------------------------------------------------------------ small matrices
@@ -505,9 +567,10 @@ struct SmallStacks {
 __host__ __device__ inline int round16(int v) { return (v + 15) & ~15; }
 __host__ __device__ inline int small_ld(int l) { return ((l + 63) & ~63) + 4; }
 inline int64_t small_lds_bytes(int64_t s, int64_t l) { return (round16((int)s) * (int64_t)small_ld((int)l) + 2 * round16((int)s) * kSmallLd) * 4; }
-inline bool is_small(int64_t m, int64_t n) {
+// (a few long ones are better spread over the chip: 32 x 1024 153 us here, 121 there; 256 of 64 x 256 81 and 300)
+inline bool is_small(int64_t B, int64_t m, int64_t n) {
   const int64_t s = m < n ? m : n, l = m < n ? n : m;
-  return s <= kSmallSide && l <= 4096 && small_lds_bytes(s, l) <= kSmallLds;
+  return s <= kSmallSide && l <= 4096 && small_lds_bytes(s, l) <= kSmallLds && (l <= 512 || B >= 64);
 }
 
 // two 16 x 16 blocks of rows . rows^T: acc[j] = A(16 i .., :) B(16 (j0 + j) .., :)^T over k
@@ -637,7 +700,7 @@ void launch_small(const SmallStacks& all, int blocks, int64_t lds, int steps, co
 
 template <typename T, bool MOMENTUM>
 int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Poly& c, float eps, const Result& res, void* workspace, hipStream_t s) {
-  if (is_small(m, n)) {
+  if (is_small(B, m, n)) {
     SmallStacks one;
     one.count = 1;
     one.stack[0] = {src, res, 0, (int)m, (int)n};
@@ -652,11 +715,11 @@ int run(const Source& src, int64_t B, int64_t m, int64_t n, int steps, const Pol
   ns_start_kernel<T, MOMENTUM><<<start_grid, 256, 0, s>>>(src, h, w, eps);
   for (int i = 0; i < steps; ++i) {
     const _Float16* x = w.x[i & 1];
-    launch_product<T, kGram>({x, x, h.s, h.s, h.lp, 0, 0}, h, w, B, i, c, res, s);
-    launch_product<T, kPoly>({w.gram, w.gram, h.s, h.s, h.sp, 0, 0}, h, w, B, i, c, res, s);
+    launch_product<float, kGram>({x, x, h.s, h.s, h.lp, 0, 0}, h, w, B, i, c, res, s);
+    launch_product<float, kPoly>({w.gram, w.gram, h.s, h.s, h.sp, 0, 0}, h, w, B, i, c, res, s);
     const Operands apply{w.poly, x, h.s, h.l, h.sp, h.s, h.lp};
     if (i + 1 < steps)
-      launch_product<T, kApply>(apply, h, w, B, i, c, res, s);
+      launch_product<float, kApply>(apply, h, w, B, i, c, res, s);
     else
       launch_product<T, kLast>(apply, h, w, B, i, c, res, s);
   }
@@ -673,7 +736,7 @@ bool sizes_ok(int64_t B, int64_t m, int64_t n, int steps) {
 }  // namespace
 
 extern "C" int64_t ps_newton_schulz_workspace(int64_t B, int64_t m, int64_t n) {
-  if (!sizes_ok(B, m, n, 1) || B == 0 || m == 0 || n == 0 || is_small(m, n)) return 0;
+  if (!sizes_ok(B, m, n, 1) || B == 0 || m == 0 || n == 0 || is_small(B, m, n)) return 0;
   return work_of(shape_of(m, n), B, nullptr).bytes;
 }
 
@@ -681,7 +744,7 @@ extern "C" int ps_newton_schulz(const void* g, int64_t B, int64_t m, int64_t n, 
                                 void* workspace, void* stream) {
   PS_REQUIRE(sizes_ok(B, m, n, steps) && grow >= 1.0f, "ps_newton_schulz: sizes out of range");
   if (B == 0 || m == 0 || n == 0) return 0;
-  PS_REQUIRE(g != nullptr && out != nullptr && (workspace != nullptr || is_small(m, n)), "ps_newton_schulz: null argument");
+  PS_REQUIRE(g != nullptr && out != nullptr && (workspace != nullptr || is_small(B, m, n)), "ps_newton_schulz: null argument");
   const Poly co{a, b, c, grow};
   const Source src{g, nullptr, 0.0f, 1.0f, 0};
   const Result res{out, 0, 0.0f, 0.0f};
@@ -700,7 +763,7 @@ extern "C" int ps_muon_step(int n_stacks, float* const* p, const float* const* g
   PS_REQUIRE(n_stacks == 0 || (p && g && buf && B && m && n && rate), "ps_muon_step: null argument");
   for (int i = 0; i < n_stacks; ++i) {
     PS_REQUIRE(sizes_ok(B[i], m[i], n[i], steps), "ps_muon_step: sizes out of range");
-    PS_REQUIRE(B[i] * m[i] * n[i] == 0 || (p[i] && g[i] && buf[i] && (workspace || is_small(m[i], n[i]))), "ps_muon_step: null argument");
+    PS_REQUIRE(B[i] * m[i] * n[i] == 0 || (p[i] && g[i] && buf[i] && (workspace || is_small(B[i], m[i], n[i]))), "ps_muon_step: null argument");
   }
   const Poly co{a, b, c, grow};
   hipStream_t s = (hipStream_t)stream;
@@ -717,7 +780,7 @@ extern "C" int ps_muon_step(int n_stacks, float* const* p, const float* const* g
     if (B[i] == 0 || m[i] == 0 || n[i] == 0) continue;
     const Source src{g[i], buf[i], (float)momentum, (float)(1.0 - momentum), nesterov};
     const Result res{p[i], 1, keep, rate[i]};
-    if (!is_small(m[i], n[i])) {
+    if (!is_small(B[i], m[i], n[i])) {
       const int rc = run<float, true>(src, B[i], m[i], n[i], steps, co, eps, res, workspace, s);
       if (rc != 0) return rc;
       continue;

@@ -191,6 +191,16 @@ def test_every_tile(dev, shape, dtype):
         assert float((got.double() - ref).norm()) <= max(4 * float((plain.double() - ref).norm()), 16 * 2.0 ** -24 * float(ref.norm())) + rounding
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("shape", [(1, 8, 4096), (3, 70, 3000), (2, 4000, 100), (5, 30, 600), (64, 30, 600), (60, 128, 128), (1, 200, 5001)])
+def test_long_and_many(dev, shape, dtype):
+    """few rows and a long other side, whose sums over it are shared out; many matrices of few tiles"""
+    x = (torch.randn(shape, generator=torch.Generator().manual_seed(16)) * 1e-2).to(TYPES[dtype])
+    check(optim.newton_schulz(x.to(dev)), x)
+    assert torch.equal(optim.newton_schulz(x.to(dev)), optim.newton_schulz(x.to(dev)))
+
+
 # ------------------------------------------------------------------------------------------------ the optimizer
 def muon_ref(p, g, buf, lr, mu, nesterov, wd, scale):
     buf = mu * buf + (1 - mu) * g
@@ -233,7 +243,7 @@ def test_muon_steps(dev, shapes, nesterov, scale):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("shape", [(12, 600, 700), (12, 701, 603), (3, 704, 500), (2, 31, 33)])
+@pytest.mark.parametrize("shape", [(12, 600, 700), (12, 701, 603), (3, 704, 500), (2, 31, 33), (2, 50, 2000), (64, 16, 700)])
 def test_muon_applies_the_orthogonalised_momentum(dev, shape):
     """the first step's u is the same bits computed outside (two products and a sum, each rounded), so its orthogonalised form is too; the
     parameter then carries two roundings of about its own size and one of the product's"""
