@@ -376,14 +376,32 @@ bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
 
 constexpr int kCompute = 256;  // compute units
 
-// Tile sizes, by work per tile.  256 x 256 reads each operand byte half as often as 128 x 128, but one tile fills a compute unit: it is taken
-// where it wastes little of itself and there is a tile for every compute unit (bf16: 65536 rows, 32 experts of 2048 x 1024 316 us, with 128
-// 375; 16384, 8 of 1024 x 1024 35 and 42).  Narrow outputs and few rows per expert take the smaller ones (128 rows each, 64 experts of 1024 x
-// 1024: tiles of 128 28 us, of 64 32; 64 rows each, 512 x 512: 11.2 and 9.4).
-int linear_tile(int64_t rows, int64_t groups, int64_t cols) {
+// What a step of k (128 bytes of it) of a 64, 128 or 256 tile was measured to take, us: of its compute unit's time (the reads from the L2; in fp32
+// the matrix instructions), and at least from its start to its end
+struct StepCost {
+  double busy[3], least[3];
+};
+StepCost step_cost(int dtype) {
+  if (dtype == kF32) return {{0.47, 1.75, 7.0}, {0.8, 1.75, 7.0}};
+  return {{0.27, 0.73, 2.1}, {0.45, 0.8, 2.1}};
+}
+
+// Tile sizes: the cheapest by these, of those that an expert's share of the rows fills for the most part (bf16: 65536 rows, 32 experts of 2048 x
+// 1024 with 256 316 us, with 128 375; 16384, 8 of 1024 x 1024 35 and 42; 128 rows each, 64 experts of 1024 x 1024 with 128 28 us, with 64 32; 64
+// rows each, 512 x 512 11.2 and 9.4; fp32, 740 rows, 3 of 495 -> 80 with 128 45, with 64 20).
+int linear_tile(int64_t rows, int64_t groups, int64_t cols, int dtype) {
+  const StepCost cost = step_cost(dtype);
   const int64_t each = rows / groups;
-  if (cols > 128 && each >= 192 && (rows / 256 + groups) * ((cols + 255) / 256) >= kCompute) return 256;
-  return cols > 64 && each >= 96 ? 128 : 64;
+  int best = 64;
+  double best_us = 1e30;
+  for (int i = 0; i < 3; ++i) {
+    const int tile = 64 << i;
+    if (i > 0 && (cols <= tile / 2 || each * 4 < tile * 3)) break;
+    const double shared = ((double)rows / tile + 0.5 * groups) * (double)((cols + tile - 1) / tile) / kCompute;  // tiles per compute unit
+    const double us = cost.busy[i] * shared > cost.least[i] ? cost.busy[i] * shared : cost.least[i];
+    if (us <= best_us) best = tile, best_us = us;
+  }
+  return best;
 }
 
 template <typename K>
@@ -442,7 +460,7 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
     const int64_t k = W_RC ? n_out : n_in;
     const Rows xs = packed<T>(x, ldx, M, k, dtype, &to, s), ws = packed<T>(weight, n_in, E * n_out, n_in, dtype, &to, s);
     const int N = (int)(W_RC ? n_in : n_out), K = (int)padded(k, dtype), rows = (int)n_out;
-    switch (linear_tile(M, E, N)) {
+    switch (linear_tile(M, E, N, dtype)) {
       case 256: return launch_linear_tile<T, 256, 2, 4, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
       case 128: return launch_linear_tile<T, 128, 2, 2, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
       default: return launch_linear_tile<T, 64, 2, 2, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
@@ -455,16 +473,13 @@ struct DwPlan {
   int tile, piece;
   int64_t units;
 };
-// The cheapest by what was measured: a step of k (128 bytes of it) of a 64, 128 or 256 tile takes its compute unit .27, .73 or 2.1 us in 16 bits,
-// of a 64 or 128 tile .44 or 1.75 in fp32 (bound by the matrix instructions: a larger one gains nothing), and no less than .45, .8 or 2.1
-// (.8 or 1.75) from its start to its end.  Pieces shorten the longest run of
-// steps and cost 5 us and the way of their fp32 sums through the memory, 4.5 TB/s; without them an expert may well have twice its
-// share of the rows.
+// The cheapest by the tiles' steps.  Pieces shorten the longest run of steps and cost 5 us and the way of their fp32 sums through the memory,
+// 4.5 TB/s; without them an expert may well have twice its share of the rows.  (fp32: tiles of 256 gain nothing.)
 //     16 experts, fp32:  131072 rows of 64 x 64 in pieces 22 us, whole 191 | 32768 rows of 128 x 128 in pieces, tiles of 64 21, of 128 30
 //     bf16:  8192 rows, 16 experts of 512 x 512 whole 12, in pieces 45 | 65536 rows, 32 experts of 2048 x 1024 tiles of 256 307, of 128 374
 DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
   const bool wide = dtype == kF32;
-  const double busy_us[3] = {wide ? 0.44 : 0.27, wide ? 1.75 : 0.73, 2.1}, least_us[3] = {wide ? 0.8 : 0.45, wide ? 1.75 : 0.8, 2.1};
+  const StepCost cost = step_cost(dtype);
   const int64_t least = n_in < n_out ? n_in : n_out, step_rows = wide ? 32 : 64, each = M / E;
   DwPlan best{64, 0, E};
   double best_us = 1e30;
@@ -482,8 +497,8 @@ DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
         p.units = row_tiles_at_most(M, E, p.piece);
       }
       const double shared = tiles * (pieces > 1 ? (double)M / rows + 0.5 * E : (double)E) / kCompute;  // workgroups per compute unit
-      const double steps = (double)((rows + step_rows - 1) / step_rows), all = busy_us[i] * (shared > 1 ? shared : 1) * (steps > 1 ? steps : 1);
-      const double run = least_us[i] * (double)((longest + step_rows - 1) / step_rows);
+      const double steps = (double)((rows + step_rows - 1) / step_rows), all = cost.busy[i] * (shared > 1 ? shared : 1) * (steps > 1 ? steps : 1);
+      const double run = cost.least[i] * (double)((longest + step_rows - 1) / step_rows);
       const double us = (all > run ? all : run) + (pieces > 1 ? 5.0 + 8e-6 / 4.5 * p.units * n_in * n_out : 0.0);
       if (us < best_us) best = p, best_us = us;
     }
