@@ -152,9 +152,9 @@ __device__ __forceinline__ void direct_loop(char* lds, int K, const DirectSource
 // A wave's part of a tile into memory, turned in LDS on the way: four values per lane and row make requests of 8 to 16 bytes (65536 x
 // 1024 bf16: 12.6 million of them, a third of the kernel's time); from a row of the wave's own LDS slice (MI * 16 rows in as many passes
 // as it takes) every lane writes 16 bytes of whole 64- to 256-byte rows.  No other wave reads the slice, and the tiles are done with.
-template <typename T, int MI, int NJ, int SLICE>
+template <typename T, int MI, int NJ, int SLICE, typename Bias>
 __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slice, T* __restrict__ y, int64_t ldy, int rows, int cols, int m0, int n0,
-                                                const T* __restrict__ bias) {
+                                                const Bias* __restrict__ bias) {
   constexpr int kRow = NJ * 16 * (int)sizeof(T), kAcross = kRow / 16;  // bytes and chunks of a row
   constexpr int kFit = SLICE / (16 * kRow), kPass = kFit < MI ? kFit : MI;  // blocks of 16 rows per pass
   constexpr int kSpread = kAcross < 8 ? kAcross - 1 : 7;
@@ -210,30 +210,58 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
 // incomplete tiles in a round of their own behind the whole ones, and lines fetched into the L2 two to eight steps of k ahead, were slower.)
 // y[p] = sum_k x[p][k] W(n,k) (+ bias).  W_RC = false: the weight's rows are k-contiguous (forward), n of them; true: n-contiguous (input
 // gradient), `w_rows` of them.  K: the rows' length in whole chunks.
-template <typename T, int BM, int BN, int WM, int WN, bool W_RC>
+// SHARED: k is shared out over `parts` workgroups per tile, whose fp32 sums go to y [parts][M][N]; linear_join_kernel adds them up in order.
+template <typename T, int BM, int BN, int WM, int WN, bool W_RC, bool SHARED>
 __global__ __launch_bounds__(64 * WM * WN) void linear_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ weight, int64_t ldw, int w_rows,
                                                               const T* __restrict__ bias, const int* __restrict__ offsets, int64_t M, int E, int N, int K,
-                                                              T* __restrict__ y) {
+                                                              int parts, std::conditional_t<SHARED, float, T>* __restrict__ y) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
+  using Out = std::conditional_t<SHARED, float, T>;
+  int k_rows = w_rows;  // of a weight with k along its rows
   extern __shared__ __attribute__((aligned(16))) char lds[];
   RowTiles tiles(offsets, E, M, BM);
-  const int n_tiles = (N + BN - 1) / BN, all = tiles.total * n_tiles, place = xcd_place(blockIdx.x, all);
+  const int n_tiles = (N + BN - 1) / BN, all = tiles.total * n_tiles;
+  int place = xcd_place(blockIdx.x, SHARED ? all * parts : all);
   if (place < 0) {
-    clear_outside<T>(offsets, E, M, xcd_spare(blockIdx.x, gridDim.x, all), gridDim.x - all, y, N);
+    if constexpr (!SHARED) clear_outside<T>(offsets, E, M, xcd_spare(blockIdx.x, gridDim.x, all), gridDim.x - all, y, N);
     return;
+  }
+  if constexpr (SHARED) {
+    const int part = place / all, steps = (K + kTileK<T> - 1) / kTileK<T>;
+    const int k0 = (int)((int64_t)steps * part / parts) * kTileK<T>, k1 = (int)((int64_t)steps * (part + 1) / parts) * kTileK<T>;
+    place -= part * all;
+    y += (int64_t)part * M * N;
+    x += k0;
+    weight += W_RC ? k0 * ldw : k0;
+    k_rows = w_rows - k0 < k1 - k0 ? w_rows - k0 : k1 - k0;
+    K = (k1 < K ? k1 : K) - k0;
+    if (part > 0) bias = nullptr;
   }
   const TileAt at = patched_tile(place, tiles.total, n_tiles);
   const RowTile t = tiles.find(at.m);
   const int n0 = at.n * BN, cols = N - n0 < BN ? N - n0 : BN;
   const T* wb = weight + (int64_t)t.expert * w_rows * ldw + (W_RC ? (int64_t)n0 : n0 * ldw);
   const DirectSource<T, BM, NT, false> sa(x + t.row0 * ldx, ldx, t.rows, K);
-  const DirectSource<T, BN, NT, W_RC> sb(wb, ldw, W_RC ? (N + kChunk<T> - 1) / kChunk<T> * kChunk<T> - n0 : cols, W_RC ? w_rows : K);
+  const DirectSource<T, BN, NT, W_RC> sb(wb, ldw, W_RC ? (N + kChunk<T> - 1) / kChunk<T> * kChunk<T> - n0 : cols, W_RC ? k_rows : K);
   f32x4 acc[MI][NJ], none[1];
   direct_loop<T, BM, BN, WM, WN, false, W_RC, false>(lds, K, sa, sb, acc, none, false);
   const int wave = uniform(threadIdx.x >> 6), wm = (wave / WN) * (BM / WM), wn = (wave % WN) * (BN / WN);
   constexpr int kSlice = 2 * (BM + BN) * kTileRowBytes / (WM * WN);
-  store_tile_rows<T, MI, NJ, kSlice>(acc, lds + wave * kSlice, y + t.row0 * N + n0, N, t.rows, cols, wm, wn,
-                                     bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
+  store_tile_rows<Out, MI, NJ, kSlice>(acc, lds + wave * kSlice, y + t.row0 * N + n0, N, t.rows, cols, wm, wn,
+                                       bias != nullptr ? bias + (int64_t)t.expert * N + n0 : nullptr);
+}
+
+// y [M,N] = the sums of parts [parts][M][N]; zeros for the rows of nobody
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ sums, int parts, const int* __restrict__ offsets, int E, int64_t M, int N,
+                                                          T* __restrict__ y) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / N, size = M * N;
+  if (i >= size) return;
+  float v = 0.0f;
+  if (row >= bounded(offsets[0], M) && row < bounded(offsets[E], M))
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) v += sums[p * size + i];
+  y[i] = from_f32<T>(v);
 }
 
 // Weight gradients.  Few and small weights with many rows would leave most of the chip idle: then (SPLIT) the experts' rows are cut into
@@ -377,32 +405,45 @@ bool sizes_ok(int64_t M, int E, int64_t n_in, int64_t n_out) {
 constexpr int kCompute = 256;  // compute units
 
 // What a step of k (128 bytes of it) of a 64, 128 or 256 tile was measured to take, us: of its compute unit's time (the reads from the L2; in fp32
-// the matrix instructions), and at least from its start to its end
+// the matrix instructions, of which 256 would spare none), and at least from its start to its end
 struct StepCost {
+  int sizes;
   double busy[3], least[3];
 };
 StepCost step_cost(int dtype) {
-  if (dtype == kF32) return {{0.47, 1.75, 7.0}, {0.8, 1.75, 7.0}};
-  return {{0.27, 0.73, 2.1}, {0.45, 0.8, 2.1}};
+  if (dtype == kF32) return {2, {0.47, 1.75}, {0.8, 1.75}};
+  return {3, {0.27, 0.73, 2.1}, {0.45, 0.8, 2.1}};
 }
 
 // Tile sizes: the cheapest by these, of those that an expert's share of the rows fills for the most part (bf16: 65536 rows, 32 experts of 2048 x
 // 1024 with 256 316 us, with 128 375; 16384, 8 of 1024 x 1024 35 and 42; 128 rows each, 64 experts of 1024 x 1024 with 128 28 us, with 64 32; 64
 // rows each, 512 x 512 11.2 and 9.4; fp32, 740 rows, 3 of 495 -> 80 with 128 45, with 64 20).
-int linear_tile(int64_t rows, int64_t groups, int64_t cols, int dtype) {
+// Few tiles and a long k: k is shared out over as many workgroups per tile as two per compute unit allow, of at least four steps, where that
+// saves more than 7 us, the second launch's and its way through the memory (1 row, 2048 -> 2048 bf16 13.0 -> 8.1 us, 4096 -> 64 fp32 87 -> 10).
+struct LinearPlan {
+  int tile, parts;
+};
+LinearPlan linear_plan(int64_t rows, int64_t groups, int64_t cols, int64_t k, int dtype) {
   const StepCost cost = step_cost(dtype);
   const int64_t each = rows / groups;
-  int best = 64;
+  LinearPlan best{64, 1};
   double best_us = 1e30;
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < cost.sizes; ++i) {
     const int tile = 64 << i;
     if (i > 0 && (cols <= tile / 2 || each * 4 < tile * 3)) break;
     const double shared = ((double)rows / tile + 0.5 * groups) * (double)((cols + tile - 1) / tile) / kCompute;  // tiles per compute unit
     const double us = cost.busy[i] * shared > cost.least[i] ? cost.busy[i] * shared : cost.least[i];
-    if (us <= best_us) best = tile, best_us = us;
+    if (us <= best_us) best.tile = tile, best_us = us;
+  }
+  if (best.tile == 64) {
+    const int step = dtype == kF32 ? 32 : 64;
+    const int64_t tiles = row_tiles_at_most(rows, (int)groups, 64) * ((cols + 63) / 64), steps = (k + step - 1) / step;
+    const int64_t room = tiles > 0 ? 2 * kCompute / tiles : 0, parts = room < steps / 4 ? room : steps / 4;
+    if (parts > 1 && (double)(steps - steps / parts) * cost.least[0] > 7.0) best.parts = (int)parts;
   }
   return best;
 }
+int64_t share_bytes(const LinearPlan& p, int64_t rows, int64_t cols) { return p.parts > 1 ? (p.parts * rows * cols * 4 + 255) & ~(int64_t)255 : 0; }
 
 template <typename K>
 void allow_lds(K* kernel, int bytes) {
@@ -438,15 +479,15 @@ Rows packed(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype, ch
   return {copy, padded(cols, dtype)};
 }
 
-template <typename T, int B, int WM, int WN, bool W_RC>
-int launch_linear_tile(const Rows& x, const Rows& w, int w_rows, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, void* y,
+template <typename T, int B, int WM, int WN, bool W_RC, bool SHARED>
+int launch_linear_tile(const Rows& x, const Rows& w, int w_rows, const void* bias, const int32_t* offsets, int64_t M, int E, int N, int K, int parts, void* y,
                        hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t blocks = xcd_blocks(row_tiles_at_most(M, E, B) * ((N + B - 1) / B) + 1);
+  const int64_t blocks = xcd_blocks(row_tiles_at_most(M, E, B) * ((N + B - 1) / B) * parts + 1);
   PS_REQUIRE(blocks * 64 * WM * WN < kMaxThreads, "ps_expert_linear: too many tiles");
-  allow_lds(linear_kernel<T, B, B, WM, WN, W_RC>, lds);
-  linear_kernel<T, B, B, WM, WN, W_RC><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)x.p, x.ld, (const T*)w.p, w.ld, w_rows, (const T*)bias, offsets,
-                                                                                  M, E, N, K, (T*)y);
+  allow_lds(linear_kernel<T, B, B, WM, WN, W_RC, SHARED>, lds);
+  linear_kernel<T, B, B, WM, WN, W_RC, SHARED><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>(
+      (const T*)x.p, x.ld, (const T*)w.p, w.ld, w_rows, (const T*)bias, offsets, M, E, N, K, parts, (std::conditional_t<SHARED, float, T>*)y);
   PS_CHECK_LAUNCH();
 }
 
@@ -456,15 +497,21 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
                   int dtype, void* y, void* workspace, hipStream_t s) {
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
-    char* to = (char*)workspace;
     const int64_t k = W_RC ? n_out : n_in;
-    const Rows xs = packed<T>(x, ldx, M, k, dtype, &to, s), ws = packed<T>(weight, n_in, E * n_out, n_in, dtype, &to, s);
     const int N = (int)(W_RC ? n_in : n_out), K = (int)padded(k, dtype), rows = (int)n_out;
-    switch (linear_tile(M, E, N, dtype)) {
-      case 256: return launch_linear_tile<T, 256, 2, 4, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
-      case 128: return launch_linear_tile<T, 128, 2, 2, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
-      default: return launch_linear_tile<T, 64, 2, 2, W_RC>(xs, ws, rows, bias, offsets, M, E, N, K, y, s);
+    const LinearPlan p = linear_plan(M, E, N, k, dtype);
+    char* to = (char*)workspace + share_bytes(p, M, N);
+    const Rows xs = packed<T>(x, ldx, M, k, dtype, &to, s), ws = packed<T>(weight, n_in, E * n_out, n_in, dtype, &to, s);
+    if (p.parts > 1) {
+      const int rc = launch_linear_tile<T, 64, 2, 2, W_RC, true>(xs, ws, rows, bias, offsets, M, E, N, K, p.parts, workspace, s);
+      if (rc != 0) return rc;
+      linear_join_kernel<T><<<(unsigned)((M * N + 255) / 256), 256, 0, s>>>((const float*)workspace, p.parts, offsets, E, M, N, (T*)y);
+      PS_CHECK_LAUNCH();
     }
+    if constexpr (sizeof(T) == 2)
+      if (p.tile == 256) return launch_linear_tile<T, 256, 2, 4, W_RC, false>(xs, ws, rows, bias, offsets, M, E, N, K, 1, y, s);
+    if (p.tile == 128) return launch_linear_tile<T, 128, 2, 2, W_RC, false>(xs, ws, rows, bias, offsets, M, E, N, K, 1, y, s);
+    return launch_linear_tile<T, 64, 2, 2, W_RC, false>(xs, ws, rows, bias, offsets, M, E, N, K, 1, y, s);
   });
 }
 
@@ -474,7 +521,7 @@ struct DwPlan {
   int64_t units;
 };
 // The cheapest by the tiles' steps.  Pieces shorten the longest run of steps and cost 5 us and the way of their fp32 sums through the memory,
-// 4.5 TB/s; without them an expert may well have twice its share of the rows.  (fp32: tiles of 256 gain nothing.)
+// 4.5 TB/s; without them an expert may well have twice its share of the rows.
 //     16 experts, fp32:  131072 rows of 64 x 64 in pieces 22 us, whole 191 | 32768 rows of 128 x 128 in pieces, tiles of 64 21, of 128 30
 //     bf16:  8192 rows, 16 experts of 512 x 512 whole 12, in pieces 45 | 65536 rows, 32 experts of 2048 x 1024 tiles of 256 307, of 128 374
 DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
@@ -483,7 +530,7 @@ DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
   const int64_t least = n_in < n_out ? n_in : n_out, step_rows = wide ? 32 : 64, each = M / E;
   DwPlan best{64, 0, E};
   double best_us = 1e30;
-  for (int i = 0; i < (wide ? 2 : 3); ++i) {
+  for (int i = 0; i < cost.sizes; ++i) {
     const int tile = 64 << i;
     if (i > 0 && least <= tile / 2) break;
     const double tiles = (double)((n_in + tile - 1) / tile) * ((n_out + tile - 1) / tile);
@@ -537,7 +584,8 @@ enum Pass { kForward, kInputGradient, kWeightGradient };
 int64_t workspace_of(int pass, const void* a, int64_t a_stride, const void* b, int64_t b_stride, int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
   if (pass == kWeightGradient)
     return dw_part_bytes(dw_plan(M, E, n_in, n_out, dtype), n_in, n_out) + pack_bytes(a, a_stride, M, n_out, dtype) + pack_bytes(b, b_stride, M, n_in, dtype);
-  return pack_bytes(a, a_stride, M, pass == kForward ? n_in : n_out, dtype) + pack_bytes(b, n_in, E * n_out, n_in, dtype);
+  const int64_t k = pass == kForward ? n_in : n_out, n = pass == kForward ? n_out : n_in;
+  return share_bytes(linear_plan(M, E, n, k, dtype), M, n) + pack_bytes(a, a_stride, M, k, dtype) + pack_bytes(b, n_in, E * n_out, n_in, dtype);
 }
 
 }  // namespace

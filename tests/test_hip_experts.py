@@ -406,6 +406,15 @@ def test_linear_of_many_experts(dev, M, E, kind, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,E,n_in,n_out,kind", [(1, 1, 4096, 130, "one"), (5, 2, 2100, 70, "ragged"), (217, 9, 1789, 667, "ragged"), (7, 3, 60, 5000, "even"),
+                                                 (30, 4, 2048, 2049, "ragged"), (16, 3, 2000, 64, "nobody")])
+def test_linear_of_few_rows_and_long_sums(dev, M, E, n_in, n_out, kind, dtype):
+    """sums that are shared out over workgroups and joined, forward and in the rows' gradient"""
+    check_linear(dev, M, E, n_in, n_out, dtype, kind, bias=True)
+
+
+@pytest.mark.gpu
 def test_linear_of_rows_far_apart(dev):
     """rows more than 2^20 elements apart are copied first"""
     x = torch.zeros(5, (1 << 20) + 4, device=dev)
