@@ -368,22 +368,29 @@ __global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ 
   }
 }
 
-// (5003 x 385 fp16: 4 us)
-// rows of `cols` elements `ld` apart -> rows of whole 16-byte chunks, zeros behind the last element
+// rows of `cols` elements `ld` apart -> rows of whole 16-byte chunks, zeros behind the last element (5003 x 385 fp16: 4 us); two operands at once
 template <typename T>
-__global__ __launch_bounds__(256) void pack_rows_kernel(const T* __restrict__ src, int64_t ld, int64_t rows, int cols, T* __restrict__ dst) {
-  const int across = (cols + kChunk<T> - 1) / kChunk<T>;
-  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < rows * across; id += (int64_t)gridDim.x * 256) {
-    const int64_t row = id / across;
-    const int c = (int)(id % across) * kChunk<T>;
+struct PackJob {
+  const T* src;
+  int64_t ld, chunks;  // chunks: of all rows
+  int cols, across;    // across: chunks of a row
+  T* dst;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(PackJob<T> a, PackJob<T> b) {
+  for (int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x; id < a.chunks + b.chunks; id += (int64_t)gridDim.x * 256) {
+    const PackJob<T>& job = id < a.chunks ? a : b;
+    const int64_t at = id < a.chunks ? id : id - a.chunks, row = at / job.across;
+    const int c = (int)(at % job.across) * kChunk<T>;
+    const T* src = job.src + row * job.ld + c;
     Pack<T, kChunk<T>> o;
-    if (c + kChunk<T> <= cols) {
-      o = load_any<T, kChunk<T>>(src + row * ld + c);
+    if (c + kChunk<T> <= job.cols) {
+      o = load_any<T, kChunk<T>>(src);
     } else {
 #pragma unroll
-      for (int q = 0; q < kChunk<T>; ++q) o.v[q] = c + q < cols ? src[row * ld + c + q] : from_f32<T>(0.0f);
+      for (int q = 0; q < kChunk<T>; ++q) o.v[q] = c + q < job.cols ? src[q] : from_f32<T>(0.0f);
     }
-    store_pack(dst + id * kChunk<T>, o);
+    store_pack(job.dst + at * kChunk<T>, o);
   }
 }
 
@@ -467,16 +474,23 @@ bool is_packed(const void* p, int64_t ld, int64_t cols, int dtype) {
 int64_t pack_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype) {
   return is_packed(p, ld, cols, dtype) ? 0 : (rows * padded(cols, dtype) * size_of(dtype) + 255) & ~(int64_t)255;
 }
-// the operand itself, or its copy at *to, which moves on
+// two operands as they are, or their copies from `to` on
+struct Operand {
+  const void* p;
+  int64_t ld, rows, cols;
+};
 template <typename T>
-Rows packed(const void* p, int64_t ld, int64_t rows, int64_t cols, int dtype, char** to, hipStream_t s) {
-  const int64_t bytes = pack_bytes(p, ld, rows, cols, dtype);
-  if (bytes == 0) return {p, ld};
-  T* copy = (T*)*to;
-  *to += bytes;
-  const int64_t chunks = rows * (padded(cols, dtype) / kChunk<T>);
-  if (chunks > 0) pack_rows_kernel<T><<<blocks_of_256(chunks), 256, 0, s>>>((const T*)p, ld, rows, (int)cols, copy);
-  return {copy, padded(cols, dtype)};
+void packed(const Operand& a, const Operand& b, int dtype, char* to, Rows* as, Rows* bs, hipStream_t s) {
+  auto job = [&](const Operand& o, Rows* r) {
+    const int64_t bytes = pack_bytes(o.p, o.ld, o.rows, o.cols, dtype);
+    const int across = (int)(padded(o.cols, dtype) / kChunk<T>);
+    PackJob<T> j{(const T*)o.p, o.ld, bytes == 0 ? 0 : o.rows * across, (int)o.cols, across, (T*)to};
+    *r = bytes == 0 ? Rows{o.p, o.ld} : Rows{to, padded(o.cols, dtype)};
+    to += bytes;
+    return j;
+  };
+  const PackJob<T> ja = job(a, as), jb = job(b, bs);
+  if (ja.chunks + jb.chunks > 0) pack_rows_kernel<T><<<blocks_of_256(ja.chunks + jb.chunks), 256, 0, s>>>(ja, jb);
 }
 
 template <typename T, int B, int WM, int WN, bool W_RC, bool SHARED>
@@ -500,8 +514,8 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
     const int64_t k = W_RC ? n_out : n_in;
     const int N = (int)(W_RC ? n_in : n_out), K = (int)padded(k, dtype), rows = (int)n_out;
     const LinearPlan p = linear_plan(M, E, N, k, dtype);
-    char* to = (char*)workspace + share_bytes(p, M, N);
-    const Rows xs = packed<T>(x, ldx, M, k, dtype, &to, s), ws = packed<T>(weight, n_in, E * n_out, n_in, dtype, &to, s);
+    Rows xs, ws;
+    packed<T>({x, ldx, M, k}, {weight, n_in, E * n_out, n_in}, dtype, (char*)workspace + share_bytes(p, M, N), &xs, &ws, s);
     if (p.parts > 1) {
       const int rc = launch_linear_tile<T, 64, 2, 2, W_RC, true>(xs, ws, rows, bias, offsets, M, E, N, K, p.parts, workspace, s);
       if (rc != 0) return rc;
@@ -629,8 +643,8 @@ extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void
   return by_type(dtype, [&](auto zero) {
     using T = decltype(zero);
     float* parts = (float*)workspace;
-    char* to = (char*)workspace + dw_part_bytes(p, n_in, n_out);
-    const Rows dys = packed<T>(dy, dy_stride, M, n_out, dtype, &to, s), xs = packed<T>(x, x_stride, M, n_in, dtype, &to, s);
+    Rows dys, xs;
+    packed<T>({dy, dy_stride, M, n_out}, {x, x_stride, M, n_in}, dtype, (char*)workspace + dw_part_bytes(p, n_in, n_out), &dys, &xs, s);
     if (p.piece == 0) return launch_dw<T, false>(p, dys, xs, offsets, M, E, N, K, K, dweight, dbias, s);
     float* db_parts = parts + p.units * n_out * ldo;
     const int rc = launch_dw<T, true>(p, dys, xs, offsets, M, E, N, K, ldo, parts, dbias != nullptr ? db_parts : nullptr, s);
