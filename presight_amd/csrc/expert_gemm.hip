@@ -120,7 +120,7 @@ __device__ __forceinline__ void direct_loop(char* lds, int K, const DirectSource
   if (K <= 0) return;
   sa.load(0, lds);
   sb.load(0, lds + BM * kTileRowBytes);
-  __syncthreads();
+  tile_barrier<0>();
   for (int k0 = 0, cur = 0; k0 < K; k0 += BK, cur ^= 1) {
     char* a = lds + cur * kStage;
     if (k0 + BK < K) {
@@ -145,7 +145,7 @@ __device__ __forceinline__ void direct_loop(char* lds, int K, const DirectSource
           for (int i = 0; i < MI; ++i) row_sums[i] = mma_block<T>(fa[i], ones, row_sums[i]);
       }
     }
-    __syncthreads();
+    tile_barrier<0>();
   }
 }
 
@@ -206,7 +206,7 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
 
 // What bounds it depends on the rows per expert.  16 rows of 16 experts' 1024 x 2048 bf16: the weights' 67 MB, 13.4 us, 5.0 TB/s.  131072 rows of 64
 // fp32, 16 experts: the rows' 67 MB and the launch, 21 us.  65536 rows, 2048 x 1024 bf16, 32 experts: the compute units' reads from the
-// L2 and the power limit (a tenth less time on zeros): 303 us forward, 383 for the input gradient, 907 and 718 TFLOP/s.  (The experts' last,
+// L2 and the power limit (a tenth less time on zeros): 300 us forward, 306 for the input gradient, 916 and 898 TFLOP/s.  (The experts' last,
 // incomplete tiles in a round of their own behind the whole ones, and lines fetched into the L2 two to eight steps of k ahead, were slower.)
 // y[p] = sum_k x[p][k] W(n,k) (+ bias).  W_RC = false: the weight's rows are k-contiguous (forward), n of them; true: n-contiguous (input
 // gradient), `w_rows` of them.  K: the rows' length in whole chunks.
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
 // pieces of `piece` rows, whoever they belong to, every piece writes its own fp32 sums [unit][out][in] (and [unit][out]), and
 // dw_join_kernel adds up the pieces of each expert in order.  Also shorter sums: a piece rounds `piece` / 4 times where the whole
 // column would round a hundred times as often.
-// 65536 rows, 2048 x 1024 bf16, 32 experts (whole): 326 us, 843 TFLOP/s; 131072 rows of 64 x 64 fp32, 16 experts (pieces): 21 us and 5 to join.
+// 65536 rows, 2048 x 1024 bf16, 32 experts (whole): 258 us, 1065 TFLOP/s; 131072 rows of 64 x 64 fp32, 16 experts (pieces): 21 us and 5 to join.
 template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
                                                                         const int* __restrict__ offsets, int64_t M, int E, int N, int K, int ldo, int piece,

@@ -31,6 +31,19 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t window(const void* base, int64
   return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(lo | (hi << 32)), 0, uniform(n), 0x00027000);
 }
 
+// The transposing LDS load.  Without what __restrict__ says here of this one read the compiler takes it to read what the loads under way
+// write, and waits for all of them first (the tiles' barriers see to it that they have landed): 65536 rows of 32 experts 2048 x 1024 bf16, input
+// gradient 364 us for 306, weights' 304 for 258.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 LdsShorts;
+__device__ __forceinline__ u32x2 turned_read(LdsShorts* __restrict__ p) {
+#ifdef __HIP_DEVICE_COMPILE__  // (the host pass drops a kernel's stub over a builtin it does not know)
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(p));
+#else
+  return u32x2{};
+#endif
+}
+
 // ------------------------------------------------------------------------------------------------ tiles loaded straight into LDS
 // Operands need no registers on the way: buffer loads write LDS directly, 1 KiB per wave and instruction in lane order.  A tile holds 128
 // bytes of k and keeps the operand's own direction: KC as rows of k, RC as rows of BR elements of one k each, from which 16-bit fragments
@@ -90,17 +103,12 @@ struct DirectTile {
       }
       return v;
     } else {
-      typedef short s16x4 __attribute__((ext_vector_type(4)));
       u32x4 v;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int k = s * 32 + g * 8 + h * 4 + (r >> 2);
         const char* p = lds + k * kRow + ((((r0 >> 3) + ((r & 3) >> 1)) ^ spread(k)) << 4) + (r & 1) * 8;
-#ifdef __HIP_DEVICE_COMPILE__  // (the host pass drops a kernel's stub over a builtin it does not know)
-        const u32x2 o = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
-#else
-        const u32x2 o = *reinterpret_cast<const u32x2*>(p);
-#endif
+        const u32x2 o = turned_read((LdsShorts*)p);
         v[2 * h] = o[0];
         v[2 * h + 1] = o[1];
       }

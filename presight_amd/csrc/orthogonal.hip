@@ -346,7 +346,7 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] += from[(i * NJ + j) * NT];
   }
-  __syncthreads();
+  tile_barrier<0>();  // (no load is left on its way into LDS)
   const float ratio = ratio_at(start_ratio, step, c.grow);
   // kPoly: a + b r^2 S^ + c r^4 S^ S^ with the coefficients as pairs of floats: an error of a coefficient would be common to all entries and
   // grow like a singular value's | kApply: over the step's growth of r | kLast: X = r X^
