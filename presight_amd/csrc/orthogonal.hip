@@ -201,11 +201,10 @@ struct Operands {  // pairs
 // A workgroup's tile: BM x BN; a stage is 32 k of both planes of either operand, one tile row of 128 bytes for a row of k (KC).  A compute
 // unit can have about 17 bytes per cycle of the L2's in flight, so the tile decides how fast the matrix instructions are fed: at their full
 // rate 256 x 128 asks for 32 bytes per cycle, 128 x 128 for 43 and 64 x 64 for 85, and a step of k takes as long as its stage of 48, 32 or
-// 16 KiB takes to arrive.
-// The two small products add up apart from the large one: each of their additions to it would cost it another rounding.
+// 16 KiB takes to arrive.  The two small products add up apart from the large one: each of their additions to it would cost it another rounding.
 //
-// 2048 x 4096: S 90 us, a I + b S + c S S 56, times X 115: 573, 464 and 897 TFLOP/s of pairs' products (half of S and S S by symmetry, three
-// products per pair), where a large fp16 product reaches 1463; 8 x 1024 x 2048: 87, 62 and 122 us.  A few tiles:
+// 2048 x 4096: S 89 us, a I + b S + c S S 57, times X 97: 580, 452 and 1063 TFLOP/s of pairs' products (half of S and S S by symmetry, three
+// products per pair), where a large fp16 product reaches 1463; 8 x 1024 x 2048: 86, 64 and 106 us.  A few tiles:
 // 3 x 385 x 129 takes 7 to 9 us a product, most of it the launch, the first loads from memory that another XCD wrote, and the way out.
 //
 // The result leaves through LDS as rows of whole lines.  Of a symmetric one only what lies on and below the diagonal's BN x BN blocks is
@@ -296,38 +295,38 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
 #pragma unroll
       for (int j = 0; j < NJ; ++j) early[0][i][j] = gram_at(i, j, 0), early[1][i][j] = gram_at(i, j, 1);
   if constexpr (PART != kJoin) {
-  __builtin_assume(first < end);  // (no way past the loop to prepare for: 3 x 385 x 129 124 -> 121 us)
+    __builtin_assume(first < end);  // (no way past the loop to prepare for: 3 x 385 x 129 124 -> 121 us)
 #pragma unroll
-  for (int i = 0; i < kStages - kGroup; ++i) load(first + i);
-  for (int i = first; i < end; i += kGroup) {
-    tile_barrier<(kStages - 2 * kGroup) * kLoads>();
+    for (int i = 0; i < kStages - kGroup; ++i) load(first + i);
+    for (int i = first; i < end; i += kGroup) {
+      tile_barrier<(kStages - 2 * kGroup) * kLoads>();
 #pragma unroll
-    for (int u = 0; u < kGroup; ++u) load(i + u + kStages - kGroup);  // (where the stages before i were; zeros behind the last)
+      for (int u = 0; u < kGroup; ++u) load(i + u + kStages - kGroup);  // (where the stages before i were; zeros behind the last)
 #pragma unroll
-    for (int u = 0; u < kGroup; ++u) {
-      const char* t = lds + (i + u) % kStages * kStage;
-      u32x4 fa[2][MI], fb[2][NJ];
+      for (int u = 0; u < kGroup; ++u) {
+        const char* t = lds + (i + u) % kStages * kStage;
+        u32x4 fa[2][MI], fb[2][NJ];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
+        for (int p = 0; p < 2; ++p) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int n = wn + j * 16;
-          fb[p][j] = kSymmetric ? decltype(sb.tile)::fragment(t + BM * kTileRowBytes, n, p)
-                                : decltype(sb.tile)::fragment(t + BM * kTileRowBytes, (int)pair_at(n, p), 0);
+          for (int j = 0; j < NJ; ++j) {
+            const int n = wn + j * 16;
+            fb[p][j] = kSymmetric ? decltype(sb.tile)::fragment(t + BM * kTileRowBytes, n, p)
+                                  : decltype(sb.tile)::fragment(t + BM * kTileRowBytes, (int)pair_at(n, p), 0);
+          }
+#pragma unroll
+          for (int q = 0; q < MI; ++q) fa[p][q] = decltype(sa.tile)::fragment(t, wm + q * 16, p);
         }
 #pragma unroll
-        for (int q = 0; q < MI; ++q) fa[p][q] = decltype(sa.tile)::fragment(t, wm + q * 16, p);
+        for (int q = 0; q < MI; ++q)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            acc[q][j] = mma_block<_Float16>(fa[0][q], fb[0][j], acc[q][j]);
+            fine[q][j] = mma_block<_Float16>(fa[0][q], fb[1][j], fine[q][j]);
+            fine[q][j] = mma_block<_Float16>(fa[1][q], fb[0][j], fine[q][j]);
+          }
       }
-#pragma unroll
-      for (int q = 0; q < MI; ++q)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          acc[q][j] = mma_block<_Float16>(fa[0][q], fb[0][j], acc[q][j]);
-          fine[q][j] = mma_block<_Float16>(fa[0][q], fb[1][j], fine[q][j]);
-          fine[q][j] = mma_block<_Float16>(fa[1][q], fb[0][j], fine[q][j]);
-        }
     }
-  }
   }
   if constexpr (PART == kShare) {
     f32x4* mine = w.shares + ((int64_t)(part * batches + batch) * tiles + place % tiles) * (NT * MI * NJ) + threadIdx.x;
@@ -469,8 +468,8 @@ int64_t product_tiles(int bm, int ra, int rb, bool symmetric) {
 }
 
 // How a product is cut: the cheapest of what a step of k of a round of tiles, one per compute unit, takes: .42 us (64 x 64, of which two or more
-// share a compute unit; alone .55), .95 (128 x 128) or 1.65 (256 x 128).  All five steps: 2048 x 4096 with tiles of 256 and 128 1236 us, 128
-// alone about 1330, 64 alone 1489; 1024 x 1024 with 64 273, with 128 479; 300 x 128 x 128 with 64 269, with 256 499.  Then the parts of k
+// share a compute unit; alone .55), .95 (128 x 128) or 1.65 (256 x 128).  All five steps: 2048 x 4096 with tiles of 256 and 128 1236 us, 64 alone
+// 1489; 1024 x 1024 with 64 273, with 128 479; 300 x 128 x 128 with 64 269, with 256 499.  Then the parts of k
 // of S: as many as two workgroups per compute unit allow, where they save more steps than they and the second launch cost (1024 x 1024,
 // 22 of 32 steps saved: 266 -> 278).
 struct ProductPlan {
