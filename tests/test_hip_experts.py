@@ -580,6 +580,32 @@ def test_captured_and_replayed(dev, dtype, N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_few_rows_captured(dev, dtype):
+    """sums shared out over workgroups, in two graphs that are replayed in turn with eager calls between them: the eager bits"""
+    T = TYPES[dtype]
+    g = torch.Generator().manual_seed(21)
+    w = [torch.randn(3, 130, n, generator=g).to(T).to(dev) for n in (4096, 2051)]
+    x = [torch.zeros(5, n, device=dev, dtype=T) for n in (4096, 2051)]
+    offsets = [torch.zeros(4, device=dev, dtype=torch.int32) for _ in x]
+    for a in zip(x, w, offsets):
+        experts.expert_linear(a[0], a[1], None, a[2])
+    graphs, out = [torch.cuda.CUDAGraph() for _ in x], []
+    for i, graph in enumerate(graphs):
+        with torch.cuda.graph(graph):
+            out.append(experts.expert_linear(x[i], w[i], None, offsets[i]))
+    for replay in range(4):
+        for i, graph in enumerate(graphs):
+            x[i].copy_(torch.randn(x[i].shape, generator=g).to(T))
+            offsets[i].copy_(torch.tensor([0, replay, 3, 3 + replay % 3], dtype=torch.int32))
+            graph.replay()
+        eager = [experts.expert_linear(x[i], w[i], None, offsets[i]) for i in range(2)]
+        torch.cuda.synchronize()
+        for kept, now, n in zip(out, eager, range(2)):
+            assert torch.equal(kept, now) and not now[3 + replay % 3:].any() and now[:1].any()
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once(dev):
     """two chains of different inputs side by side on two streams give what they give alone"""
     g = torch.Generator().manual_seed(8)

@@ -312,6 +312,23 @@ def test_muon_state_and_refusals(dev):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(3, 70, 3000), (12, 600, 700)])
+def test_newton_schulz_captured(dev, shape):
+    g = torch.Generator().manual_seed(17)
+    x = torch.randn(shape, generator=g).to(dev)
+    optim.newton_schulz(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = optim.newton_schulz(x)
+    for _ in range(3):
+        x.copy_(torch.randn(shape, generator=g))
+        graph.replay()
+        eager = optim.newton_schulz(x)
+        torch.cuda.synchronize()
+        assert torch.equal(y, eager)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shapes", [[(16, 64, 40), (3, 64)], [(2, 200, 300)]])
 def test_muon_captured(dev, shapes):
     """a captured step, replayed on new gradients with eager work in between, walks the eager path bit for bit"""
