@@ -14,7 +14,7 @@ import torch
 from ._lib import check, lib
 from .dist import intersect_ranges
 from .experts import DTYPE_CODES, _gpu, _on, _typed
-from .ops import _p, _stream
+from .ops import _p, _stream, join_side_streams
 
 
 class HipAdam:
@@ -334,6 +334,15 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
     return out
 
 
+def _with_gradients(params: Sequence[torch.nn.Parameter]) -> List[int]:
+    """indices of the parameters that have received a gradient.  Gradients written in place (FlatGrads) may still be on their way on a
+    side stream, which autograd does not see: the current stream waits for it first."""
+    held = [i for i, p in enumerate(params) if p.grad is not None]
+    if any(getattr(params[i], "_ps_direct_grad", False) for i in held):
+        join_side_streams()
+    return [i for i in held if not getattr(params[i], "_ps_direct_grad", False) or params[i]._ps_touched]
+
+
 class HipMuon:
     """Momentum with an orthogonalised update, for weight matrices [out, in] and stacks of them [experts, out, in] (embeddings, hash
     tables, biases and output scalars belong to HipAdam):
@@ -374,10 +383,9 @@ class HipMuon:
     def step(self) -> None:
         self.step_count += 1
         by_device: dict = {}
-        for p, buf in zip(self.params, self.momentum_buffers):
+        for i in _with_gradients(self.params):
+            p, buf = self.params[i], self.momentum_buffers[i]
             g = p.grad
-            if g is None or (getattr(p, "_ps_direct_grad", False) and not p._ps_touched):
-                continue
             if getattr(p, "_ps_group", None) is not None:
                 raise RuntimeError("HipMuon: whether this parameter has a gradient is decided on the device; it belongs to HipAdam")
             if p.device != buf.device or not p.is_contiguous() or p.dtype != torch.float32 or p.shape != buf.shape:

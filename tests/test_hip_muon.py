@@ -394,3 +394,47 @@ def test_experts_trained_by_muon(dev):
         # the gradient's relative error (sums of about 170 rows of about 100 terms) grows by at most the polynomial's slope per step
         slack = rate * 4 ** 5 * (N + D + H) * 2.0 ** -23 * math.sqrt(E * 40) + 4 * 2.0 ** -24 * float(new.norm())
         assert float((p.detach().cpu().double() - new).norm()) <= slack
+
+
+# ------------------------------------------------------------------------------------------------ gradients that live in a FlatGrads
+def test_step_waits_for_gradients_written_on_side_streams(monkeypatch):
+    """gradients of a FlatGrads are written in place, some of them on the proposal networks' side stream: it is joined before any is read"""
+    from presight_amd.dist import FlatGrads
+
+    joins = []
+    monkeypatch.setattr(optim, "join_side_streams", lambda: joins.append(1))
+    plain, held = torch.nn.Parameter(torch.zeros(4, 5)), [torch.nn.Parameter(torch.zeros(3, 4)) for _ in range(2)]
+    plain.grad = torch.ones(4, 5)
+    assert optim._with_gradients([plain]) == [0] and not joins
+    fg = FlatGrads(held)
+    held[1]._ps_touched = True
+    assert optim._with_gradients([plain] + held) == [0, 2] and len(joins) == 1
+    fg.zero_()
+    assert optim._with_gradients(held) == []
+
+
+@pytest.mark.gpu
+def test_muon_of_gradients_written_on_a_side_stream(dev):
+    from presight_amd import ops
+    from presight_amd.dist import FlatGrads
+
+    g = torch.Generator().manual_seed(18)
+    start, grad = torch.randn(4, 96, 80, generator=g).to(dev), torch.randn(4, 96, 80, generator=g).to(dev)
+    alone, held = torch.nn.Parameter(start.clone()), torch.nn.Parameter(start.clone())
+    alone.grad = grad
+    a, b = optim.HipMuon([alone]), optim.HipMuon([held])
+    fg = FlatGrads([held])
+    busy = torch.randn(4096, 4096, device=dev)
+    side = ops.side_stream(dev)
+    for _ in range(3):
+        a.step()
+        fg.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(20):  # (the write comes late)
+                busy = busy @ busy * 1e-4
+            held.grad.copy_(grad)
+        ops.mark_touched([held])
+        b.step()
+        torch.cuda.synchronize()
+        assert torch.equal(alone, held) and torch.equal(a.momentum_buffers[0], b.momentum_buffers[0])
