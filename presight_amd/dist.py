@@ -21,6 +21,7 @@ during backward) or from finish_exchange (a sub-field without samples on this ra
 from __future__ import annotations
 
 import os
+import weakref
 
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple
 
@@ -134,6 +135,17 @@ def _zero_ranges(flat: torch.Tensor, ranges) -> None:
                                        torch._C._cuda_getCurrentRawStream(flat.device.index)), "ps_zero_ranges")
 
 
+_LIVE_FLAT_GRADS: "weakref.WeakSet" = weakref.WeakSet()
+
+
+def flat_grads_of(p: torch.nn.Parameter) -> Optional["FlatGrads"]:
+    """the FlatGrads whose buffer p.grad is a part of; None where p.grad is a tensor of its own"""
+    if p.grad is None or not getattr(p, "_ps_direct_grad", False):
+        return None
+    at = p.grad.untyped_storage().data_ptr()
+    return next((fg for fg in _LIVE_FLAT_GRADS if fg.flat.untyped_storage().data_ptr() == at), None)
+
+
 class FlatGrads:
     def __init__(self, params: Iterable[torch.nn.Parameter], bucket_sizes: Optional[Sequence[int]] = None, shard_world: int = 1,
                  splits: Optional[Dict[int, int]] = None):
@@ -177,6 +189,7 @@ class FlatGrads:
         self.total = off
         dev = self.params[0].device
         self.flat = torch.zeros(self.total, device=dev, dtype=torch.float32)
+        _LIVE_FLAT_GRADS.add(self)
         for p, o in zip(self.params, self.offsets):
             n = p.numel()
             p.grad = self.flat[o:o + n].view_as(p)

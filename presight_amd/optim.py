@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from ._lib import check, lib
-from .dist import intersect_ranges
+from .dist import flat_grads_of, intersect_ranges
 from .experts import DTYPE_CODES, _gpu, _on, _typed
 from .ops import _p, _stream, join_side_streams
 
@@ -336,11 +336,17 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
 
 def _with_gradients(params: Sequence[torch.nn.Parameter]) -> List[int]:
     """indices of the parameters that have received a gradient.  Gradients written in place (FlatGrads) may still be on their way on a
-    side stream, which autograd does not see: the current stream waits for it first."""
+    side stream, which autograd does not see: the current stream waits for it first.  A sharded exchange leaves no rank with a whole
+    matrix's averaged gradient: refused."""
     held = [i for i, p in enumerate(params) if p.grad is not None]
-    if any(getattr(params[i], "_ps_direct_grad", False) for i in held):
+    direct = {i for i in held if getattr(params[i], "_ps_direct_grad", False)}
+    for fg in {flat_grads_of(params[i]) for i in direct} - {None}:
+        if fg.mode == "sharded" and fg._distributed() and fg._rank_world()[1] > 1:
+            raise RuntimeError("HipMuon: in the sharded exchange a rank holds the averaged gradient of its shard only, and this update needs "
+                               "whole matrices: exchange with mode='allreduce'")
+    if direct:
         join_side_streams()
-    return [i for i in held if not getattr(params[i], "_ps_direct_grad", False) or params[i]._ps_touched]
+    return [i for i in held if i not in direct or params[i]._ps_touched]
 
 
 class HipMuon:
@@ -354,7 +360,8 @@ class HipMuon:
     Parameters are contiguous fp32; one without a gradient is skipped, its momentum included.  lr may be changed between steps; a captured
     step keeps the lr, weight_decay and set of parameters it was captured with.
     Gradients held by a FlatGrads are read where it keeps them (a parameter counts as without a gradient until the backward pass has
-    reached it); parameters of its device-decided groups are refused."""
+    reached it); parameters of its device-decided groups and gradients of its sharded exchange (a rank has its shard of a matrix only) are
+    refused."""
 
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, ns_steps: int = 5, ns_coefficients: Tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7,

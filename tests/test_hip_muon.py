@@ -7,6 +7,10 @@ but sum the same fp32 way: each of a step's three stored results (S, a + b S + c
 each of the three products a dropped term of 2^-24, so at most four times the unit that the plain form rounds with: 4 x its distance.  A
 matrix for which that distance happens to be tiny gets 16 * 2^-24 of its norm instead.  The result's own rounding comes on top."""
 import math
+import os
+import subprocess
+import sys
+import textwrap
 
 import pytest
 import torch
@@ -438,3 +442,53 @@ def test_muon_of_gradients_written_on_a_side_stream(dev):
         b.step()
         torch.cuda.synchronize()
         assert torch.equal(alone, held) and torch.equal(a.momentum_buffers[0], b.momentum_buffers[0])
+
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+_HEAD = """
+    import sys, torch, torch.distributed as dist
+    sys.path.insert(0, {root!r})
+    from presight_amd import optim
+    from presight_amd.dist import FlatGrads, init_from_env
+    rank, local, world = init_from_env("cpu")
+    params = [torch.nn.Parameter(torch.zeros(4, 8)) for _ in range(3)]
+"""
+_TAIL = """
+    dist.barrier(); dist.destroy_process_group()
+    print("rank", rank, "ok")
+"""
+_SHARDED = """
+    fg = FlatGrads(params, bucket_sizes=[1, 2], shard_world=world)
+    assert optim._with_gradients(params) == []  # (nothing is exchanged yet)
+    fg.enable_overlap([params[:1], params[1:]], mode="sharded")
+    fg.zero_()
+    sum(p.sum() * (rank + 1.0) for p in params).backward()
+    fg.finish_exchange()
+    try:
+        optim._with_gradients(params)
+        raise SystemExit("gradients that are averaged in shards must be refused")
+    except RuntimeError as e:
+        assert "sharded" in str(e)
+    own = torch.nn.Parameter(torch.zeros(4, 8))
+    own.grad = torch.ones(4, 8)
+    assert optim._with_gradients([own]) == [0]
+    fg = FlatGrads(params)  # a new buffer takes the gradients over
+    fg.enable_overlap([params], mode="allreduce")
+    fg.zero_()
+    sum(p.sum() * (rank + 1.0) for p in params).backward()
+    fg.finish_exchange()
+    assert optim._with_gradients(params) == [0, 1, 2] and all(bool((p.grad == 1.5).all()) for p in params)
+"""
+
+
+def two_ranks(tmp_path, body, port):
+    script = tmp_path / "worker.py"
+    script.write_text("".join(textwrap.dedent(t) for t in (_HEAD, body, _TAIL)).format(root=ROOT))
+    env = dict(os.environ, MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    r = subprocess.run([sys.executable, "-m", "torch.distributed.run", "--nnodes=1", "--nproc-per-node=2", "--master-addr", "127.0.0.1",
+                        "--master-port", str(port), str(script)], capture_output=True, text=True, env=env, timeout=300)
+    assert r.returncode == 0 and r.stdout.count("ok") == 2, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+def test_gradients_averaged_in_shards_are_refused(tmp_path):
+    two_ranks(tmp_path, _SHARDED, 29761)
