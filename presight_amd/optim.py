@@ -335,18 +335,27 @@ def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Tuple[float, fl
 
 
 def _with_gradients(params: Sequence[torch.nn.Parameter]) -> List[int]:
-    """indices of the parameters that have received a gradient.  Gradients written in place (FlatGrads) may still be on their way on a
-    side stream, which autograd does not see: the current stream waits for it first.  A sharded exchange leaves no rank with a whole
-    matrix's averaged gradient: refused."""
+    """indices of the parameters that have received a gradient: of those whose gradient a FlatGrads holds, the ones it counts, which is the
+    same on every rank.  Gradients written in place may still be on their way on a side stream, which autograd does not see: the
+    current stream waits for it first.  A sharded exchange leaves no rank with a whole matrix's averaged gradient: refused."""
     held = [i for i, p in enumerate(params) if p.grad is not None]
-    direct = {i for i in held if getattr(params[i], "_ps_direct_grad", False)}
-    for fg in {flat_grads_of(params[i]) for i in direct} - {None}:
+    direct = [i for i in held if getattr(params[i], "_ps_direct_grad", False)]
+    buffers = {i: flat_grads_of(params[i]) for i in direct}
+    owners = list(dict.fromkeys(fg for fg in buffers.values() if fg is not None))  # (in the parameters' order: touched() may be a collective)
+    for fg in owners:
         if fg.mode == "sharded" and fg._distributed() and fg._rank_world()[1] > 1:
             raise RuntimeError("HipMuon: in the sharded exchange a rank holds the averaged gradient of its shard only, and this update needs "
                                "whole matrices: exchange with mode='allreduce'")
     if direct:
         join_side_streams()
-    return [i for i in held if i not in direct or params[i]._ps_touched]
+    counted = {id(p) for fg in owners for p, touched in zip(fg.params, fg.touched()) if touched}
+
+    def received(i: int) -> bool:
+        if i not in buffers:
+            return True
+        return params[i]._ps_touched if buffers[i] is None else id(params[i]) in counted
+
+    return [i for i in held if received(i)]
 
 
 class HipMuon:

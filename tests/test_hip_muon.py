@@ -492,3 +492,20 @@ def two_ranks(tmp_path, body, port):
 
 def test_gradients_averaged_in_shards_are_refused(tmp_path):
     two_ranks(tmp_path, _SHARDED, 29761)
+
+
+_AGREED = """
+    fg = FlatGrads(params)
+    fg.flags_may_differ_across_ranks = True  # (routing left the middle one without samples on rank 1)
+    fg.zero_()
+    (params[0].sum() + (params[1].sum() * 4.0 if rank == 0 else 0.0)).backward()
+    fg.finish_exchange()
+    assert optim._with_gradients(params) == [0, 1] and bool((params[1].grad == 2.0).all())
+    assert optim._with_gradients(params[1:]) == [0]
+    fg.flags_may_differ_across_ranks = False  # (ranks are known to agree: nothing is asked)
+    assert optim._with_gradients(params) == ([0, 1] if rank == 0 else [0])
+"""
+
+
+def test_ranks_agree_on_who_has_a_gradient(tmp_path):
+    two_ranks(tmp_path, _AGREED, 29763)
