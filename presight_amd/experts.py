@@ -21,6 +21,7 @@ from typing import Optional, Union
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import check, lib
@@ -58,7 +59,10 @@ def _rows(t: Tensor) -> Tensor:
 
 
 def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """whether a call goes through autograd: to be differentiated, or to be refused by it where an input carries a forward-mode tangent"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _once(fn):

@@ -634,3 +634,39 @@ def test_second_derivatives_are_refused(dev):
     (g,) = torch.autograd.grad(experts.expert_dispatch(x, plan).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), x)
+
+
+# ------------------------------------------------------------------------------------------------ forward-mode derivatives
+def test_a_tangent_is_not_dropped():
+    """an input that carries a tangent takes the way through autograd, which refuses it; without one nothing changes"""
+    from torch.autograd import forward_ad
+
+    t = torch.zeros(3, 4)
+    assert not experts._wants_grad(t, None) and experts._wants_grad(t, t.clone().requires_grad_(True))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t, torch.ones_like(t))
+        assert experts._wants_grad(None, dual) and not experts._wants_grad(t, None)
+        with torch.no_grad():
+            assert experts._wants_grad(t, dual)
+    assert not experts._wants_grad(t)
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused(dev):
+    from torch.autograd import forward_ad
+
+    plan = experts.expert_plan(torch.zeros(4, 1, dtype=torch.int64, device=dev), 1)
+    x, w, gates = torch.randn(4, 8, device=dev), torch.randn(1, 6, 8, device=dev), torch.rand(4, 1, device=dev)
+    b = torch.randn(1, 6, device=dev)
+    with forward_ad.dual_level():
+        d = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: experts.expert_dispatch(d(x), plan), lambda: experts.expert_combine(d(x), gates, plan),
+                     lambda: experts.expert_combine(x, d(gates), plan), lambda: experts.expert_combine(d(x), None, plan),
+                     lambda: experts.expert_linear(d(x), w, None, plan), lambda: experts.expert_linear(x, d(w), b, plan),
+                     lambda: experts.expert_linear(x, w, d(b), plan)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+            with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+        y = experts.expert_linear(x, w, b, plan)  # (no tangent: as ever)
+        assert forward_ad.unpack_dual(y).tangent is None
