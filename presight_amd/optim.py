@@ -430,8 +430,9 @@ class HipMuon:
         return {"step": self.step_count, "lr": self.lr, "momentum_buffers": self.momentum_buffers}
 
     def load_state_dict(self, sd):
-        if len(sd["momentum_buffers"]) != len(self.momentum_buffers):
-            raise ValueError("HipMuon: the state holds another number of parameters")
+        here, there = ([tuple(b.shape) for b in bufs] for bufs in (self.momentum_buffers, sd["momentum_buffers"]))
+        if here != there:  # (copy_ would spread a smaller one over a stack)
+            raise ValueError(f"HipMuon: the state is of other parameters: shapes {there} for {here}")
         self.step_count, self.lr = sd["step"], sd["lr"]
         for a, b in zip(self.momentum_buffers, sd["momentum_buffers"]):
             a.copy_(b)

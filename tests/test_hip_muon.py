@@ -509,3 +509,17 @@ _AGREED = """
 
 def test_ranks_agree_on_who_has_a_gradient(tmp_path):
     two_ranks(tmp_path, _AGREED, 29763)
+
+
+# ------------------------------------------------------------------------------------------------ states of other parameters
+def test_state_of_other_shapes_is_refused_whole():
+    """a momentum that would broadcast into a stack, one that fits no buffer, and one too few: refused before anything is taken over"""
+    opt = optim.HipMuon([])
+    opt.momentum_buffers = [torch.zeros(3, 4, 5), torch.zeros(6, 7)]
+    ok = torch.ones(3, 4, 5)
+    for bad in ([torch.ones(4, 5), torch.ones(6, 7)], [torch.ones(1, 4, 5), torch.ones(6, 7)], [ok, torch.ones(7, 6)], [ok, torch.ones(7)], [ok]):
+        with pytest.raises(ValueError, match="other parameters"):
+            opt.load_state_dict({"step": 9, "lr": 0.5, "momentum_buffers": bad})
+    assert opt.step_count == 0 and opt.lr == 0.02 and not any(b.any() for b in opt.momentum_buffers)
+    opt.load_state_dict({"step": 9, "lr": 0.5, "momentum_buffers": [ok, torch.ones(6, 7)]})
+    assert opt.step_count == 9 and opt.lr == 0.5 and all(b.all() for b in opt.momentum_buffers)
