@@ -397,7 +397,6 @@ class HipMuon:
 
     @torch.no_grad()
     def step(self) -> None:
-        self.step_count += 1
         by_device: dict = {}
         for i in _with_gradients(self.params):
             p, buf = self.params[i], self.momentum_buffers[i]
@@ -409,6 +408,7 @@ class HipMuon:
             if g.layout != torch.strided or g.dtype != torch.float32 or g.device != p.device or g.shape != p.shape:
                 raise RuntimeError("HipMuon: gradients must be dense fp32 tensors on their parameter's device")
             by_device.setdefault(p.device, []).append((p, g.contiguous(), buf))
+        self.step_count += 1  # (a refused step is none)
         for device, stacks in by_device.items():
             k = len(stacks)
             sizes = [_matrices(p, "a parameter") for p, _, _ in stacks]

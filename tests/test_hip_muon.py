@@ -523,3 +523,13 @@ def test_state_of_other_shapes_is_refused_whole():
     assert opt.step_count == 0 and opt.lr == 0.02 and not any(b.any() for b in opt.momentum_buffers)
     opt.load_state_dict({"step": 9, "lr": 0.5, "momentum_buffers": [ok, torch.ones(6, 7)]})
     assert opt.step_count == 9 and opt.lr == 0.5 and all(b.all() for b in opt.momentum_buffers)
+
+
+def test_a_refused_step_does_not_count():
+    opt = optim.HipMuon([])
+    p = torch.nn.Parameter(torch.zeros(4, 5))
+    opt.params, opt.momentum_buffers = [p], [torch.zeros(4, 6)]
+    p.grad = torch.zeros(4, 5)
+    with pytest.raises(RuntimeError, match="has changed"):
+        opt.step()
+    assert opt.step_count == 0
