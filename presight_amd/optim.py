@@ -279,12 +279,10 @@ def _ns_check(steps: int, a: float, b: float, c: float) -> float:
         p = max(abs(a + b * v + c * v * v) for v in inner)
         # extremes of v (a + b v^2 + c v^4) on [0, u]: the ends and the roots of a + 3 b w + 5 c w^2, w = v^2
         roots: List[float] = []
-        if c != 0:
-            d = 9 * b * b - 20 * a * c
-            if d >= 0:
-                roots = [(-3 * b + s * math.sqrt(d)) / (10 * c) for s in (1, -1)]
-        elif b != 0:
-            roots = [-a / (3 * b)]
+        d = 9 * b * b - 20 * a * c
+        if d >= 0:  # (as 2 a / h and h / (10 c), of which neither cancels; a very small c has one root far outside)
+            h = -3 * b - math.copysign(math.sqrt(d), b)
+            roots = [num / den for num, den in ((2 * a, h), (h, 10 * c)) if abs(num) < t * abs(den)]
         ends = [u] + [math.sqrt(w) for w in roots if 0 < w < t]
         u = max(abs(v * (a + b * v * v + c * v ** 4)) for v in ends)
         if max(p, u * u) > _NS_BOUND:

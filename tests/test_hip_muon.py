@@ -533,3 +533,27 @@ def test_a_refused_step_does_not_count():
     with pytest.raises(RuntimeError, match="has changed"):
         opt.step()
     assert opt.step_count == 0
+
+
+# ------------------------------------------------------------------------------------------------ the polynomial's bound
+@pytest.mark.parametrize("abc", [ABC, (2.0, -1.5, 0.5), (1.5, -0.5, 0.0), (3.0, -16 / 5, 6 / 5), (1.0, 0.0, 0.0), (3.9, -4.0, 0.0), (3.9, -4.0, 1e-17),
+                                 (3.9, -4.0, -1e-17), (1.5, -0.5, 1e-20), (-3.0, 3.5, 1e-18), (0.0, 0.0, 1.0), (0.5, 0.0, 1.0), (1.0, 1.0, -0.25),
+                                 (3.0, -3.0, 5e-324), (1e200, -1e200, 1e200)])
+def test_bound_that_the_kernels_rely_on(abc):
+    """what _ns_check returns is a power of two that the polynomial stays under, on a fine grid of every iterate's singular values; what
+    leaves the range is refused, however small the leading coefficient"""
+    a, b, c = abc
+    v, most, polynomial = torch.linspace(0, 1, 100001, dtype=torch.float64), 0.0, 0.0
+    for _ in range(3):
+        p = (a + b * v ** 2 + c * v ** 4).abs()
+        polynomial = max(polynomial, float(p.max()))
+        top = float((v * p).max())
+        most = max(most, polynomial, top * top)
+        v = torch.linspace(0, top, 100001, dtype=torch.float64)
+    if most > 15.0:
+        with pytest.raises(ValueError):
+            optim._ns_check(3, *abc)
+    else:
+        assert most < 14.9  # (no case sits on the border)
+        grow = optim._ns_check(3, *abc)
+        assert grow >= polynomial and math.log2(grow) % 1 == 0 and 1 <= grow <= 16
