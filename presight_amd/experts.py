@@ -283,6 +283,11 @@ class _ExpertLinear(torch.autograd.Function):
         return dx, dw if need_w else None, db, None
 
 
+def _offsets32(offsets: Tensor, M: int) -> Tensor:
+    """as the kernels read them: those of a longer list may lie beyond 32 bits, and mean "behind the M rows" there too"""
+    return (offsets if offsets.dtype == torch.int32 else offsets.clamp(0, M).to(torch.int32)).contiguous()
+
+
 def expert_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Union[Tensor, ExpertPlan]) -> Tensor:
     """x [M, in] sorted by expert, weight [E, out, in], bias [E, out] or None -> y [M, out], y[p] = weight[e] x[p] + bias[e] for the rows
     p in offsets[e] .. offsets[e+1].  offsets: an ExpertPlan, or int32 / int64 [E+1], ascending (others give undefined rows, within the
@@ -307,7 +312,7 @@ def expert_linear(x: Tensor, weight: Tensor, bias: Optional[Tensor], offsets: Un
         raise ValueError(f"presight_amd: x must have the plan's {plan.num_places} rows (got {x.shape[0]})")
     if max(weight.shape[1:]) > MAX_WIDTH or weight.shape[0] > 65536:
         raise ValueError("presight_amd: expert_linear takes up to 65536 experts and 2**20 features")
-    offsets = offsets.to(torch.int32).contiguous()
+    offsets = _offsets32(offsets, x.shape[0])
     if not _wants_grad(x, weight, bias):
         return _linear_fwd(x, weight, bias, offsets)
     return _ExpertLinear.apply(x, weight, bias, offsets)

@@ -670,3 +670,18 @@ def test_forward_mode_is_refused(dev):
                 call()
         y = experts.expert_linear(x, w, b, plan)  # (no tangent: as ever)
         assert forward_ad.unpack_dual(y).tangent is None
+
+
+# ------------------------------------------------------------------------------------------------ offsets beyond 32 bits
+def test_offsets_beyond_32_bits_are_bounded_before_they_are_narrowed():
+    wide = torch.tensor([-2 ** 33, 0, 3, 2 ** 31, 2 ** 32 + 1, 2 ** 62])
+    assert experts._offsets32(wide, 7).tolist() == [0, 0, 3, 7, 7, 7] and experts._offsets32(wide, 7).dtype == torch.int32
+    narrow = torch.tensor([0, 3, 9, 9], dtype=torch.int32)
+    assert experts._offsets32(narrow, 7) is narrow and experts._offsets32(narrow[::2], 7).is_contiguous()
+
+
+@pytest.mark.gpu
+def test_linear_of_the_first_rows_of_a_very_long_list(dev):
+    x, w = torch.randn(50, 24, device=dev), torch.randn(3, 8, 24, device=dev)
+    want = experts.expert_linear(x, w, None, torch.tensor([0, 20, 50, 50], device=dev))
+    assert torch.equal(experts.expert_linear(x, w, None, torch.tensor([0, 20, 2 ** 32 + 5, 2 ** 33], device=dev)), want)
