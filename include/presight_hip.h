@@ -663,7 +663,7 @@ int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void* x, int64_
 /* ---- the orthogonalised update: G [B,m,n] (dtype as above) -> X of the same type after `steps` of X <- a X + (b S + c S S) X, S = X X^T,
  * from X = G / (||G||_F + eps), every matrix by itself.  The caller checks that, from singular values in [0, 1], the iterates' squared
  * singular values t and |a + b t + c t^2| stay under 15, and gives a power of two >= 1 that the latter stays under (grow).
- * min(m, n) <= 16384, steps 1..64.  workspace: ps_newton_schulz_workspace bytes (NULL if 0).
+ * min(m, n) <= 16384, B ceil(m / 64) ceil(n / 64) < 2^24 - 8, steps 1..64.  workspace: ps_newton_schulz_workspace bytes (NULL if 0).
  *   ps_muon_step            for each of n_stacks stacks (HOST arrays of device pointers and sizes): buf <- momentum buf + (1 - momentum) g;
  *                           u = nesterov ? momentum buf + (1 - momentum) g : buf; p <- keep p - rate X(u); p, g, buf fp32 [B,m,n].  One
  *                           workspace, the largest that any stack needs, serves them one after the other */

@@ -729,7 +729,7 @@ constexpr int64_t kMaxSide = 1 << 20;
 
 bool sizes_ok(int64_t B, int64_t m, int64_t n, int steps) {
   return B >= 0 && B <= 65535 && m >= 0 && n >= 0 && m <= kMaxSide && n <= kMaxSide && steps >= 1 && steps <= 64 && (m < n ? m : n) <= 16384 &&
-         ((m + 127) / 128) * ((n + 127) / 128) * B < ((int64_t)1 << 30);
+         ((m + 63) / 64) * ((n + 63) / 64) * B < kMaxThreads / 256 - kXcds;  // (tiles of 64 x 64: the most threads a launch takes)
 }
 
 }  // namespace

@@ -263,6 +263,7 @@ class WarmupMultiStepSchedule:
 # ------------------------------------------------------------------------------------------------ the orthogonalised update
 NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)  # pushes (0, 1] into about [0.7, 1.2] in five steps: steep at zero, flat around one
 NS_MAX_SIDE = 16384  # of the short side
+_NS_MAX_TILES = (1 << 24) - 8  # of 64 x 64 over a whole stack: their launch holds fewer than 2^32 threads
 _NS_BOUND = 15.0  # on squared singular values and on the polynomial: what the kernels' fp16 planes can hold (csrc/orthogonal.hip)
 
 
@@ -310,6 +311,8 @@ def _matrices(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
     B = math.prod(t.shape[:-2])
     if min(m, n) > NS_MAX_SIDE or max(m, n) > 1 << 20 or B > 65535:
         raise ValueError(f"presight_amd: {name}: up to 65535 matrices of {NS_MAX_SIDE} x {1 << 20} (got shape {tuple(t.shape)})")
+    if B * -(-m // 64) * -(-n // 64) >= _NS_MAX_TILES:
+        raise ValueError(f"presight_amd: {name}: up to {_NS_MAX_TILES - 1} tiles of 64 x 64 in a stack (got shape {tuple(t.shape)})")
     return B, m, n
 
 

@@ -557,3 +557,19 @@ def test_bound_that_the_kernels_rely_on(abc):
         assert most < 14.9  # (no case sits on the border)
         grow = optim._ns_check(3, *abc)
         assert grow >= polynomial and math.log2(grow) % 1 == 0 and 1 <= grow <= 16
+
+
+# ------------------------------------------------------------------------------------------------ stacks that no launch holds
+def test_stacks_of_too_many_tiles_are_refused():
+    """65535 rows of 20000 elements: 20.5 million tiles of 256 threads, more than 2^32; 16000 are the most"""
+    from presight_amd._lib import check, lib
+
+    h = lib()
+    optim._matrices(torch.empty(65535, 1, 16000, device="meta"), "g")
+    assert h.ps_newton_schulz_workspace(65535, 1, 16000) > 0
+    for shape in ((65535, 1, 20000), (65535, 20000, 1), (65535, 1, 1 << 20), (16500, 64, 65536)):
+        with pytest.raises(ValueError, match="tiles"):
+            optim._matrices(torch.empty(shape, device="meta"), "g")
+        assert h.ps_newton_schulz_workspace(*shape) == 0
+        with pytest.raises(RuntimeError, match="sizes out of range"):
+            check(h.ps_newton_schulz(256, *shape, 0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, 256, 256, None), "ps_newton_schulz")
