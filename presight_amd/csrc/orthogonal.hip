@@ -3,14 +3,18 @@
 // first: [s, l] with s = min(m, n), l = max(m, n), so both products of a step with X and the square of S have the fewest operations.
 //
 // Arithmetic.  The polynomial multiplies what rounding leaves in the small singular directions by up to a^steps, so one 16-bit rounding
-// per step is not enough for an fp32 result.  Every matrix is kept as a PAIR of fp16 planes, value = (hi + lo) / 1024: 22 bits and the
-// sign, and a product is three matrix instructions, hi hi + hi lo + lo hi, summed in fp32 (lo lo, 2^-24 of the product, is left out).
-// That is fp32's own precision at a third of the fp16 rate, three times the fp32 matrix rate (large products: 1463 and 154 TFLOP/s).
+// per step is not enough for an fp32 result.  Every matrix is kept as a PAIR of fp16 planes, value = (hi + lo / 2048) / scale: 22 bits
+// and the sign, and a product is three matrix instructions, hi hi + (hi lo + lo hi) / 2048, summed in fp32 (lo lo, 2^-24 of the product, is
+// left out).  That is nearly fp32's precision at a third of the fp16 rate, three times the fp32 matrix rate (large products: 1463 and 154
+// TFLOP/s).
 //
 // Range.  The planes hold X^ = X / r with r = norm / (norm + eps) at the start, so an input far below eps loses nothing; a step
 // multiplies r by the power of two `grow` that bounds a + b t + c t^2, until r passes 1/2, and keeps it from then on.  The caller
-// checks that the iterates' squared singular values and the polynomial stay under 15: with X^ <= 2 X all entries are below 64, the
-// planes' end, and 1024 * entry keeps the low half normal down to entries of 2^-12.
+// checks that the iterates' squared singular values and the polynomial stay under 15: with X^ <= 2 X the entries of X^ are below 7.75,
+// those of S^ below 60 and those of the polynomial below 15, and each is scaled to the planes' end, 65504.  lo is 2048 times what hi leaves,
+// so it is as far from the subnormal numbers as hi is: X^ has its 22 bits down to entries of 2^-27 (of the whole matrix' norm, at the start),
+// and smaller ones are off by up to 2^-49.  (385 x 1290 normal numbers, one of them 10^6 times the rest: 5e-7 from 64 bits relative to the
+// norm, plain fp32 3e-7; with lo in hi's units, subnormal below 2^-12, 8e-6.)
 #include <type_traits>
 #include "gemm_core.hpp"
 
@@ -18,16 +22,15 @@ namespace {
 
 using namespace ps;
 
-constexpr float kPlaneScale = 1024.0f;                       // fp16 planes hold 1024 * value
-constexpr float kProductScale = 1.0f / (1024.0f * 1024.0f);  // of a product of two
+constexpr float kScaleX = 8192.0f, kScaleS = 1024.0f, kScaleP = 4096.0f;  // what the planes of X^, S^ and the polynomial hold of a value
+constexpr float kLowScale = 2048.0f, kLowUnit = 1.0f / kLowScale;         // lo's part of hi's unit
 constexpr int kCompute = 256;                                // compute units
 constexpr int kNormParts = 256;                              // partial sums of squares per matrix, at most
 
-template <typename V>  // float or double
-__device__ __forceinline__ void split(V v, _Float16& hi, _Float16& lo) {
-  const V t = v * (V)kPlaneScale;
+template <typename V>  // float or double, scaled
+__device__ __forceinline__ void split(V t, _Float16& hi, _Float16& lo) {
   hi = (_Float16)(float)t;
-  lo = (_Float16)(float)(t - (V)(float)hi);
+  lo = (_Float16)(float)((t - (V)(float)hi) * (V)kLowScale);
 }
 
 // The two planes lie side by side, 32 columns of hi and then the same 32 of lo: 128 bytes, a cache line and a tile row.  Rows are padded to
@@ -161,7 +164,7 @@ __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int row = h.tall ? c + k : r, col = h.tall ? r : c + k;
-      split(v[k] * inv, tile[0][row][col], tile[1][row][col]);
+      split(v[k] * inv * (double)kScaleX, tile[0][row][col], tile[1][row][col]);
     }
   }
   __syncthreads();
@@ -333,7 +336,7 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) mine[(i * NJ + j) * NT] = acc[i][j] + fine[i][j];
+      for (int j = 0; j < NJ; ++j) mine[(i * NJ + j) * NT] = acc[i][j] + fine[i][j] * kLowUnit;
     tile_barrier<0>();  // (no load is left on its way into LDS)
     return;
   }
@@ -349,11 +352,13 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
   const float ratio = ratio_at(start_ratio, step, c.grow);
   // kPoly: a + b r^2 S^ + c r^4 S^ S^ with the coefficients as pairs of floats: an error of a coefficient would be common to all entries and
   // grow like a singular value's | kApply: over the step's growth of r | kLast: X = r X^
-  const double r2 = (double)ratio * ratio, cb = c.b * r2 / kPlaneScale, cc = c.c * r2 * r2 * kProductScale;
+  const double r2 = (double)ratio * ratio, cb = c.b * r2 / kScaleS, cc = c.c * r2 * r2 / (kScaleS * kScaleS);
   const float cb_hi = (float)cb, cb_lo = (float)(cb - cb_hi), cc_hi = (float)cc, cc_lo = (float)(cc - cc_hi);
   const float ca_hi = (float)c.a, ca_lo = (float)(c.a - ca_hi);
-  const float out_scale = WHAT == kApply ? kProductScale * (ratio > 0.0f ? ratio / ratio_at(ratio, 1, c.grow) : 1.0f)
-                                         : (WHAT == kLast ? kProductScale * ratio : kProductScale);
+  // of the sums: to the planes of the result, or to the result itself
+  const float out_scale = WHAT == kGram    ? kScaleS / (kScaleX * kScaleX)
+                          : WHAT == kApply ? 1.0f / kScaleP * (ratio > 0.0f ? ratio / ratio_at(ratio, 1, c.grow) : 1.0f)
+                                           : 1.0f / (kScaleP * kScaleX) * ratio;
   if constexpr (WHAT == kLast) {
     const int image = (h.tall ? BM : BN) * 4;  // bytes of a row of G's direction
 #pragma unroll
@@ -361,7 +366,7 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int m = wm + i * 16 + r, n = wn + j * 16 + g * 4;
-        const f32x4 v = (acc[i][j] + fine[i][j]) * out_scale;
+        const f32x4 v = (acc[i][j] + fine[i][j] * kLowUnit) * out_scale;
         if (h.tall) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) *reinterpret_cast<float*>(lds + out_addr(n + q, image, m * 4)) = v[q];
@@ -423,12 +428,12 @@ __global__ __launch_bounds__(PairTile<BM>::kThreads) void ns_product_kernel(Oper
             gh = gram_at(i, j, 0), gl = gram_at(i, j, 1);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const float sum = acc[i][j][q] + fine[i][j][q];
+            const float sum = fmaf(fine[i][j][q], kLowUnit, acc[i][j][q]);
             if constexpr (WHAT == kPoly) {
               const bool one = m0 + m == n0 + n + q && m < rows;  // (rows and columns of the padding stay zero)
-              const float was = (float)gh.v[q] + (float)gl.v[q];
+              const float was = fmaf((float)gl.v[q], kLowUnit, (float)gh.v[q]);
               const float small = fmaf(cc_lo, sum, fmaf(cb_lo, was, one ? ca_lo : 0.0f));
-              split(fmaf(cb_hi, was, one ? ca_hi : 0.0f) + fmaf(cc_hi, sum, small), hi.v[q], lo.v[q]);
+              split((fmaf(cb_hi, was, one ? ca_hi : 0.0f) + fmaf(cc_hi, sum, small)) * kScaleP, hi.v[q], lo.v[q]);
             } else {
               split(sum * out_scale, hi.v[q], lo.v[q]);
             }

@@ -320,7 +320,8 @@ def _matrices(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
 def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """g [..., m, n] in fp32, fp16 or bf16 -> a tensor of its shape and type: every matrix scaled to X = G / (||G||_F + eps) and taken
     `steps` times through X <- a X + (b S + c S S) X with S = X X^T: its singular vectors kept, its singular values moved towards one.
-    Products of fp16 pairs (22 bits) summed in fp32, one rounding at the end.  A zero matrix stays zero; a matrix with an infinite or
+    Matrices of more than 64 rows and columns are held as fp16 pairs: 22 bits of every entry, and what lies below 2^-27 of the matrix' norm to
+    2^-49 of it; smaller ones in fp32.  Sums in fp32, one rounding at the end.  A zero matrix stays zero; a matrix with an infinite or
     undefined entry becomes undefined, without touching the others of the stack.  Not differentiable."""
     args = _ns_args(steps, tuple(coefficients), eps)
     code = _typed(_gpu(g, "g"), "g")

@@ -573,3 +573,49 @@ def test_stacks_of_too_many_tiles_are_refused():
         assert h.ps_newton_schulz_workspace(*shape) == 0
         with pytest.raises(RuntimeError, match="sizes out of range"):
             check(h.ps_newton_schulz(256, *shape, 0, 5, 1.0, 0.0, 0.0, 1.0, 0.0, 256, 256, None), "ps_newton_schulz")
+
+
+# ------------------------------------------------------------------------------------------------ entries of very different size
+def uneven(m, n, kind, size, seed=19):
+    """normal numbers, among them an entry, a row or a column `size` times the rest, or rows of every size between"""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(m, n, generator=g)
+    if kind == "entry":
+        x[m // 3, n // 2] = size
+    elif kind == "row":
+        x[m // 2] *= size
+    elif kind == "column":
+        x[:, n // 3] *= size
+    else:
+        x *= size ** torch.rand(m, 1, generator=g)
+    return x
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e3, 1e5, 1e6, 1e8, 1e10])
+@pytest.mark.parametrize("m,n,kind", [(200, 300, "entry"), (200, 300, "row"), (200, 300, "column"), (300, 200, "rows"), (385, 1290, "entry"),
+                                      (1290, 385, "row"), (64, 48, "entry"), (70, 3000, "entry")])
+def test_outliers(dev, m, n, kind, size):
+    """what is small beside the largest entries keeps its bits: the bound of evenly sized ones holds"""
+    x = uneven(m, n, kind, size)
+    check(optim.newton_schulz(x.to(dev)), x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 8, 12])
+def test_outliers_over_more_steps(dev, steps):
+    """each step lifts the small directions further, and with them what rounding left there"""
+    for kind, size in (("entry", 1e6), ("entry", 1e8), ("row", 1e5)):
+        x = uneven(200, 300, kind, size)
+        check(optim.newton_schulz(x.to(dev), steps=steps), x, steps)
+
+
+@pytest.mark.gpu
+def test_an_outlier_in_a_stack_of_large_tiles(dev):
+    x = torch.stack([uneven(600, 700, k, s, seed=i) for i, (k, s) in enumerate([("entry", 1e6), ("row", 1e5), ("entry", 1.0), ("column", 1e8)] * 3)])
+    y = optim.newton_schulz(x.to(dev)).cpu()
+    for got, g in zip(y[:4], x[:4]):
+        check(got, g)
+    ref = iterate(x.to(dev).double()).cpu()
+    for got, want in zip(y, ref):  # (the same four kinds again: 16 units of the norm or four times what plain fp32 is off by, 2e-6 of it)
+        assert float((got.double() - want).norm()) <= 8e-6 * float(want.norm())
