@@ -23,13 +23,16 @@ __device__ __forceinline__ int64_t bounded(int v, int64_t M) { return v < 0 ? 0 
 // what M rows of E experts can make at most
 __host__ __device__ inline int64_t row_tiles_at_most(int64_t M, int E, int piece) { return (M + piece - 1) / piece + (M < E ? M : E); }
 
-// The tiles of `piece` rows that the experts' rows make: a prefix sum over the lanes, each with its share of neighbouring experts, and a second
+// ... and those of more than `above` rows: one piece more than its share for each, of M / (above + 1) at most
+__host__ __device__ inline int64_t crowded_pieces_at_most(int64_t M, int above) { return 2 * (M / above); }
+
+// The tiles of `piece` rows that the experts' rows make (above > 0: pieces of `above` rows, of the experts with more than that): a prefix sum over the lanes, each with its share of neighbouring experts, and a second
 // one over the experts of the lane that holds the tile, where it has several.  (64 experts after the other instead, and a workgroup per
 // expert whether it can have rows or not: 16 rows of 256 experts, 1024 x 2048 bf16, 30.7 us for 14.9; 8192 of 1024, 256 x 512, 157 for 80.)
 struct RowTiles {
   const int* offsets;
   int64_t M;
-  int E, piece, each;  // each: experts per lane
+  int E, piece, above, each;  // each: experts per lane
   int lo, len;         // rows of this lane's last expert
   unsigned mine, incl; // tiles of this lane's experts; up to and with them
   int total;           // tiles in all
@@ -38,6 +41,7 @@ struct RowTiles {
     const int64_t first = bounded(offsets[e], M), end = bounded(offsets[e + 1], M);
     lo = (int)first;
     len = end > first ? (int)(end - first) : 0;
+    if (len <= above) len = 0;
     return ((unsigned)len + (unsigned)piece - 1u) / (unsigned)piece;
   }
   __device__ __forceinline__ unsigned scan() {  // incl from mine -> their sum
@@ -49,10 +53,10 @@ struct RowTiles {
     }
     return (unsigned)__builtin_amdgcn_readlane((int)incl, 63);
   }
-  __device__ __forceinline__ RowTiles(const int* offsets_, int E_, int64_t M_, int piece_)
-      : offsets(offsets_), M(M_), E(E_), piece(piece_), each((E_ + 63) / 64), lo(0), len(0), mine(0), total(0) {
+  __device__ __forceinline__ RowTiles(const int* offsets_, int E_, int64_t M_, int piece_, int above_ = 0)
+      : offsets(offsets_), M(M_), E(E_), piece(piece_), above(above_), each((E_ + 63) / 64), lo(0), len(0), mine(0), total(0) {
     // (offsets that do not ascend could ask for more than there is room for; 64 lanes' `most` stay below 2^32)
-    const unsigned most = (unsigned)row_tiles_at_most(M, E, piece);
+    const unsigned most = (unsigned)(above > 0 ? crowded_pieces_at_most(M, above) : row_tiles_at_most(M, E, piece));
     const int e0 = (threadIdx.x & 63) * each, e1 = e0 + each < E ? e0 + each : E;
 #pragma unroll 4
     for (int e = e0; e < e1; ++e) {
@@ -63,24 +67,25 @@ struct RowTiles {
     total = (int)(sum < most ? sum : most);
   }
   // tile t < total, uniform over the wave
-  __device__ __forceinline__ RowTile find(int t_) {
+  __device__ __forceinline__ RowTile find(int t_) const {
+    RowTiles s = *this;
     unsigned t = (unsigned)t_;
-    int who = uniform(__ffsll((long long)__ballot(t < incl)) - 1), e0 = 0;
+    int who = uniform(__ffsll((long long)__ballot(t < s.incl)) - 1), e0 = 0;
     if (each > 1) {
-      t -= (unsigned)__builtin_amdgcn_readlane((int)(incl - mine), who);
+      t -= (unsigned)__builtin_amdgcn_readlane((int)(s.incl - s.mine), who);
       e0 = who * each;
       const int e1 = e0 + each < E ? e0 + each : E;
       for (;; e0 += 64) {
         const int e = e0 + (threadIdx.x & 63);
-        mine = e < e1 ? read(e) : 0;
-        const unsigned n = scan();
+        s.mine = e < e1 ? s.read(e) : 0;
+        const unsigned n = s.scan();
         if (t < n || e0 + 64 >= e1) break;
         t -= n;
       }
-      who = uniform(__ffsll((long long)__ballot(t < incl)) - 1);
+      who = uniform(__ffsll((long long)__ballot(t < s.incl)) - 1);
     }
-    const int n = __builtin_amdgcn_readlane(len, who), k = (int)(t - (unsigned)__builtin_amdgcn_readlane((int)(incl - mine), who));
-    return {e0 + who, (int64_t)__builtin_amdgcn_readlane(lo, who) + (int64_t)k * piece, n - k * piece < piece ? n - k * piece : piece};
+    const int n = __builtin_amdgcn_readlane(s.len, who), k = (int)(t - (unsigned)__builtin_amdgcn_readlane((int)(s.incl - s.mine), who));
+    return {e0 + who, (int64_t)__builtin_amdgcn_readlane(s.lo, who) + (int64_t)k * piece, n - k * piece < piece ? n - k * piece : piece};
   }
 };
 
@@ -269,25 +274,30 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
 // dw_join_kernel adds up the pieces of each expert in order.  Also shorter sums: a piece rounds `piece` / 4 times where the whole
 // column would round a hundred times as often.
 // 65536 rows, 2048 x 1024 bf16, 32 experts (whole): 258 us, 1065 TFLOP/s; 131072 rows of 64 x 64 fp32, 16 experts (pieces): 21 us and 5 to join.
-template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
+// Many experts whose share is short are summed whole, but all rows may go to a few of them (kCrowded): the first `piece_blocks` workgroups take the
+// pieces of those with more than `piece` rows, the others leave these experts out, and dw_join_crowded_kernel adds the pieces up.
+enum DwCut { kWhole, kPieces, kCrowded };
+
+template <typename T, int BM, int BN, int WM, int WN, DwCut CUT>
 __global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __restrict__ dy, int64_t ldy, const T* __restrict__ x, int64_t ldx,
-                                                                        const int* __restrict__ offsets, int64_t M, int E, int N, int K, int ldo, int piece,
-                                                                 void* __restrict__ dw, void* __restrict__ db) {
+                                                                 const int* __restrict__ offsets, int64_t M, int E, int N, int K, int ldo, int piece,
+                                                                 int piece_blocks, void* __restrict__ dw, void* __restrict__ db,
+                                                                 float* __restrict__ parts, float* __restrict__ db_parts) {
   constexpr int NT = 64 * WM * WN, MI = BM / WM / 16, NJ = BN / WN / 16;
-  using Out = std::conditional_t<SPLIT, float, T>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int n_tiles = (K + BN - 1) / BN, m_tiles = (N + BM - 1) / BM;
   // (a unit's tiles share all of their operands: they stay on one XCD)
   const int tiles = n_tiles * m_tiles;
+  const bool cut = CUT == kPieces || (CUT == kCrowded && (int)blockIdx.x < piece_blocks);
   int units = E, unit, len;
   int64_t row0;
-  RowTiles pieces(offsets, SPLIT ? E : 0, M, SPLIT ? piece : 1);
-  if constexpr (SPLIT) units = pieces.total;
-  const int place = xcd_place(blockIdx.x, units * tiles);
+  RowTiles pieces(offsets, cut ? E : 0, M, CUT == kWhole ? 1 : piece, CUT == kCrowded ? piece : 0);
+  if (cut) units = pieces.total;
+  const int place = xcd_place(CUT == kCrowded && !cut ? (int)blockIdx.x - piece_blocks : (int)blockIdx.x, units * tiles);
   if (place < 0) return;
   unit = place / tiles;
   const int tn = place % n_tiles, tm = place % tiles / n_tiles;
-  if constexpr (SPLIT) {
+  if (cut) {
     const RowTile t = pieces.find(unit);
     row0 = t.row0;
     len = t.rows;
@@ -295,6 +305,7 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __rest
     const int64_t lo = bounded(offsets[unit], M), hi = bounded(offsets[unit + 1], M);
     row0 = lo;
     len = uniform(hi > lo ? (int)(hi - lo) : 0);
+    if (CUT == kCrowded && len > piece) return;
   }
   const int m0 = tm * BM, n0 = tn * BN;
   constexpr int kC = kChunk<T>;  // (rows hold whole chunks)
@@ -304,41 +315,33 @@ __global__ __launch_bounds__(64 * WM * WN) void linear_dw_kernel(const T* __rest
   const bool sums = db != nullptr && tn == 0 && wn == 0;
   f32x4 acc[MI][NJ], row_sums[MI];
   direct_loop<T, BM, BN, WM, WN, true, true, true>(lds, len, sa, sb, acc, row_sums, sums);
-  Out* o = reinterpret_cast<Out*>(dw) + ((int64_t)unit * N + m0) * ldo + n0;
   constexpr int kSlice = 2 * (BM + BN) * kTileRowBytes / (WM * WN);
-  store_tile_rows<Out, MI, NJ, kSlice>(acc, lds + wave * kSlice, o, ldo, N - m0 < BM ? N - m0 : BM, K - n0 < BN ? K - n0 : BN, wm, wn,
-                                       static_cast<const Out*>(nullptr));
-  if (sums && (threadIdx.x & 63) < 16) {
+  auto leave = [&](auto* o, int64_t ld, auto* ob, int64_t ldb) {
+    using Out = std::remove_pointer_t<decltype(o)>;
+    store_tile_rows<Out, MI, NJ, kSlice>(acc, lds + wave * kSlice, o + ((int64_t)unit * N + m0) * ld + n0, ld, N - m0 < BM ? N - m0 : BM,
+                                         K - n0 < BN ? K - n0 : BN, wm, wn, static_cast<const Out*>(nullptr));
+    if (sums && (threadIdx.x & 63) < 16) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int m = m0 + wm + i * 16 + (threadIdx.x & 15);
-      if (m < N) reinterpret_cast<Out*>(db)[(int64_t)unit * (SPLIT ? (N + 3) / 4 * 4 : N) + m] = from_f32<Out>(row_sums[i][0]);
+      for (int i = 0; i < MI; ++i) {
+        const int m = m0 + wm + i * 16 + (threadIdx.x & 15);
+        if (m < N) ob[(int64_t)unit * ldb + m] = from_f32<Out>(row_sums[i][0]);
+      }
     }
-  }
+  };
+  if (cut)
+    leave(parts, ldo, db_parts, (N + 3) / 4 * 4);
+  else
+    leave(reinterpret_cast<T*>(dw), K, reinterpret_cast<T*>(db), N);
 }
 
-// dW_e, db_e = the sums of expert e's pieces: parts [unit][out][ldo] (ldo: in, rounded up to four) and db_parts [unit][out rounded up].
-// Four lanes share the pieces of four neighbouring sums, each takes every fourth in order, and the four meet in LDS in order.
+// dW_e, db_e = the sums of expert e's n pieces from `first` on: parts [unit][out][ldo] (ldo: in, rounded up to four) and db_parts [unit][out
+// rounded up].  Four lanes share the pieces of four neighbouring sums, each takes every fourth in order, and the four meet in LDS in order.
 template <typename T>
-__global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ parts, const float* __restrict__ db_parts, const int* __restrict__ offsets,
-                                                      int64_t M, int N, int K, int ldo, int piece, T* __restrict__ dw, T* __restrict__ db) {
-  __shared__ int wave_sum[4];
+__device__ __forceinline__ void join_pieces(const float* __restrict__ parts, const float* __restrict__ db_parts, int e, int64_t first, int n, int64_t chunk, int N,
+                                            int K, int ldo, T* __restrict__ dw, T* __restrict__ db) {
   __shared__ f32x4 quarter[4][64];
-  const int e = blockIdx.y;
-  int before = 0;
-  for (int i = threadIdx.x; i < e; i += 256) {
-    const int64_t lo = bounded(offsets[i], M), hi = bounded(offsets[i + 1], M);
-    if (hi > lo) before += (int)((hi - lo + piece - 1) / piece);
-  }
-  for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d, 64);
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  if (lane == 0) wave_sum[wave] = before;
-  __syncthreads();
-  const int64_t most = row_tiles_at_most(M, gridDim.y, piece), all = (int64_t)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
-  const int64_t first = all < most ? all : most, lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
-  const int64_t mine = hi > lo ? (hi - lo + piece - 1) / piece : 0;
-  const int n = (int)(mine < most - first ? mine : most - first);
-  const int64_t size = (int64_t)N * ldo, db_size = (N + 3) / 4 * 4, i = ((int64_t)blockIdx.x * 64 + lane) * 4;
+  const int64_t size = (int64_t)N * ldo, db_size = (N + 3) / 4 * 4, i = (chunk * 64 + lane) * 4;
   const bool bias = i >= size;  // (the weights' sums first, then the bias's)
   const float* p = bias ? db_parts + first * db_size + (i - size) : parts + first * size + i;
   const int64_t step = bias ? db_size : size;
@@ -355,15 +358,54 @@ __global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ 
   }
   quarter[wave][lane] = v;
   __syncthreads();
-  if (wave != 0 || !on) return;
-  v = (quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]);
+  if (wave == 0 && on) {
+    v = (quarter[0][lane] + quarter[1][lane]) + (quarter[2][lane] + quarter[3][lane]);
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    if (bias) {
-      if (i - size + q < N) db[(int64_t)e * N + (i - size) + q] = from_f32<T>(v[q]);
-    } else {
-      const int64_t m = (i + q) / ldo, c = (i + q) % ldo;
-      if (c < K) dw[((int64_t)e * N + m) * K + c] = from_f32<T>(v[q]);
+    for (int q = 0; q < 4; ++q) {
+      if (bias) {
+        if (i - size + q < N) db[(int64_t)e * N + (i - size) + q] = from_f32<T>(v[q]);
+      } else {
+        const int64_t m = (i + q) / ldo, c = (i + q) % ldo;
+        if (c < K) dw[((int64_t)e * N + m) * K + c] = from_f32<T>(v[q]);
+      }
+    }
+  }
+}
+
+// ... of every expert
+template <typename T>
+__global__ __launch_bounds__(256) void dw_join_kernel(const float* __restrict__ parts, const float* __restrict__ db_parts, const int* __restrict__ offsets,
+                                                      int64_t M, int N, int K, int ldo, int piece, T* __restrict__ dw, T* __restrict__ db) {
+  __shared__ int wave_sum[4];
+  const int e = blockIdx.y;
+  int before = 0;
+  for (int i = threadIdx.x; i < e; i += 256) {
+    const int64_t lo = bounded(offsets[i], M), hi = bounded(offsets[i + 1], M);
+    if (hi > lo) before += (int)((hi - lo + piece - 1) / piece);
+  }
+  for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d, 64);
+  if ((threadIdx.x & 63) == 0) wave_sum[threadIdx.x >> 6] = before;
+  __syncthreads();
+  const int64_t most = row_tiles_at_most(M, gridDim.y, piece), all = (int64_t)wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
+  const int64_t first = all < most ? all : most, lo = bounded(offsets[e], M), hi = bounded(offsets[e + 1], M);
+  const int64_t mine = hi > lo ? (hi - lo + piece - 1) / piece : 0;
+  join_pieces(parts, db_parts, e, first, (int)(mine < most - first ? mine : most - first), blockIdx.x, N, K, ldo, dw, db);
+}
+
+// ... of the experts with more than `piece` rows: the workgroups of a row of the grid look at every gridDim.y-th piece, and where it is its
+// expert's first share out the sums
+template <typename T>
+__global__ __launch_bounds__(256) void dw_join_crowded_kernel(const float* __restrict__ parts, const float* __restrict__ db_parts,
+                                                              const int* __restrict__ offsets, int64_t M, int E, int N, int K, int ldo, int piece, int chunks,
+                                                              T* __restrict__ dw, T* __restrict__ db) {
+  const RowTiles pieces(offsets, E, M, piece, piece);
+  for (int u = blockIdx.y; u < pieces.total; u += gridDim.y) {
+    const RowTile t = pieces.find(u);
+    const int64_t lo = bounded(offsets[t.expert], M), n = (bounded(offsets[t.expert + 1], M) - lo + piece - 1) / piece;
+    if (t.row0 != lo) continue;
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+      join_pieces(parts, db_parts, t.expert, u, (int)(n < pieces.total - u ? n : pieces.total - u), chunk, N, K, ldo, dw, db);
+      __syncthreads();
     }
   }
 }
@@ -529,38 +571,47 @@ int launch_linear(const void* x, int64_t ldx, const void* weight, const void* bi
   });
 }
 
-// How the weight gradients are cut: the tile, and the rows of a piece (0: one piece per expert)
+// How the weight gradients are cut: the tile, the rows of a piece and the pieces that there are room for
 struct DwPlan {
+  DwCut cut;
   int tile, piece;
   int64_t units;
 };
 // The cheapest by the tiles' steps.  Pieces shorten the longest run of steps and cost 5 us and the way of their fp32 sums through the memory,
-// 4.5 TB/s; without them an expert may well have twice its share of the rows.
+// 4.5 TB/s; without them an expert may well have twice its share of the rows.  Where one that had them all would keep its compute units busy for
+// more than 150 us (a router that has collapsed), those with more than four times their share, and 2048 rows, are cut all the same: a launch
+// more, which finds nothing to join as a rule.  No sum is then longer than that, and no longer than 150 us of steps otherwise.
+//     evenly shared / all rows to one expert, cut and not:  131072 rows, 1024 experts of 64 x 64 fp32 24 / 75 us, 20 / 4090 | 65536, 128 of 256 x 256
+//     fp32 92 / 191, 84 / 5566 | 65536, 32 of 2048 x 1024 bf16 277 / 298, 275 / 1769 | 16384, 8 of 1024 x 1024 bf16 43 / 107, 43 / 225
 //     16 experts, fp32:  131072 rows of 64 x 64 in pieces 22 us, whole 191 | 32768 rows of 128 x 128 in pieces, tiles of 64 21, of 128 30
 //     bf16:  8192 rows, 16 experts of 512 x 512 whole 12, in pieces 45 | 65536 rows, 32 experts of 2048 x 1024 tiles of 256 307, of 128 374
 DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
   const bool wide = dtype == kF32;
   const StepCost cost = step_cost(dtype);
   const int64_t least = n_in < n_out ? n_in : n_out, step_rows = wide ? 32 : 64, each = M / E;
-  DwPlan best{64, 0, E};
+  DwPlan best{kWhole, 64, 0, 0};
   double best_us = 1e30;
   for (int i = 0; i < cost.sizes; ++i) {
     const int tile = 64 << i;
     if (i > 0 && least <= tile / 2) break;
     const double tiles = (double)((n_in + tile - 1) / tile) * ((n_out + tile - 1) / tile);
     for (int64_t pieces = 1; pieces == 1 || each / pieces >= 192; pieces *= 2) {
-      DwPlan p{tile, 0, E};
+      DwPlan p{kWhole, tile, 0, 0};
       int64_t rows = each, longest = E > 1 ? 2 * each : each;
+      double more = 0.0;  // what the pieces cost
       if (pieces > 1) {
         rows = ((each + pieces - 1) / pieces + 63) & ~(int64_t)63;
         longest = rows = rows < 256 ? 256 : rows;
-        p.piece = (int)rows;
-        p.units = row_tiles_at_most(M, E, p.piece);
+        p = {kPieces, tile, (int)rows, row_tiles_at_most(M, E, (int)rows)};
+        more = 5.0 + 8e-6 / 4.5 * p.units * n_in * n_out;
+      } else if (cost.least[i] * (double)((M + step_rows - 1) / step_rows) > 150.0) {
+        const int64_t share = ((M + E - 1) / E * 4 + 63) & ~(int64_t)63, most = share < 2048 ? 2048 : share;
+        if (most < M) p = {kCrowded, tile, (int)most, crowded_pieces_at_most(M, (int)most)}, more = 3.0;
       }
       const double shared = tiles * (pieces > 1 ? (double)M / rows + 0.5 * E : (double)E) / kCompute;  // workgroups per compute unit
       const double steps = (double)((rows + step_rows - 1) / step_rows), all = cost.busy[i] * (shared > 1 ? shared : 1) * (steps > 1 ? steps : 1);
       const double run = cost.least[i] * (double)((longest + step_rows - 1) / step_rows);
-      const double us = (all > run ? all : run) + (pieces > 1 ? 5.0 + 8e-6 / 4.5 * p.units * n_in * n_out : 0.0);
+      const double us = (all > run ? all : run) + more;
       if (us < best_us) best = p, best_us = us;
     }
   }
@@ -569,28 +620,34 @@ DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
 
 int64_t round4(int64_t v) { return (v + 3) / 4 * 4; }
 int64_t dw_part_bytes(const DwPlan& p, int64_t n_in, int64_t n_out) {
-  return p.piece == 0 ? 0 : (p.units * (n_out * round4(n_in) + round4(n_out)) * (int64_t)sizeof(float) + 255) & ~(int64_t)255;
+  return p.cut == kWhole ? 0 : (p.units * (n_out * round4(n_in) + round4(n_out)) * (int64_t)sizeof(float) + 255) & ~(int64_t)255;
 }
 
-template <typename T, int B, int WM, int WN, bool SPLIT>
-int launch_dw_tile(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t* offsets, int64_t M, int E, int N, int K, int ldo, void* dw, void* db,
-                   hipStream_t s) {
+struct DwArgs {
+  const int32_t* offsets;
+  int64_t M;
+  int E, N, K, ldo;
+  void *dw, *db;
+  float *parts, *db_parts;
+};
+template <typename T, int B, int WM, int WN, DwCut CUT>
+int launch_dw_tile(const DwPlan& p, const Rows& dy, const Rows& x, const DwArgs& d, hipStream_t s) {
   constexpr int lds = 4 * B * kTileRowBytes;
-  const int64_t blocks = xcd_blocks(p.units * ((N + B - 1) / B) * ((K + B - 1) / B));
+  const int64_t tiles = ((d.N + B - 1) / B) * (int64_t)((d.K + B - 1) / B), pieces = CUT == kWhole ? 0 : xcd_blocks(p.units * tiles);
+  const int64_t blocks = pieces + (CUT == kPieces ? 0 : xcd_blocks(d.E * tiles));
   PS_REQUIRE(blocks * 64 * WM * WN < kMaxThreads, "ps_expert_linear_dw: too many tiles");
-  allow_lds(linear_dw_kernel<T, B, B, WM, WN, SPLIT>, lds);
-  linear_dw_kernel<T, B, B, WM, WN, SPLIT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy.p, dy.ld, (const T*)x.p, x.ld, offsets, M, E, N, K, ldo,
-                                                                                      p.piece, dw, db);
+  allow_lds(linear_dw_kernel<T, B, B, WM, WN, CUT>, lds);
+  linear_dw_kernel<T, B, B, WM, WN, CUT><<<(unsigned)blocks, 64 * WM * WN, lds, s>>>((const T*)dy.p, dy.ld, (const T*)x.p, x.ld, d.offsets, d.M, d.E, d.N, d.K,
+                                                                                    d.ldo, p.piece, (int)pieces, d.dw, d.db, d.parts, d.db_parts);
   PS_CHECK_LAUNCH();
 }
 
-template <typename T, bool SPLIT>
-int launch_dw(const DwPlan& p, const Rows& dy, const Rows& x, const int32_t* offsets, int64_t M, int E, int N, int K, int ldo, void* dw, void* db,
-              hipStream_t s) {
+template <typename T, DwCut CUT>
+int launch_dw(const DwPlan& p, const Rows& dy, const Rows& x, const DwArgs& d, hipStream_t s) {
   if constexpr (sizeof(T) == 2)
-    if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
-  if (p.tile == 128) return launch_dw_tile<T, 128, 2, 2, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
-  return launch_dw_tile<T, 64, 2, 2, SPLIT>(p, dy, x, offsets, M, E, N, K, ldo, dw, db, s);
+    if (p.tile == 256) return launch_dw_tile<T, 256, 2, 4, CUT>(p, dy, x, d, s);
+  if (p.tile == 128) return launch_dw_tile<T, 128, 2, 2, CUT>(p, dy, x, d, s);
+  return launch_dw_tile<T, 64, 2, 2, CUT>(p, dy, x, d, s);
 }
 
 enum Pass { kForward, kInputGradient, kWeightGradient };
@@ -645,13 +702,20 @@ extern "C" int ps_expert_linear_dw(const void* dy, int64_t dy_stride, const void
     float* parts = (float*)workspace;
     Rows dys, xs;
     packed<T>({dy, dy_stride, M, n_out}, {x, x_stride, M, n_in}, dtype, (char*)workspace + dw_part_bytes(p, n_in, n_out), &dys, &xs, s);
-    if (p.piece == 0) return launch_dw<T, false>(p, dys, xs, offsets, M, E, N, K, K, dweight, dbias, s);
     float* db_parts = parts + p.units * n_out * ldo;
-    const int rc = launch_dw<T, true>(p, dys, xs, offsets, M, E, N, K, ldo, parts, dbias != nullptr ? db_parts : nullptr, s);
+    const DwArgs d{offsets, M, E, N, K, ldo, dweight, dbias, parts, db_parts};
+    if (p.cut == kWhole) return launch_dw<T, kWhole>(p, dys, xs, d, s);
+    const int rc = p.cut == kPieces ? launch_dw<T, kPieces>(p, dys, xs, d, s) : launch_dw<T, kCrowded>(p, dys, xs, d, s);
     if (rc != 0) return rc;
     const int64_t sums = n_out * ldo + (dbias != nullptr ? round4(n_out) : 0);
-    dw_join_kernel<T><<<dim3((unsigned)((sums + 255) / 256), (unsigned)E), 256, 0, s>>>(parts, db_parts, offsets, M, N, K, ldo, p.piece, (T*)dweight,
-                                                                                       (T*)dbias);
+    const unsigned chunks = (unsigned)((sums + 255) / 256);
+    if (p.cut == kPieces)
+      dw_join_kernel<T><<<dim3(chunks, (unsigned)E), 256, 0, s>>>(parts, db_parts, offsets, M, N, K, ldo, p.piece, (T*)dweight, (T*)dbias);
+    else {  // (as a rule there is nothing to do: few workgroups)
+      const unsigned across = chunks < 512 ? chunks : 512, most = across < 256 ? 256 / across : 1;
+      dw_join_crowded_kernel<T><<<dim3(across, p.units < most ? (unsigned)p.units : most), 256, 0, s>>>(parts, db_parts, offsets, M, E, N, K, ldo, p.piece,
+                                                                                                       (int)chunks, (T*)dweight, (T*)dbias);
+    }
     PS_CHECK_LAUNCH();
   });
 }

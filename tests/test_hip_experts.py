@@ -685,3 +685,85 @@ def test_linear_of_the_first_rows_of_a_very_long_list(dev):
     x, w = torch.randn(50, 24, device=dev), torch.randn(3, 8, 24, device=dev)
     want = experts.expert_linear(x, w, None, torch.tensor([0, 20, 50, 50], device=dev))
     assert torch.equal(experts.expert_linear(x, w, None, torch.tensor([0, 20, 2 ** 32 + 5, 2 ** 33], device=dev)), want)
+
+
+# ------------------------------------------------------------------------------------------------ crowded experts
+def test_weight_gradients_of_many_experts_make_room_for_a_crowded_one():
+    """sums of the weights' gradients are cut where one expert that had all rows would be summed in one run for long"""
+    from presight_amd._lib import lib
+
+    need = lambda M, E, n_in, n_out, code: lib().ps_expert_linear_workspace(2, 256, n_out, 256, n_in, M, E, n_in, n_out, code)  # noqa: E731
+    for M, E, code in ((65536, 512, 0), (131072, 1024, 0), (131072, 1024, 1), (65536, 32, 2)):
+        assert need(M, E, 64, 64, code) > 0
+    # room for two pieces of 2048 rows, or of four times the even share, for every one that fits the rows; 64 more sums for the bias
+    assert need(131072, 1024, 64, 64, 0) == 2 * 64 * (64 * 64 + 64) * 4
+    assert need(65536, 32, 2048, 1024, 2) == 2 * 8 * (2048 * 1024 + 1024) * 4
+    assert need(2048, 16, 64, 64, 0) == need(5000, 64, 512, 512, 2) == 0  # (short whoever has them)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,E", [(131072, 1024), (70000, 300)])
+def test_a_crowded_experts_sums_are_cut(dev, M, E):
+    """all rows to one expert: its first term is one and every other one 2^-28, which one run of fp32 additions loses; cut to 2048 rows it
+    is off by 2048 + the pieces of additions at most"""
+    x, dy = torch.full((M, 64), 2.0 ** -28, device=dev), torch.ones(M, 64, device=dev)
+    x[0] = 1.0
+    x.requires_grad_(True)
+    w, b = torch.zeros(E, 64, 64, device=dev, requires_grad=True), torch.zeros(E, 64, device=dev, requires_grad=True)
+    for at in (0, E // 2, E - 1):
+        offsets = torch.where(torch.arange(E + 1, device=dev) > at, M, 0)
+        dw, db = torch.autograd.grad(experts.expert_linear(x, w, b, offsets), [w, b], dy)
+        ref = torch.full((64, 64), 1.0 + (M - 1) * 2.0 ** -28, dtype=torch.float64)
+        within(dw[at], ref, 2048 + M // 2048 + 66, ref)
+        assert (db[at] == M).all()  # (whole numbers below 2^24: exact)
+        keep = torch.arange(E, device=dev) != at
+        assert not dw[keep].any() and not db[keep].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("M,E,n_in,n_out,kind", [(70000, 300, 24, 40, "one"), (70000, 300, 24, 40, "ragged"), (66000, 5000, 16, 33, "one"),
+                                                 (40000, 64, 136, 130, "one"), (30000, 64, 264, 300, "ragged"), (30011, 70, 265, 301, "one")])
+def test_linear_of_crowded_experts(dev, M, E, n_in, n_out, kind, dtype):
+    """some or all rows at one or a few of many experts, every tile, odd rows, with and without room for more than one piece"""
+    check_linear(dev, M, E, n_in, n_out, dtype, kind, bias=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,E", [(70000, 300), (66000, 5000)])
+def test_crowded_offsets_that_do_not_ascend(dev, M, E):
+    """ask for more pieces than there is room for: every access stays inside, what follows is right"""
+    x, w = torch.ones(M, 24, device=dev, requires_grad=True), torch.ones(E, 40, 24, device=dev, requires_grad=True)
+    for first, second in ((0, M), (M, 0), (M + 7, -9)):
+        offsets = torch.tensor([first, second] * E, dtype=torch.int32, device=dev)[: E + 1]
+        torch.autograd.grad(experts.expert_linear(x, w, None, offsets), [w], torch.ones(M, 40, device=dev))
+    offsets = torch.tensor([0] * E + [M], device=dev)
+    (dw,) = torch.autograd.grad(experts.expert_linear(x, w, None, offsets), [w], torch.ones(M, 40, device=dev))
+    assert (dw[-1] == M).all() and not dw[:-1].any()
+
+
+@pytest.mark.gpu
+def test_crowded_experts_captured(dev):
+    """one captured pass replayed for even, crowded and missing rows in turn: the eager bits"""
+    M, E = 70000, 300
+    g = torch.Generator().manual_seed(23)
+    x, dy = torch.randn(M, 24, generator=g).to(dev), torch.randn(M, 40, generator=g).to(dev)
+    w = torch.randn(E, 40, 24, generator=g).to(dev).requires_grad_(True)
+    b = torch.randn(E, 40, generator=g).to(dev).requires_grad_(True)
+    kinds = [lengths(M, E, kind, 5).to(torch.int32).to(dev) for kind in ("even", "one", "ragged", "nobody", "one")]
+    offsets = kinds[0].clone()
+    step = lambda: torch.autograd.grad(experts.expert_linear(x, w, b, offsets), [w, b], dy)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for o in kinds:
+        offsets.copy_(o)
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in out]
+        assert all(torch.equal(a, r) for a, r in zip(kept, step()))
