@@ -828,3 +828,27 @@ def test_sparse_record_exchange_gloo_world2(tmp_path, world):
                         "--master-port", "29747", str(script)], capture_output=True, text=True, env=env, timeout=300)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-3000:]
     assert r.stdout.count("ok") == world
+
+
+def test_traffic_of_launches_over_parts_is_refused(tmp_path):
+    """tools/pmc_traffic.py averages a counter over a kernel's launches: a summary in which the accumulation was launched over parts of the table
+    as well (more launches than the binning had) gives no figure"""
+    def summary(added):
+        lines = ["src_sha16=0123456789abcdef"]
+        for counter in ("FETCH_SIZE", "WRITE_SIZE"):
+            lines.append(f"== pass: --pmc {counter} (rc=0)")
+            for name, launches, avg in (("main_fwd_kernel", 31, 10.0), ("bin_kernel<2, false, 3>", 31, 20.0), ("accumulate_kernel<2>", added, 30.0)):
+                lines += [f"void (anonymous namespace)::{name}(float const*, floa", f"    {counter:36s} launches {launches:4d}  avg {avg:18.1f}"]
+        path = tmp_path / f"summary_{added}.txt"
+        path.write_text("\n".join(lines) + "\n")
+        return path
+
+    out = tmp_path / "traffic.json"
+    run = lambda path: subprocess.run([sys.executable, os.path.join(ROOT, "tools", "pmc_traffic.py"), str(path), str(out)],  # noqa: E731
+                                      capture_output=True, text=True, timeout=120)
+    r = run(summary(55))
+    assert r.returncode != 0 and "part of the table" in r.stderr and not out.exists()
+    r = run(summary(31))
+    assert r.returncode == 0, r.stderr[-500:]
+    got = json.loads(out.read_text())
+    assert got["kernels"]["accumulate_kernel"]["hbm_bytes_per_launch"] == (2 * 30 + 30) * 1024

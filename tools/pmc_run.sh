@@ -3,6 +3,7 @@
 #   gpurun -- 'bash tools/pmc_run.sh [tag] [bench args]'  ->  gpurun_out/pmc_summary_<tag>.txt
 TAG=${1:-dev}; shift
 cd /tmp && export TMPDIR=/tmp && cd $GRAFT_REPO_ROOT
+export PRESIGHT_NO_DRY_OVERLAP=1  # (counters of the plain step: the dry run of the overlapped exchange launches kernels over parts of the table)
 mkdir -p gpurun_out /tmp/pmc
 KERN="main_bwd,main_fwd,accumulate_kernel,bin_kernel,grid_encode,prop_bwd_kernel,prop_fwd_kernel,composite,absmax,adam,grid4,flow_,blend_,route,voxel,points,interlevel,per_ray"
 OUT=gpurun_out/pmc_summary_$TAG.txt

@@ -1,7 +1,9 @@
 """profiles/traffic.json from a PMC summary (tools/pmc_run.sh): HBM bytes per launch of the dominant kernels =
 2 x FETCH_SIZE (gfx950: the counter reports half the bytes of 16-byte streaming reads, MI355X_MICROARCH.md) + WRITE_SIZE,
 both in KB, stamped with the hash of the kernel sources they were measured on (bench.py drops a stale figure).
-    python tools/pmc_traffic.py gpurun_out/pmc_summary_<tag>.txt profiles/traffic.json"""
+    python tools/pmc_traffic.py gpurun_out/pmc_summary_<tag>.txt profiles/traffic.json
+A summary in which a kernel's launches are not all whole ones (the dry run of the overlapped exchange accumulates the main table in pieces:
+one bin_kernel launch, several accumulate_kernel launches) is refused: an average over them is no launch's traffic."""
 import json
 import os
 import re
@@ -11,7 +13,7 @@ sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
 import bench
 
 src, dst = sys.argv[1], sys.argv[2]
-cur, data, sha = None, {}, None
+cur, data, counts, sha = None, {}, {}, None
 for line in open(src):
     if line.startswith("src_sha16="):
         sha = line.strip().split("=", 1)[1]
@@ -19,8 +21,14 @@ for line in open(src):
     m = re.match(r"\s+(\S+)\s+launches\s+(\d+)\s+avg\s+([\d.]+)", line)
     if m and cur:
         data.setdefault(cur, {})[m.group(1)] = float(m.group(3))
+        counts.setdefault(cur, {})[m.group(1)] = int(m.group(2))
     elif not line.startswith(" ") and not line.startswith("=="):
         cur = line.strip()
+for counter in ("FETCH_SIZE", "WRITE_SIZE"):  # one accumulate launch per bin launch
+    binned, added = ({c[counter] for k, c in counts.items() if pat in k and counter in c} for pat in ("bin_kernel<2", "accumulate_kernel<2"))
+    if binned != added:
+        sys.exit(f"{src}: {counter} of {sorted(added)} launches of accumulate_kernel<2> for {sorted(binned)} of bin_kernel<2>: some cover a part of "
+                 "the table only (collect with PRESIGHT_NO_DRY_OVERLAP=1 and --no-secondary)")
 out = {}
 for key, pat in (("main_fwd_kernel", "main_fwd_kernel"), ("main_bwd_sem_kernel", "main_bwd_sem_kernel"), ("main_bwd_rgb_kernel", "main_bwd_rgb_kernel"),
                  ("main_bwd_base_kernel", "main_bwd_base_kernel")):
