@@ -320,8 +320,10 @@ def _matrices(t: torch.Tensor, name: str) -> Tuple[int, int, int]:
 def newton_schulz(g: torch.Tensor, steps: int = 5, coefficients: Tuple[float, float, float] = NS_COEFFICIENTS, eps: float = 1e-7) -> torch.Tensor:
     """g [..., m, n] in fp32, fp16 or bf16 -> a tensor of its shape and type: every matrix scaled to X = G / (||G||_F + eps) and taken
     `steps` times through X <- a X + (b S + c S S) X with S = X X^T: its singular vectors kept, its singular values moved towards one.
-    Matrices of more than 64 rows and columns are held as fp16 pairs: 22 bits of every entry, and what lies below 2^-27 of the matrix' norm to
-    2^-49 of it; smaller ones in fp32.  Sums in fp32, one rounding at the end.  A zero matrix stays zero; a matrix with an infinite or
+    A matrix with a short side up to 64 is computed in fp32 where a workgroup's memory holds it (and it is not long, one of few); others as
+    fp16 pairs: 22 bits of every entry, and what lies below 2^-27 of the matrix' norm to 2^-49 of it.  Sums in fp32, one rounding at the
+    end.  The way and the tiles that a matrix takes go by its shape and by how many the stack holds: the same matrix may differ in its last bits
+    between stacks of different length.  A zero matrix stays zero; a matrix with an infinite or
     undefined entry becomes undefined, without touching the others of the stack.  Not differentiable."""
     args = _ns_args(steps, tuple(coefficients), eps)
     code = _typed(_gpu(g, "g"), "g")
@@ -370,8 +372,8 @@ class HipMuon:
            "rms": 0.2 * sqrt(max(out, in)), an update of the size Adam's has (its learning rates carry over).
     Parameters are contiguous fp32; one without a gradient is skipped, its momentum included.  lr may be changed between steps; a captured
     step keeps the lr, weight_decay and set of parameters it was captured with.
-    Gradients held by a FlatGrads are read where it keeps them (a parameter counts as without a gradient until the backward pass has
-    reached it); parameters of its device-decided groups and gradients of its sharded exchange (a rank has its shard of a matrix only) are
+    Gradients held by a FlatGrads are read where it keeps them (a parameter counts as without a gradient from its zero_() until the backward
+    pass has reached it; a step that is captured is captured together with that pass, whose side streams it waits for); parameters of its device-decided groups and gradients of its sharded exchange (a rank has its shard of a matrix only) are
     refused."""
 
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,

@@ -619,3 +619,56 @@ def test_an_outlier_in_a_stack_of_large_tiles(dev):
     ref = iterate(x.to(dev).double()).cpu()
     for got, want in zip(y, ref):  # (the same four kinds again: 16 units of the norm or four times what plain fp32 is off by, 2e-6 of it)
         assert float((got.double() - want).norm()) <= 8e-6 * float(want.norm())
+
+
+# ------------------------------------------------------------------------------------------------ a layer's gradients and the step on them
+@pytest.mark.gpu
+def test_a_layer_and_its_step_apart(dev):
+    """the gradients of two expert layers against 64 bits, bounded by the sums of absolute values they are made of, and the step against the
+    definition on those very gradients"""
+    from presight_amd import experts
+
+    g = torch.Generator().manual_seed(24)
+    N, k, E, D, H = 700, 2, 5, 72, 96
+    ids = torch.randint(-1, E, (N, k), generator=g)
+    x, gates, dy = torch.randn(N, D, generator=g), torch.rand(N, k, generator=g), torch.randn(N, D, generator=g)
+    start = [torch.randn(E, H, D, generator=g) / D ** 0.5, torch.randn(E, D, H, generator=g) / H ** 0.5]
+    params = [torch.nn.Parameter(t.to(dev)) for t in start]
+    opt = optim.HipMuon(params, lr=0.02, weight_decay=0.01)
+    plan = experts.expert_plan(ids.to(dev), E)
+    a = experts.expert_linear(experts.expert_dispatch(x.to(dev), plan), params[0], None, plan)
+    h = torch.relu(a)
+    experts.expert_combine(experts.expert_linear(h, params[1], None, plan), gates.to(dev), plan).backward(dy.to(dev))
+    opt.step()
+    # (which hidden values are cut off is taken from the rows as they came: next to zero a rounding decides it)
+    open_ = (a.detach() > 0).cpu()
+    place, off = plan.dst.cpu().long(), plan.offsets.tolist()
+    src = plan.src.cpu().long()
+    for size in (lambda t: t, torch.abs):  # the gradients, and the sums of their terms' absolute values
+        xs, w1, w2 = size(x.double()), size(start[0].double()), size(start[1].double())
+        grads = [torch.zeros_like(w1), torch.zeros_like(w2)]
+        for e in range(E):
+            rows = slice(off[e], off[e + 1])
+            f = src[rows]
+            d = size(dy.double())[f // k] * gates.double().reshape(-1)[f][:, None]
+            hid = (xs[f // k] @ w1[e].T) * open_[rows]
+            grads[1][e] = d.T @ hid
+            grads[0][e] = ((d @ w2[e]) * open_[rows]).T @ xs[f // k]
+        if size is torch.abs:
+            sums = grads
+        else:
+            ref = grads
+    terms = D + H + int(max(b - a for a, b in zip(off, off[1:]))) + 70
+    for p, want, absum, w in zip(params, ref, sums, start):
+        assert ((p.grad.cpu().double() - want).abs() <= terms * 2.0 ** -23 * absum).all()
+        grad = p.grad.cpu()
+        buf = (1 - 0.95) * grad
+        u = 0.95 * buf + (1 - 0.95) * grad
+        y = iterate(u.double())
+        off_by = torch.maximum(4 * norms(iterate(u).double() - y), 16 * 2.0 ** -24 * norms(y))  # (of check(), per matrix)
+        rate = 0.02 * math.sqrt(max(1.0, w.shape[1] / w.shape[2]))
+        new = (1 - 0.02 * 0.01) * w.double() - rate * y
+        # (u is the same bits here and there; the parameter carries the roundings of keep, of rate and of its two operations)
+        slack = rate * off_by + 4 * 2.0 ** -24 * (norms(w) + rate * norms(y))
+        assert (norms(p.detach().cpu().double() - new) <= slack).all()
+    assert int((place >= 0).sum()) == off[-1]
