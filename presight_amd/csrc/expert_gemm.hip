@@ -26,8 +26,8 @@ __host__ __device__ inline int64_t row_tiles_at_most(int64_t M, int E, int piece
 // ... and those of more than `above` rows: one piece more than its share for each, of M / (above + 1) at most
 __host__ __device__ inline int64_t crowded_pieces_at_most(int64_t M, int above) { return 2 * (M / above); }
 
-// The tiles of `piece` rows that the experts' rows make (above > 0: pieces of `above` rows, of the experts with more than that): a prefix sum over the lanes, each with its share of neighbouring experts, and a second
-// one over the experts of the lane that holds the tile, where it has several.  (64 experts after the other instead, and a workgroup per
+// The tiles of `piece` rows that the experts' rows make (above > 0: pieces of `above` rows, of the experts with more than that): a prefix sum over
+// the lanes, each with its share of neighbouring experts, and a second one over the experts of the lane that holds the tile, where it has several.  (64 experts after the other instead, and a workgroup per
 // expert whether it can have rows or not: 16 rows of 256 experts, 1024 x 2048 bf16, 30.7 us for 14.9; 8192 of 1024, 256 x 512, 157 for 80.)
 struct RowTiles {
   const int* offsets;
@@ -211,8 +211,9 @@ __device__ __forceinline__ void store_tile_rows(f32x4 (&acc)[MI][NJ], char* slic
 
 // What bounds it depends on the rows per expert.  16 rows of 16 experts' 1024 x 2048 bf16: the weights' 67 MB, 13.4 us, 5.0 TB/s.  131072 rows of 64
 // fp32, 16 experts: the rows' 67 MB and the launch, 21 us.  65536 rows, 2048 x 1024 bf16, 32 experts: the compute units' reads from the
-// L2 and the power limit (a tenth less time on zeros): 300 us forward, 306 for the input gradient, 916 and 898 TFLOP/s.  (The experts' last,
-// incomplete tiles in a round of their own behind the whole ones, and lines fetched into the L2 two to eight steps of k ahead, were slower.)
+// L2 and the power limit (a tenth less time on zeros), and the experts' last, incomplete tiles: 302 us forward, 310 for the input gradient, 910 and
+// 887 TFLOP/s; 286 and 295 where every expert has 2048 rows.  (Those tiles in a round of their own behind the whole ones, and lines fetched into
+// the L2 two to eight steps of k ahead, were slower.)
 // y[p] = sum_k x[p][k] W(n,k) (+ bias).  W_RC = false: the weight's rows are k-contiguous (forward), n of them; true: n-contiguous (input
 // gradient), `w_rows` of them.  K: the rows' length in whole chunks.
 // SHARED: k is shared out over `parts` workgroups per tile, whose fp32 sums go to y [parts][M][N]; linear_join_kernel adds them up in order.
@@ -579,8 +580,9 @@ struct DwPlan {
 };
 // The cheapest by the tiles' steps.  Pieces shorten the longest run of steps and cost 5 us and the way of their fp32 sums through the memory,
 // 4.5 TB/s; without them an expert may well have twice its share of the rows.  Where one that had them all would keep its compute units busy for
-// more than 150 us (a router that has collapsed), those with more than four times their share, and 2048 rows, are cut all the same: a launch
-// more, which finds nothing to join as a rule.  No sum is then longer than that, and no longer than 150 us of steps otherwise.
+// more than 150 us (a router that has collapsed), those with more than four times their share, 2048 rows, and what it takes of all rows for two
+// workgroups per compute unit, are cut all the same: a launch more, which finds nothing to join as a rule, and room for half as many sums as there
+// are experts, or as 1024 tiles hold, at most.  No sum is then longer than that, and no longer than 150 us of steps otherwise.
 //     evenly shared / all rows to one expert, cut and not:  131072 rows, 1024 experts of 64 x 64 fp32 24 / 75 us, 20 / 4090 | 65536, 128 of 256 x 256
 //     fp32 92 / 191, 84 / 5566 | 65536, 32 of 2048 x 1024 bf16 277 / 298, 275 / 1769 | 16384, 8 of 1024 x 1024 bf16 43 / 107, 43 / 225
 //     16 experts, fp32:  131072 rows of 64 x 64 in pieces 22 us, whole 191 | 32768 rows of 128 x 128 in pieces, tiles of 64 21, of 128 30
@@ -605,7 +607,8 @@ DwPlan dw_plan(int64_t M, int E, int64_t n_in, int64_t n_out, int dtype) {
         p = {kPieces, tile, (int)rows, row_tiles_at_most(M, E, (int)rows)};
         more = 5.0 + 8e-6 / 4.5 * p.units * n_in * n_out;
       } else if (cost.least[i] * (double)((M + step_rows - 1) / step_rows) > 150.0) {
-        const int64_t share = ((M + E - 1) / E * 4 + 63) & ~(int64_t)63, most = share < 2048 ? 2048 : share;
+        const double share = 4.0 * (double)M / E, full = (double)M * tiles / (2 * kCompute);
+        const int64_t most = ((int64_t)(share > full ? (share > 2048 ? share : 2048) : (full > 2048 ? full : 2048)) + 63) & ~(int64_t)63;
         if (most < M) p = {kCrowded, tile, (int)most, crowded_pieces_at_most(M, (int)most)}, more = 3.0;
       }
       const double shared = tiles * (pieces > 1 ? (double)M / rows + 0.5 * E : (double)E) / kCompute;  // workgroups per compute unit

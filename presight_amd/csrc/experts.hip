@@ -6,9 +6,10 @@
 //     dispatch   rows[dst[n,j]] = x[n]                              gradient   dx[n] = sum_j drows[dst[n,j]]      (= combine, w = 1)
 //     combine    y[n] = sum_j w[n,j] * rows[dst[n,j]]               gradient   drows[dst[n,j]] = w[n,j] * dy[n],  dw[n,j] = <dy[n], rows[dst[n,j]]>
 // All four run over n: x / dy / y are streamed once in order, the k sorted rows are touched as whole rows.  Nothing is computed that
-// is not moved, so all of them are bound by HBM.  16384 rows to 8 of 128 experts each, 2048 bf16 features (a large copy reaches 4.9 TB/s):
-//     dispatch 604 MB 119 us, 5.1 TB/s | combine 604 MB 127 us, 4.7 TB/s | combine's gradients 1141 MB 245 us, 4.7 TB/s |
-//     the plan of 131072 assignments 14 us
+// is not moved, so all of them are bound by HBM.  16384 rows to 8 of 128 experts each, 2048 bf16 features (a large copy reaches 4.9 TB/s),
+// one behind the other as a training pass has them, and each repeated by itself:
+//     dispatch 604 MB 99 us, 6.1 TB/s, and 118 | combine 604 MB 152 us, 4.0 TB/s, and 123 | combine's gradients 1141 MB 245 us, 4.7 TB/s |
+//     the plan of 131072 assignments 15 us
 // One row after the other, each fetched whole, is best: four or eight rows of an assignment's at once were a tenth to a half slower.
 // 65536 rows to 2 of 16, 64 fp32 features: 10 us and less for 50 MB, 17 us for 84; one row: 2 us each and 4 for its plan, all latency.
 #include "common.hpp"
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count_kernel(const void* __
   for (int e = threadIdx.x; e < E; e += kPlanThreads) hist[(int64_t)blockIdx.x * E + e] = cnt[e];
 }
 
-// 131072 assignments: 4 us to count and 9 to place them, neither near a limit of the memory: a workgroup's two passes over its ids, the
+// 131072 assignments: 5 us to count and 10 to place them, neither near a limit of the memory: a workgroup's two passes over its ids, the
 // second one's ranks, and the scans between them wait for each other.
 // One workgroup places the assignments [f0, f0 + chunk).  Each wave owns a contiguous run of them and counts it by itself (cnt[wave][e],
 // ballots instead of atomics: the rank inside a 64-wide round is a popcount), the counts become first places by a scan over waves, the

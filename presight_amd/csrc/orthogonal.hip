@@ -103,7 +103,7 @@ __device__ __forceinline__ void source_pack(const Source& src, int64_t i, int64_
   if constexpr (MOMENTUM && UPDATE) store_any(src.buf + i, b);
 }
 
-// 2048 x 4096 fp32: 11 us for 34 MB; with the momentum, 8 x 1024 x 2048: 35 us for 201 MB (5.7 TB/s, some of it from the last-level cache).
+// 2048 x 4096 fp32: 13 us for 34 MB; with the momentum, 8 x 1024 x 2048: 35 us for 201 MB (5.7 TB/s, some of it from the last-level cache).
 // partial sums of squares, in 64 bits: entries of any fp32 size neither overflow nor vanish
 template <typename T, bool MOMENTUM>
 __global__ __launch_bounds__(256) void ns_norm_kernel(Source src, int64_t size, Work w) {
@@ -135,7 +135,7 @@ __device__ __forceinline__ float ratio_at(float r, int i, float grow) {
   return r;
 }
 
-// 2048 x 4096 fp32: 25 us for 67 MB; 8 x 1024 x 2048 with the momentum: 45 us for 201 MB.
+// 2048 x 4096 fp32: 25 us for 67 MB; 8 x 1024 x 2048 with the momentum: 48 us for 201 MB.
 // X^ = G / norm as pairs [s][2 lp], 64 x 64 elements at a time (turned in LDS where G is tall); zeros in the padding
 template <typename T, bool MOMENTUM>
 __global__ __launch_bounds__(256) void ns_start_kernel(Source src, Shape h, Work w, float eps) {
@@ -206,8 +206,8 @@ struct Operands {  // pairs
 // rate 256 x 128 asks for 32 bytes per cycle, 128 x 128 for 43 and 64 x 64 for 85, and a step of k takes as long as its stage of 48, 32 or
 // 16 KiB takes to arrive.  The two small products add up apart from the large one: each of their additions to it would cost it another rounding.
 //
-// 2048 x 4096: S 89 us, a I + b S + c S S 57, times X 97: 580, 452 and 1063 TFLOP/s of pairs' products (half of S and S S by symmetry, three
-// products per pair), where a large fp16 product reaches 1463; 8 x 1024 x 2048: 86, 64 and 106 us.  A few tiles:
+// 2048 x 4096: S 90 us, a I + b S + c S S 57, times X 99: 573, 452 and 1041 TFLOP/s of pairs' products (half of S and S S by symmetry, three
+// products per pair), where a large fp16 product reaches 1463; 8 x 1024 x 2048: 87, 64 and 107 us.  A few tiles:
 // 3 x 385 x 129 takes 7 to 9 us a product, most of it the launch, the first loads from memory that another XCD wrote, and the way out.
 //
 // The result leaves through LDS as rows of whole lines.  Of a symmetric one only what lies on and below the diagonal's BN x BN blocks is

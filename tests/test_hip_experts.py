@@ -698,6 +698,7 @@ def test_weight_gradients_of_many_experts_make_room_for_a_crowded_one():
     # room for two pieces of 2048 rows, or of four times the even share, for every one that fits the rows; 64 more sums for the bias
     assert need(131072, 1024, 64, 64, 0) == 2 * 64 * (64 * 64 + 64) * 4
     assert need(65536, 32, 2048, 1024, 2) == 2 * 8 * (2048 * 1024 + 1024) * 4
+    assert need(1 << 20, 512, 2048, 2048, 2) < 1 << 29  # (large weights: no more pieces than fill the chip)
     assert need(2048, 16, 64, 64, 0) == need(5000, 64, 512, 512, 2) == 0  # (short whoever has them)
 
 
