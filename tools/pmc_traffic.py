@@ -1,7 +1,7 @@
 """profiles/traffic.json from a PMC summary (tools/pmc_run.sh): HBM bytes per launch of the dominant kernels =
 2 x FETCH_SIZE (gfx950: the counter reports half the bytes of 16-byte streaming reads, MI355X_MICROARCH.md) + WRITE_SIZE,
 both in KB, stamped with the hash of the kernel sources they were measured on (bench.py drops a stale figure).
-    python tools/pmc_traffic.py gpurun_out/pmc_summary_<tag>.txt profiles/traffic.json
+    python tools/pmc_traffic.py pmc_summary_<tag>.txt profiles/traffic.json
 A summary in which a kernel's launches are not all whole ones (the dry run of the overlapped exchange accumulates the main table in pieces:
 one bin_kernel launch, several accumulate_kernel launches) is refused: an average over them is no launch's traffic."""
 import json
